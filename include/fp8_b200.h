@@ -258,6 +258,87 @@ int fp8b200_gemm_16bit(const void *A, const void *B, int dtype, int64_t lda, int
                        void *stream);
 
 /*
+ * ---- Serving from a paged key/value cache (no counterpart in the reference,
+ * which has no cache and no attention).
+ * A cache is a pool of `pages` pages of page_size slots of n_kv_heads x
+ * head_dim values; token j of request r sits in slot j % page_size of page
+ * block_table[r][j / page_size].
+ */
+
+/*
+ * Page allotment and token placement of one step, from device-resident
+ * request lengths, in one launch. With have_r = ceil(cached_r / page_size) and
+ * add_r = ceil((cached_r + new_r) / page_size) - have_r, the new pages of the
+ * requests are taken in order from free_pages[free_head ..]:
+ *   block_table[r][have_r + i] = free_pages[free_head + base_r + i], i < add_r,
+ *                                base_r = sum of add over the requests before r
+ *                                (-1 once the list is used up)
+ *   cu_new[r] = sum of new over the requests before r (requests + 1 values)
+ *   kv_lens[r] = cached_r + new_r
+ *   token t of request r: positions[t] = cached_r + t - cu_new[r], slots[t] =
+ *     page * page_size + position % page_size, -1 where it has no page
+ *   tokens from cu_new[requests] on: position 0, slot -1
+ *   free_head_out[0] = free_head + sum of add (beyond n_free: the pool is short)
+ * `tokens`: rows of positions / slots, at least the sum of new. free_head may
+ * be NULL (0). Lengths below zero count as zero. At most 16384 requests; sums
+ * of lengths below 2^31.
+ */
+int fp8b200_paged_slots(const int32_t *cached_lens, const int32_t *new_lens, int64_t requests,
+                        int32_t *block_table, int64_t table_ld, int64_t table_cols,
+                        const int32_t *free_pages, int64_t n_free, const int32_t *free_head, int64_t page_size,
+                        int64_t tokens, int32_t *cu_new, int32_t *kv_lens, int32_t *positions,
+                        int64_t *slots, int32_t *free_head_out, void *stream);
+
+/*
+ * Rotary embedding of a step's q and k and the write of its k and v into the
+ * paged cache, in one pass over the fused projection. qkv: tokens x ld of
+ * `dtype` (BF16 / F16), row t holding n_q_heads q, n_kv_heads k and n_kv_heads
+ * v heads of head_dim values (a multiple of 16). cos / sin tables: table_rows
+ * x head_dim/2 float32, row positions[t] for token t; a position outside them
+ * gives NaN. (a, b) -> (a cos - b sin, b cos + a sin) over the head's halves in
+ * float32, one rounding at the end. q_out: tokens x n_q_heads x head_dim,
+ * contiguous. The caches hold qkv's type, or E4M3 / E5M2 codes of value /
+ * scale, saturated at the largest finite value (NaN stays NaN); strides in
+ * elements, multiples of 8. k_scale / v_scale: float32, one value (step 0) or
+ * one per head (step 1), NULL for 1. A token whose slot is outside the pool is
+ * not written; slots must be distinct.
+ */
+int fp8b200_rope_write_paged(const void *qkv, int dtype, int64_t tokens, int64_t ld, int n_q_heads,
+                             int n_kv_heads, int head_dim, const float *cos_table, const float *sin_table,
+                             int64_t table_rows, const int32_t *positions, const int64_t *slots, void *q_out,
+                             void *k_cache, void *v_cache, int cache_dtype, int64_t pages, int64_t page_size,
+                             int64_t stride_page, int64_t stride_slot, int64_t stride_head,
+                             const float *k_scale, int k_scale_step, const float *v_scale, int v_scale_step,
+                             void *stream);
+
+/*
+ * Causal attention of each request's new tokens over its pages. Request r's
+ * queries are rows cu_new[r] .. cu_new[r+1] of q (offsets clipped to `tokens`),
+ * the last at position kv_lens[r] - 1; a query at position p sees key j where
+ * j <= p and (window == 0 or p - j < window or j < sinks). Query head h reads
+ * key/value head h / (n_q_heads / n_kv_heads). out = softmax(scale * q k^T) v;
+ * a query that sees nothing (or only scores of -inf) gives 0. A table entry
+ * outside the pool hides its keys. Rows of no request are left as they were, or
+ * set to 0 with zero_rest.
+ * q / out: BF16 or F16, strides in elements, multiples of 8; the caches as
+ * fp8b200_rope_write_paged leaves them, strides multiples of 16 bytes.
+ * head_dim: a multiple of 16 up to 256. max_new: the most new tokens of a
+ * request if the host knows (0: not known); it picks the kernels, a wrong value
+ * costs time but not results. workspace: fp8b200_paged_attention_workspace(head_dim)
+ * bytes that no other call uses at the same time.
+ */
+int64_t fp8b200_paged_attention_workspace(int head_dim);
+int fp8b200_paged_attention(const void *q, int dtype, int64_t q_stride_token, int64_t q_stride_head,
+                            int64_t tokens, int n_q_heads, int n_kv_heads, int head_dim, const void *k_cache,
+                            const void *v_cache, int cache_dtype, int64_t pages, int64_t page_size,
+                            int64_t stride_page, int64_t stride_slot, int64_t stride_head,
+                            const int32_t *block_table, int64_t table_ld, int64_t table_cols,
+                            const int32_t *cu_new, const int32_t *kv_lens, int64_t requests, float scale,
+                            const float *k_scale, int k_scale_step, const float *v_scale, int v_scale_step,
+                            int window, int sinks, int64_t max_new, void *out, int64_t out_stride_token,
+                            int64_t out_stride_head, int zero_rest, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
  * Device-side status of the scaled GEMM on the current device: 0 if no
  * bounded wait has timed out, else FP8B200_ETIMEOUT with *status_out holding
  * the site code of the last launch that timed out (that launch's output is

@@ -1,0 +1,199 @@
+// Shared pieces of the paged attention kernels.
+#pragma once
+
+#include "common.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace fp8b200 {
+namespace paged {
+
+// One call. Element strides throughout; the two caches share their strides.
+struct AttnParams {
+  const uint16_t *q;
+  int64_t q_tok, q_head;
+  uint16_t *out;
+  int64_t o_tok, o_head;
+  const uint8_t *k, *v;
+  int64_t s_page, s_slot, s_head;
+  int64_t pages;
+  int page;
+  const int32_t *table;
+  int64_t table_ld;
+  int table_cols;
+  const int32_t *cu, *kv;
+  int requests;
+  int tokens;                 // rows of q
+  int hq, hk, group, d;
+  float scale_log2;           // softmax scale times log2(e)
+  const float *ks, *vs;
+  int ks_step, vs_step;       // 0: one scale, 1: one per head
+  int window, sinks;          // window 0: none
+  int zero_rest;              // zero the rows of out that belong to no request
+  int rows_over, rows_upto;   // requests whose query rows (tokens x group) lie in (rows_over, rows_upto] are taken
+  // split segments: partial results and which block continues what
+  float *part;
+  int4 *desc;
+};
+
+// The new tokens of request r: rows [start, start + n) of q, the last at
+// position kv - 1. Offsets outside q's rows are clipped, so no row is read or
+// written behind it.
+struct Request {
+  int start, n, first;        // first: position of row `start`, negative where kv < n
+};
+__device__ __forceinline__ Request load_request(const AttnParams &p, int r) {
+  Request q;
+  const int a = min(max(__ldg(p.cu + r), 0), p.tokens), b = min(max(__ldg(p.cu + r + 1), a), p.tokens);
+  const int kv = max(__ldg(p.kv + r), 0);
+  q.start = a;
+  q.n = b - a;
+  q.first = kv - q.n;
+  return q;
+}
+__device__ __forceinline__ bool takes(const AttnParams &p, int n) {
+  const int64_t rows = (int64_t)n * p.group;
+  return rows > p.rows_over && rows <= p.rows_upto;
+}
+
+// Zeros to the rows of out that no request has (a padded batch), by blocks
+// [block, blocks) of the launch.
+__device__ __forceinline__ void zero_rest(const AttnParams &p, int block, int blocks) {
+  const int a = min(max(__ldg(p.cu), 0), p.tokens);
+  const int b = p.requests > 0 ? min(max(__ldg(p.cu + p.requests), a), p.tokens) : a;
+  const int rest = a + p.tokens - b, units = p.hq * (p.d / 8);
+  for (int i = block; i < rest; i += blocks) {
+    const int row = i < a ? i : b + i - a;
+    for (int u = threadIdx.x; u < units; u += blockDim.x) {
+      const int head = u / (p.d / 8), c = u - head * (p.d / 8);
+      *reinterpret_cast<uint4 *>(p.out + (int64_t)row * p.o_tok + (int64_t)head * p.o_head + c * 8) = make_uint4(0, 0, 0, 0);
+    }
+  }
+}
+
+// Key tiles that any query at positions [lo, hi] can see: the tiles of the
+// sinks, [0, sinks), and those of the windows, [from, to).
+template <int BN>
+struct Tiles {
+  int sinks, from, to;
+  __device__ __forceinline__ int count() const { return sinks + to - from; }
+  __device__ __forceinline__ int at(int i) const { return i < sinks ? i : from + i - sinks; }
+};
+template <int BN>
+__device__ __forceinline__ Tiles<BN> visible_tiles(const AttnParams &p, int lo, int hi) {
+  Tiles<BN> t;
+  // keys behind the last table column have no page
+  const int64_t cap = (int64_t)p.table_cols * p.page;
+  const int end = hi < 0 ? 0 : (int)min((int64_t)hi + 1, cap);
+  t.to = (int)(((int64_t)end + BN - 1) / BN);
+  t.from = 0;
+  t.sinks = 0;
+  if (p.window > 0 && end > 0) {
+    const int64_t first = (int64_t)max(lo, 0) - p.window + 1;
+    if (first > 0) t.from = min((int)(first / BN), t.to);
+    t.sinks = (int)min(((int64_t)p.sinks + BN - 1) / BN, (int64_t)t.from);
+  }
+  return t;
+}
+__device__ __forceinline__ bool visible(const AttnParams &p, int key, int pos) {
+  return key <= pos && (p.window <= 0 || pos - key < p.window || key < p.sinks);
+}
+
+// Element offset of key j's slot in the pool, -1 where it has no page: a
+// table entry outside the pool hides its keys.
+__device__ __forceinline__ int64_t slot_offset(const AttnParams &p, int r, int j) {
+  const uint32_t col = (uint32_t)j / (uint32_t)p.page;
+  if (col >= (uint32_t)p.table_cols) return -1;
+  const int page = __ldg(p.table + (int64_t)r * p.table_ld + col);
+  if (page < 0 || page >= p.pages) return -1;
+  return (int64_t)page * p.s_page + (int64_t)((uint32_t)j - col * (uint32_t)p.page) * p.s_slot;
+}
+
+__device__ __forceinline__ uint32_t saddr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool F16>
+__device__ __forceinline__ float to_f32(uint16_t v) {
+  if constexpr (F16) return __half2float(__ushort_as_half(v));
+  else return u2f((uint32_t)v << 16);
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (F16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+}
+// Two float8 codes (low 16 bits) to a half pair: exact, infinities and NaN kept.
+template <int KV>
+__device__ __forceinline__ uint32_t fp8x2_to_f16x2(uint32_t two) {
+  uint32_t h;
+  const uint16_t in = (uint16_t)two;
+  if constexpr (KV == FP8B200_E4M3) asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(in));
+  else asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(h) : "h"(in));
+  return h;
+}
+// One cached value as float (KV: E4M3, E5M2, or the 16-bit type).
+template <bool F16, int KV>
+__device__ __forceinline__ float cache_value(const uint8_t *base, int64_t elem) {
+  if constexpr (KV == FP8B200_E4M3 || KV == FP8B200_E5M2)
+    return __half2float(__ushort_as_half((uint16_t)fp8x2_to_f16x2<KV>(__ldg(base + elem))));
+  else
+    return to_f32<F16>(__ldg(reinterpret_cast<const uint16_t *>(base) + elem));
+}
+
+// One query row over the keys of tiles [t0, t1) of `tiles`, value by value:
+// the way out where a hidden key's infinity or NaN met a zero weight in a
+// matrix product (0 * inf). Hidden keys are not touched here. The warp's
+// lanes hold dims lane, lane + 32, ...; returns the running maximum (log2
+// units) and sum, and the unnormalised output in o.
+template <bool F16, int KV, int DMAX, int BN>
+__device__ __noinline__ void careful_row(const AttnParams &p, int r, int tok, int head, int pos, const Tiles<BN> tiles,
+                                         int t0, int t1, float &m_out, float &l_out, float (&o)[DMAX / 32]) {
+  const int lane = threadIdx.x & 31;
+  const int kh = head / p.group;
+  const uint16_t *q = p.q + (int64_t)tok * p.q_tok + (int64_t)head * p.q_head;
+  const float s2 = p.scale_log2 * (p.ks ? __ldg(p.ks + p.ks_step * kh) : 1.0f);
+  float qv[DMAX / 32];
+#pragma unroll
+  for (int i = 0; i < DMAX / 32; i++) {
+    qv[i] = lane + 32 * i < p.d ? to_f32<F16>(__ldg(q + lane + 32 * i)) : 0.0f;
+    o[i] = 0.0f;
+  }
+  float m = -INFINITY, l = 0.0f;
+  for (int t = t0; t < t1; t++) {
+    const int k0 = tiles.at(t) * BN;
+    for (int j = k0; j < k0 + BN; j++) {
+      if (!visible(p, j, pos)) continue;
+      const int64_t off = slot_offset(p, r, j);
+      if (off < 0) continue;
+      const int64_t e = off + (int64_t)kh * p.s_head;
+      float s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < DMAX / 32; i++)
+        if (lane + 32 * i < p.d) s += qv[i] * cache_value<F16, KV>(p.k, e + lane + 32 * i);
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+      s *= s2;
+      const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.0f : mn;
+      const float keep = exp2f(m - base), w = exp2f(s - base);
+      m = mn;
+      l = l * keep + w;
+#pragma unroll
+      for (int i = 0; i < DMAX / 32; i++)
+        if (lane + 32 * i < p.d) o[i] = o[i] * keep + w * cache_value<F16, KV>(p.v, e + lane + 32 * i);
+    }
+  }
+  m_out = m;
+  l_out = l;
+}
+
+}  // namespace paged
+}  // namespace fp8b200

@@ -43,7 +43,7 @@ def dtype_code(dt: torch.dtype) -> int:
 
 
 def _declare(L):
-    vp, i64, i32, u64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_uint64
+    vp, i64, i32, u64, f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_uint64, ctypes.c_float
     L.fp8b200_version.restype = i32
     L.fp8b200_last_error.restype = ctypes.c_char_p
     L.fp8b200_launch_count.restype = u64
@@ -62,6 +62,12 @@ def _declare(L):
                               vp, i32, vp, i32, vp, i32, vp, vp, i32, i64, vp],
         "fp8b200_linear_fp8w": [vp, i32, i64, vp, i32, i64, i64, i64, i64, vp, i32, vp, i32, vp, i32, i64, vp],
         "fp8b200_gemm_16bit": [vp, vp, i32, i64, i64, i64, i64, i64, vp, i32, vp, i32, vp, i32, i64, vp],
+        "fp8b200_paged_slots": [vp, vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp],
+        "fp8b200_rope_write_paged": [vp, i32, i64, i64, i32, i32, i32, vp, vp, i64, vp, vp, vp, vp, vp, i32,
+                                     i64, i64, i64, i64, i64, vp, i32, vp, i32, vp],
+        "fp8b200_paged_attention": [vp, i32, i64, i64, i64, i32, i32, i32, vp, vp, i32, i64, i64, i64, i64, i64,
+                                    vp, i64, i64, vp, vp, i64, f32, vp, i32, vp, i32, i32, i32, i64, vp, i64,
+                                    i64, i32, vp, i64, vp],
         "fp8b200_gemm_status": [ctypes.POINTER(ctypes.c_uint32), i32],
         "fp8b200_debug_gemm": [i32, ctypes.c_ulonglong],
         "fp8b200_gemm_set_path": [i32],
@@ -71,6 +77,8 @@ def _declare(L):
             fn = getattr(L, name)
             fn.argtypes = args
             fn.restype = i32
+    L.fp8b200_paged_attention_workspace.argtypes = [i32]
+    L.fp8b200_paged_attention_workspace.restype = i64
 
 
 def lib():

@@ -12,14 +12,16 @@ current CUDA device, as the reference moves them to "mps".
 Additions beyond the reference (used by the aten overrides in ops.py):
 `encode_fp8` / `decode_fp8` for both fp8 formats and any float dtype,
 `quantize_fp8`, `fp4_decode` (shape-preserving, any float dtype, f32
-scale), `scaled_mm` with torch._scaled_mm's full argument set, and
-`fp4_scaled_mm` (packed FP4 operands multiplied on the tensor cores).
+scale), `scaled_mm` with torch._scaled_mm's full argument set,
+`fp4_scaled_mm` (packed FP4 operands multiplied on the tensor cores), and the
+paged key/value-cache operators of paged.py.
 """
 from __future__ import annotations
 
 import torch
 
 from . import _lib as L
+from .paged import PagedStep, paged_attention, paged_slots, rope_write_paged  # noqa: F401
 
 _FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
 _FLOAT = (torch.float32, torch.bfloat16, torch.float16)

@@ -504,3 +504,57 @@ def fp4_dequantize(input: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
 @fp4_dequantize.register_fake
 def _(input, scale):
     return input.new_empty(input.numel() * 2, dtype=torch.float16)
+
+
+# ------------------------------------------------------------------ paged key/value cache (additions to the reference)
+@torch.library.custom_op("fp8_mps::paged_slots", mutates_args=("block_table",))
+def paged_slots(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                page_size: int, num_tokens: int, free_head: Optional[torch.Tensor] = None
+                ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Page allotment and token placement of one step: (cu_new, kv_lens,
+    positions, slots, free_head); block_table is grown in place."""
+    from fp4_fp8_for_torch_mps.paged import PagedStep, paged_slots as _slots
+
+    def separate(n, t, dev):  # an op's results must not share storage
+        cu, kv, pos, head = (torch.empty(k, dtype=torch.int32, device=dev) for k in (n + 1, n, t, 1))
+        return PagedStep(cu, kv, pos, torch.empty(t, dtype=torch.int64, device=dev), head)
+
+    return tuple(_slots(cached_lens, new_lens, block_table, free_pages, page_size, num_tokens, free_head, separate))
+
+
+@paged_slots.register_fake
+def _(cached_lens, new_lens, block_table, free_pages, page_size, num_tokens, free_head=None):
+    n = cached_lens.shape[0]
+    return (cached_lens.new_empty(n + 1), cached_lens.new_empty(n), cached_lens.new_empty(num_tokens),
+            cached_lens.new_empty(num_tokens, dtype=torch.int64), cached_lens.new_empty(1))
+
+
+@torch.library.custom_op("fp8_mps::rope_write_paged", mutates_args=("k_cache", "v_cache"))
+def rope_write_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                     slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_q_heads: int,
+                     k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Rotary embedding of q and k, and k and v into the paged cache; returns q."""
+    from fp4_fp8_for_torch_mps.paged import rope_write_paged as _write
+    return _write(qkv, cos, sin, positions, slots, k_cache, v_cache, n_q_heads, k_scale, v_scale)
+
+
+@rope_write_paged.register_fake
+def _(qkv, cos, sin, positions, slots, k_cache, v_cache, n_q_heads, k_scale=None, v_scale=None):
+    return qkv.new_empty((qkv.shape[0], n_q_heads, k_cache.shape[3]))
+
+
+@torch.library.custom_op("fp8_mps::paged_attention", mutates_args=())
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    cu_new: torch.Tensor, kv_lens: torch.Tensor, scale: Optional[float] = None, window: int = 0,
+                    sinks: int = 0, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                    max_new: Optional[int] = None) -> torch.Tensor:
+    """Causal attention of each request's new tokens over its pages."""
+    from fp4_fp8_for_torch_mps.paged import paged_attention as _attention
+    return _attention(q, k_cache, v_cache, block_table, cu_new, kv_lens, scale=scale, window=window, sinks=sinks,
+                      k_scale=k_scale, v_scale=v_scale, max_new=max_new)
+
+
+@paged_attention.register_fake
+def _(q, k_cache, v_cache, block_table, cu_new, kv_lens, scale=None, window=0, sinks=0, k_scale=None, v_scale=None,
+      max_new=None):
+    return q.new_empty(q.shape)

@@ -1,0 +1,265 @@
+"""Serving from a paged key/value cache: host launchers.
+
+One step of a batch of requests, each with tokens already cached and new
+tokens to add (one when it decodes, many when it is prefilled):
+
+    step = paged_slots(cached_lens, new_lens, block_table, free_pages, page_size, num_tokens)
+    q = rope_write_paged(qkv, cos, sin, step.positions, step.slots, k_cache, v_cache, n_q_heads)
+    a = paged_attention(q, k_cache, v_cache, block_table, step.cu_new, step.kv_lens)
+
+`paged_slots` runs once a step, the other two once a layer. Everything that
+depends on the lengths stays on the device, so a step can be captured in a
+CUDA graph and replayed with other lengths. A cache is a (pages, page_size,
+kv_heads, head_dim) tensor of the activations' type or of a float8 type; k and
+v caches have the same strides (two tensors, or two views of one).
+
+No counterpart in the reference, which has no cache and no attention.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib as L
+
+_FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
+_16BIT = (torch.bfloat16, torch.float16)
+MAX_REQUESTS = 16384
+
+
+class PagedStep(NamedTuple):
+    """What `paged_slots` lays out for one step."""
+    cu_new: torch.Tensor      # (requests + 1,) int32: first row of each request's new tokens
+    kv_lens: torch.Tensor     # (requests,) int32: cached + new tokens
+    positions: torch.Tensor   # (num_tokens,) int32
+    slots: torch.Tensor       # (num_tokens,) int64: page * page_size + offset, -1 for none
+    free_head: torch.Tensor   # (1,) int32: first free page not taken
+
+
+_workspace_bytes: dict[tuple[int, int], int] = {}
+
+
+def _check(t: torch.Tensor, name: str, what: str, dtype: torch.dtype, dim: int, dev: torch.device) -> None:
+    if t.dtype != dtype or t.dim() != dim:
+        raise RuntimeError(f"{what}: {name} must be a {dim}-D {dtype} tensor, got {t.dim()}-D {t.dtype}")
+    if t.device != dev:
+        raise RuntimeError(f"{what}: {name} is on {t.device}, expected {dev}")
+    if dim == 1 and not t.is_contiguous():
+        raise RuntimeError(f"{what}: {name} must be contiguous")
+
+
+def _check_table(table: torch.Tensor, what: str, dev: torch.device) -> int:
+    """The row stride of a (requests, columns) block table."""
+    _check(table, "block_table", what, torch.int32, 2, dev)
+    n, cols = table.shape
+    ld = table.stride(0) if n > 1 else cols
+    if (n and cols > 1 and table.stride(1) != 1) or ld < cols:
+        raise RuntimeError(f"{what}: block_table rows must be contiguous and not overlap, got strides {table.stride()}")
+    return ld
+
+
+def _check_caches(k: torch.Tensor, v: torch.Tensor, x: torch.Tensor, what: str) -> tuple[int, ...]:
+    """(pages, page_size, kv_heads, head_dim) of two caches that go with x."""
+    if k.dim() != 4 or v.shape != k.shape:
+        raise RuntimeError(f"{what}: k_cache and v_cache must be (pages, page_size, kv_heads, head_dim) tensors of one "
+                           f"shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+    if x.dtype not in _16BIT:
+        raise RuntimeError(f"{what}: activations must be bfloat16 or float16, got {x.dtype}")
+    if v.dtype != k.dtype or (k.dtype != x.dtype and k.dtype not in _FP8):
+        raise RuntimeError(f"{what}: the caches must both be {x.dtype} or both one float8 type, got {k.dtype} and {v.dtype}")
+    if k.device != x.device or v.device != x.device:
+        raise RuntimeError(f"{what}: the caches are on {k.device} and {v.device}, expected {x.device}")
+    if v.stride() != k.stride() or (k.numel() and k.stride(3) != 1):
+        raise RuntimeError(f"{what}: the caches must have the same strides and contiguous heads, got {k.stride()} and {v.stride()}")
+    return tuple(k.shape)
+
+
+def _check_scale(s: torch.Tensor | None, name: str, what: str, cache: torch.Tensor) -> tuple[int | None, int]:
+    """(pointer, step) of a cache scale: one value or one per key/value head."""
+    if s is None:
+        return None, 0
+    if cache.dtype not in _FP8:
+        raise RuntimeError(f"{what}: {name} goes with a float8 cache only")
+    if s.dtype != torch.float32 or s.device != cache.device or s.numel() not in (1, cache.shape[2]) or not s.is_contiguous():
+        raise RuntimeError(f"{what}: {name} must be 1 or {cache.shape[2]} contiguous float32 values on {cache.device}")
+    return s.data_ptr(), 0 if s.numel() == 1 else 1
+
+
+def _launch(dev: torch.device, fn, what: str, *args) -> None:
+    """fn(*args, current stream) on `dev`."""
+    if dev.type != "cuda":
+        raise RuntimeError(f"{what}: tensors must be on a CUDA device, got {dev}")
+    if torch.cuda.current_device() == dev.index:
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        if rc:
+            L.check(rc, what)
+    else:
+        with torch.cuda.device(dev):
+            L.check(fn(*args, torch.cuda.current_stream(dev).cuda_stream), what)
+
+
+def slots_outputs(requests: int, num_tokens: int, dev: torch.device) -> PagedStep:
+    """The tensors of a step, the int32 ones in one allocation."""
+    cu, kv, pos, head = torch.empty(2 * requests + 2 + num_tokens, dtype=torch.int32, device=dev).split(
+        [requests + 1, requests, num_tokens, 1])
+    return PagedStep(cu, kv, pos, torch.empty(num_tokens, dtype=torch.int64, device=dev), head)
+
+
+def paged_slots(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
+                page_size: int, num_tokens: int, free_head: torch.Tensor | None = None,
+                outputs=slots_outputs) -> PagedStep:
+    """Page allotment and token placement of one step, one launch, no host sync.
+
+    cached_lens, new_lens: (requests,) int32, tokens each request holds and
+    adds (0: it pauses). block_table: (requests, columns) int32, row r listing
+    r's pages in order; the new pages' entries are written in place.
+    free_pages: int32 ids of free pages, taken in order of the requests from
+    `free_head` (int32, one value on the device; None: 0) on. num_tokens: rows
+    of the step, at least the sum of new_lens (more in a padded batch: those
+    rows get position 0 and slot -1; fewer: the tokens behind them are not
+    placed, nor the pages that they open). outputs(requests, num_tokens,
+    device) allocates the results.
+
+    Returns a PagedStep. Once the list of free pages is used up, the requests
+    after it get table entries of -1 and slots of -1 (`rope_write_paged` skips
+    them); the returned free_head is then beyond free_pages.numel(). A token
+    beyond the table's columns also gets slot -1. Lengths below zero count as
+    zero; sums of lengths stay below 2^31."""
+    what = "paged_slots"
+    dev = cached_lens.device
+    _check(cached_lens, "cached_lens", what, torch.int32, 1, dev)
+    _check(new_lens, "new_lens", what, torch.int32, 1, dev)
+    _check(free_pages, "free_pages", what, torch.int32, 1, dev)
+    ld = _check_table(block_table, what, dev)
+    n = cached_lens.numel()
+    if new_lens.numel() != n or block_table.shape[0] != n:
+        raise RuntimeError(f"{what}: {n} cached_lens, {new_lens.numel()} new_lens and {block_table.shape[0]} block_table rows")
+    if n > MAX_REQUESTS:
+        raise RuntimeError(f"{what}: {n} requests, at most {MAX_REQUESTS}")
+    if page_size < 1 or num_tokens < 0:
+        raise RuntimeError(f"{what}: page_size={page_size} must be positive and num_tokens={num_tokens} not negative")
+    if free_head is not None and (free_head.dtype != torch.int32 or free_head.numel() != 1 or free_head.device != dev):
+        raise RuntimeError(f"{what}: free_head must be one int32 value on {dev}")
+    step = outputs(n, num_tokens, dev)
+    _launch(dev, L.lib().fp8b200_paged_slots, what, cached_lens.data_ptr(), new_lens.data_ptr(), n,
+            block_table.data_ptr(), ld, block_table.shape[1], free_pages.data_ptr(), free_pages.numel(),
+            None if free_head is None else free_head.data_ptr(), page_size, num_tokens, step.cu_new.data_ptr(),
+            step.kv_lens.data_ptr(), step.positions.data_ptr(), step.slots.data_ptr(), step.free_head.data_ptr())
+    return step
+
+
+def rope_write_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                     slots: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_q_heads: int,
+                     k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary embedding of a step's q and k, and its k and v into the paged
+    cache, in one pass over the fused projection.
+
+    qkv: (tokens, ld) bfloat16 or float16, row t holding n_q_heads q heads and
+    then the k and the v heads (a column slice of a wider tensor is fine).
+    cos, sin: (positions, head_dim / 2) float32 tables, read at positions[t]
+    (int32; outside the tables: NaN). The head's halves (a, b) become
+    (a cos - b sin, b cos + a sin), computed in float32 and rounded once.
+    slots: (tokens,) int64 from paged_slots; a token whose slot is outside the
+    pool is not kept. Slots must differ: of two tokens with one slot either
+    may stay, value by value.
+    k_cache, v_cache: written in place, in qkv's type or as float8 codes of
+    value / scale (k_scale, v_scale: one float32 value or one per head; None:
+    1), saturated at the format's largest finite value; NaN stays NaN.
+    Returns q, (tokens, n_q_heads, head_dim)."""
+    what = "rope_write_paged"
+    dev = qkv.device
+    pages, page, hk, d = _check_caches(k_cache, v_cache, qkv, what)
+    width = (n_q_heads + 2 * hk) * d
+    if qkv.dim() != 2 or n_q_heads < 0 or qkv.shape[1] < width:
+        raise RuntimeError(f"{what}: qkv must be (tokens, at least {width}), got {tuple(qkv.shape)}")
+    t = qkv.shape[0]
+    ld = qkv.stride(0) if t > 1 else width
+    if (t and qkv.stride(1) != 1) or ld < width:
+        raise RuntimeError(f"{what}: qkv rows must be contiguous and not overlap, got strides {qkv.stride()}")
+    _check(cos, "cos", what, torch.float32, 2, dev)
+    _check(sin, "sin", what, torch.float32, 2, dev)
+    if cos.shape != sin.shape or cos.shape[1] * 2 != d or not cos.is_contiguous() or not sin.is_contiguous():
+        raise RuntimeError(f"{what}: cos and sin must be contiguous (positions, {d // 2}) tables, got {tuple(cos.shape)} and "
+                           f"{tuple(sin.shape)}")
+    _check(positions, "positions", what, torch.int32, 1, dev)
+    _check(slots, "slots", what, torch.int64, 1, dev)
+    if positions.numel() != t or slots.numel() != t:
+        raise RuntimeError(f"{what}: {t} rows, {positions.numel()} positions and {slots.numel()} slots")
+    ks, ks_step = _check_scale(k_scale, "k_scale", what, k_cache)
+    vs, vs_step = _check_scale(v_scale, "v_scale", what, v_cache)
+    q = torch.empty((t, n_q_heads, d), dtype=qkv.dtype, device=dev)
+    sp, ss, sh, _ = k_cache.stride()
+    _launch(dev, L.lib().fp8b200_rope_write_paged, what, qkv.data_ptr(), L.dtype_code(qkv.dtype), t, ld, n_q_heads, hk, d,
+            cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), slots.data_ptr(), q.data_ptr(),
+            k_cache.data_ptr(), v_cache.data_ptr(), L.dtype_code(k_cache.dtype), pages, page, sp, ss, sh, ks, ks_step, vs,
+            vs_step)
+    return q
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                    cu_new: torch.Tensor, kv_lens: torch.Tensor, *, scale: float | None = None, window: int = 0,
+                    sinks: int = 0, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None,
+                    max_new: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of each request's new tokens over its pages.
+
+    q: (tokens, q_heads, head_dim) bfloat16 or float16; rows cu_new[r] to
+    cu_new[r + 1] are request r's, the last at position kv_lens[r] - 1 (cu_new,
+    kv_lens: int32, from paged_slots; the step's k and v already in the
+    caches). A query at position p sees key j where j <= p and, with window >
+    0, p - j < window or j < sinks: a sliding window whose first tokens stay
+    visible. Query head h reads key/value head h // (q_heads // kv_heads).
+    scale: of the scores, default head_dim ** -0.5. k_scale, v_scale: as in
+    rope_write_paged. head_dim: a multiple of 16 up to 256.
+
+    max_new: the largest number of new tokens of one request, where the host
+    knows it (it picks the kernels; a wrong value costs time, not results).
+    Scores, maxima, sums and outputs are float32, rounded once to q's type;
+    see the kernels for the weights' type. A query that sees no key gives 0; a
+    table entry outside the pool hides its keys; hidden keys' values, NaN
+    included, have no effect. Rows that belong to no request are left as they
+    were in a given `out` (of q's shape and type, any 16-byte aligned rows)
+    and 0 in a new one."""
+    what = "paged_attention"
+    dev = q.device
+    pages, page, hk, d = _check_caches(k_cache, v_cache, q, what)
+    if q.dim() != 3 or q.shape[2] != d or (q.numel() and q.stride(2) != 1):
+        raise RuntimeError(f"{what}: q must be (tokens, q_heads, {d}) with contiguous heads, got {tuple(q.shape)}")
+    t, hq, _ = q.shape
+    if hq < 1 or hk < 1 or hq % hk:
+        raise RuntimeError(f"{what}: {hq} query heads over {hk} key/value heads")
+    ld = _check_table(block_table, what, dev)
+    _check(cu_new, "cu_new", what, torch.int32, 1, dev)
+    _check(kv_lens, "kv_lens", what, torch.int32, 1, dev)
+    n, cols = block_table.shape
+    if cu_new.numel() != n + 1 or kv_lens.numel() != n:
+        raise RuntimeError(f"{what}: {n} block_table rows need {n + 1} cu_new and {n} kv_lens, got {cu_new.numel()} and "
+                           f"{kv_lens.numel()}")
+    if window < 0 or sinks < 0:
+        raise RuntimeError(f"{what}: window={window} and sinks={sinks} must not be negative")
+    if max_new is not None and max_new < 1:
+        raise RuntimeError(f"{what}: max_new={max_new} must be positive")
+    ks, ks_step = _check_scale(k_scale, "k_scale", what, k_cache)
+    vs, vs_step = _check_scale(v_scale, "v_scale", what, v_cache)
+    new_out = out is None
+    if new_out:
+        out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or (out.numel() and out.stride(2) != 1):
+        raise RuntimeError(f"{what}: `out` must be a {q.dtype} tensor of q's shape on {dev} with contiguous heads")
+    size = _workspace_bytes.get((dev.index, d), 0)
+    if size == 0 and dev.type == "cuda":
+        with torch.cuda.device(dev):
+            size = L.lib().fp8b200_paged_attention_workspace(d)
+        if size < 0:
+            L.check(size, what)
+        _workspace_bytes[dev.index, d] = size
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    sp, ss, sh, _ = k_cache.stride()
+    q_tok, q_head, _ = q.stride()
+    o_tok, o_head, _ = out.stride()
+    _launch(dev, L.lib().fp8b200_paged_attention, what, q.data_ptr(), L.dtype_code(q.dtype), q_tok, q_head, t, hq, hk, d,
+            k_cache.data_ptr(), v_cache.data_ptr(), L.dtype_code(k_cache.dtype), pages, page, sp, ss, sh,
+            block_table.data_ptr(), ld, cols, cu_new.data_ptr(), kv_lens.data_ptr(), n, d ** -0.5 if scale is None else scale,
+            ks, ks_step, vs, vs_step, window, sinks, max_new or 0, out.data_ptr(), o_tok, o_head, 1 if new_out else 0,
+            ws.data_ptr(), size)
+    return out
