@@ -324,10 +324,11 @@ int fp8b200_rope_write_paged(const void *qkv, int dtype, int64_t tokens, int64_t
  * fp8b200_rope_write_paged leaves them, strides multiples of 16 bytes.
  * head_dim: a multiple of 16 up to 256. max_new: the most new tokens of a
  * request if the host knows (0: not known); it picks the kernels, a wrong value
- * costs time but not results. workspace: fp8b200_paged_attention_workspace(head_dim)
- * bytes that no other call uses at the same time.
+ * costs time but not results. workspace:
+ * fp8b200_paged_attention_workspace(head_dim, max_new * group) bytes (max_new 0:
+ * tokens * group) that no other call uses at the same time.
  */
-int64_t fp8b200_paged_attention_workspace(int head_dim);
+int64_t fp8b200_paged_attention_workspace(int head_dim, int64_t max_rows);
 int fp8b200_paged_attention(const void *q, int dtype, int64_t q_stride_token, int64_t q_stride_head,
                             int64_t tokens, int n_q_heads, int n_kv_heads, int head_dim, const void *k_cache,
                             const void *v_cache, int cache_dtype, int64_t pages, int64_t page_size,
@@ -337,6 +338,13 @@ int fp8b200_paged_attention(const void *q, int dtype, int64_t q_stride_token, in
                             const float *k_scale, int k_scale_step, const float *v_scale, int v_scale_step,
                             int window, int sinks, int64_t max_new, void *out, int64_t out_stride_token,
                             int64_t out_stride_head, int zero_rest, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Device-side status of the attention kernels' bounded waits on the current
+ * device: FP8B200_OK, or FP8B200_ETIMEOUT with the site of the first one that
+ * ran out in *status_out. Synchronises the device; `reset` clears the word.
+ */
+int fp8b200_paged_status(uint32_t *status_out, int reset);
 
 /*
  * Device-side status of the scaled GEMM on the current device: 0 if no

@@ -670,14 +670,20 @@ int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 }  // namespace paged
 }  // namespace fp8b200
 
-extern "C" int64_t fp8b200_paged_attention_workspace(int head_dim) {
+// Requests with more query rows than TC_OVER (tokens x group) go to the
+// tensor-memory kernel when the longest has more than TC_FROM and the head
+// size is at most 128.
+static constexpr int64_t TC_FROM = 64, TC_OVER = 16;
+static int64_t paged_generic_workspace(int dp, int sms) { return 2 * (int64_t)sms * (2 * 64 * (int64_t)(dp + 2) * 4 + 16); }
+
+extern "C" int64_t fp8b200_paged_attention_workspace(int head_dim, int64_t max_rows) {
   using namespace fp8b200;
   using namespace fp8b200::paged;
   int dev;
   if (int rc = check_device(&dev)) return rc;
   if (head_dim < 16 || head_dim > 256) return set_error(FP8B200_EINVAL, "paged_attention: head_dim must be in 16 .. 256");
-  const int64_t blocks = 2 * (int64_t)current_sm_count();
-  return blocks * (2 * 64 * (int64_t)(padded_dim(head_dim) + 2) * 4 + 16);
+  const int dp = padded_dim(head_dim), sms = current_sm_count();
+  return paged_generic_workspace(dp, sms) + (dp <= 128 && max_rows > TC_FROM ? tc_workspace(dp, sms) : 0);
 }
 
 extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_stride_token, int64_t q_stride_head,
@@ -718,7 +724,9 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
     return set_error(FP8B200_EINVAL, "paged_attention: null pointer");
   if (!aligned16(q) || !aligned16(out) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace))
     return set_error(FP8B200_EINVAL, "paged_attention: tensors must be 16-byte aligned");
-  const int64_t need = fp8b200_paged_attention_workspace(head_dim);
+  const int64_t group = n_q_heads / n_kv_heads;
+  const int64_t most = std::min(max_new > 0 ? max_new : tokens, tokens) * group;  // query rows of the longest request
+  const int64_t need = fp8b200_paged_attention_workspace(head_dim, most);
   if (need < 0) return (int)need;
   if (workspace_bytes < need)
     return set_error(FP8B200_EINVAL, "paged_attention: workspace of %lld bytes, %lld are needed", (long long)workspace_bytes,
@@ -751,10 +759,23 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
   p.rows_upto = INT32_MAX;
   p.desc = (int4 *)workspace;
   p.part = (float *)((uint8_t *)workspace + (int64_t)blocks_max * 16);
-  const int64_t most = std::min(max_new > 0 ? max_new : tokens, tokens) * p.group;  // query rows of the longest request
-  const int rw = most <= 16 ? 1 : most <= 32 ? 2 : 4;
   const int dp = padded_dim(head_dim);
   const bool f16 = dtype == FP8B200_F16;
+  if (dp <= 128 && most > TC_FROM && requests > 0) {
+    // all requests alike: one launch; else the short ones (decoding among chunks) keep the kernel made for them
+    const bool alike = max_new > 0 && max_new * requests == tokens;
+    AttnParams t = p;
+    if (!alike) {
+      t.rows_over = TC_OVER;
+      p.rows_upto = TC_OVER;
+    }
+    if (int rc = launch_tc(t, f16, cache_dtype, dp, current_sm_count(), (uint8_t *)workspace + paged_generic_workspace(dp, current_sm_count()),
+                           (cudaStream_t)stream))
+      return rc;
+    if (alike) return FP8B200_OK;
+    p.zero_rest = 0;
+  }
+  const int rw = p.rows_upto <= 16 || most <= 16 ? 1 : most <= 32 ? 2 : 4;
   Variant v;
   if (cache_dtype == FP8B200_E4M3) v = f16 ? pick<true, FP8B200_E4M3>(dp, rw) : pick<false, FP8B200_E4M3>(dp, rw);
   else if (cache_dtype == FP8B200_E5M2) v = f16 ? pick<true, FP8B200_E5M2>(dp, rw) : pick<false, FP8B200_E5M2>(dp, rw);

@@ -149,6 +149,10 @@ __device__ __forceinline__ float cache_value(const uint8_t *base, int64_t elem) 
     return to_f32<F16>(__ldg(reinterpret_cast<const uint16_t *>(base) + elem));
 }
 
+// The kernel for many query rows (paged_attention_tc.cu): head sizes up to 128.
+int64_t tc_workspace(int dp, int sms);
+int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int sms, uint8_t *workspace, cudaStream_t st);
+
 // One query row over the keys of tiles [t0, t1) of `tiles`, value by value:
 // the way out where a hidden key's infinity or NaN met a zero weight in a
 // matrix product (0 * inf). Hidden keys are not touched here. The warp's

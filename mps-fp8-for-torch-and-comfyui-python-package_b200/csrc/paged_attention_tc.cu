@@ -1,0 +1,917 @@
+// Attention over the pages of a key/value cache for requests with many query
+// rows (chunks and prompts), on the 5th-generation tensor cores.
+//
+// The mathematics, the masks and the segments are those of paged_attention.cu;
+// a block of rows is 256 (two tiles of 128: one row per tensor-memory lane),
+// a key tile 128. One persistent CTA an SM, 12 warps:
+//   warps 0-3, 4-7  one softmax group per row tile, a thread a row: S from
+//                   tensor memory, weights back to it as the second product's
+//                   A operand, running maximum and sum in registers
+//   warp 8          issues the MMAs (one thread): S = Q K^T and O += P V
+//   warps 9-11      bring K and V tiles into shared memory: cp.async gathers
+//                   the rows of the pages (any page size); float8 codes are
+//                   staged raw and converted to f16 (exact)
+// While one group computes its weights the tensor core works for the other.
+// Tensor memory: S of either tile (128 columns each, P over its first 64) and
+// O of either tile.
+//
+// O is rescaled only when a row's maximum has grown by more than 2^8 since its
+// base was set (the weights stay below 2^8, or 2^15 with the f16 scaling, so
+// nothing overflows and the quotient is the same): after the first tiles that
+// is rare, and the O accumulator stays in tensor memory.
+//
+// Work: the units (key tiles) of all segments in one line, cut into one share
+// a CTA; a cut within a sixteenth of a share of a segment's edge moves there,
+// so with many segments none is split, and with few all SMs still work.
+//
+// Bound by the tensor core and the exponentials alike: 256 x 128 scores cost
+// 2048 cycles of MMA at head size 128 and 2048 cycles of ex2 (16 a cycle).
+//
+// No counterpart in the reference.
+#include "paged_attention.cuh"
+
+#include <algorithm>
+#include <atomic>
+
+namespace fp8b200 {
+namespace paged {
+namespace {
+
+constexpr int KT = 128;          // keys a tile
+constexpr int QT = 128;          // rows a tile
+constexpr int QB = 2 * QT;       // rows a block
+constexpr int TC_THREADS = 384;
+constexpr int PRODUCERS = 96;
+constexpr int HIDE_RING = 8;     // tiles whose page masks are kept: more than the producers run ahead of the softmax
+constexpr unsigned long long WAIT_NS = 2000000000ull;
+
+__device__ uint32_t g_paged_status;  // 0, or the site of a wait that ran out
+
+template <bool F16, int KV, int DP>
+struct Tc {
+  static constexpr bool FP8 = KV == FP8B200_E4M3 || KV == FP8B200_E5M2;
+  static constexpr bool MF16 = F16 || FP8;
+  static constexpr int TILE = KT * DP * 2;                // K or V tile, Q tile (16-bit)
+  static constexpr int SLOTS = FP8 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 5 : 8);
+  static constexpr int RAW = FP8 ? KT * DP : 0;
+  static constexpr int RAWS = FP8 ? 2 : 0;
+  static constexpr int OFF_KV = 2 * TILE;
+  static constexpr int OFF_RAW = OFF_KV + SLOTS * TILE;
+  static constexpr int OFF_OFFS = OFF_RAW + RAWS * RAW;   // slot offsets of two tiles
+  static constexpr int OFF_HIDE = OFF_OFFS + 2 * KT * 8;  // page masks, 128 bits a tile
+  static constexpr int OFF_BARS = OFF_HIDE + HIDE_RING * 16;
+  static constexpr int BARS = 2 * SLOTS + 8;
+  static constexpr int SMEM = OFF_BARS + BARS * 8 + 16;
+  static constexpr float SHIFT = MF16 ? 7.0f : 0.0f;      // weights are scaled by 2^SHIFT and stay below 2^(SHIFT + 8)
+  static constexpr uint32_t FMT = MF16 ? 0u : 1u;
+  // f32 accumulator, A and B of one type, M = 128; S: N = 128 keys, B K-major; O: N = DP, B (V) MN-major
+  static constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t)(KT >> 3) << 17) | ((128u >> 4) << 24);
+  static constexpr uint32_t IDESC_O =
+      (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((128u >> 4) << 24);
+  static_assert(OFF_OFFS >= (16384 + 1) * 4, "the requests' first rows fit in front of it");
+  static_assert(SMEM <= 232448, "shared memory of one CTA");
+};
+
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Bounded: a wait that runs out records its site, tells the CTA's other roles
+// (s_failed) and holds its thread for 200 us so that copies and MMAs issued
+// before it have landed when the CTA tears down.
+__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t *s_failed, uint32_t site) {
+  const uint64_t t0 = now_ns();
+  for (uint32_t n = 1;; n++) {
+    if (bar_test(bar, parity)) return true;
+    if ((n & 31u) == 0) {
+      const bool late = now_ns() - t0 > WAIT_NS;
+      if (late || *s_failed) {
+        if (late) {
+          *s_failed = 1;
+          atomicCAS(&g_paged_status, 0u, 0x80000000u | site);
+        }
+        const uint64_t t1 = now_ns();
+        while (now_ns() - t1 < 200000ull) __nanosleep(1000);
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t *s_failed, uint32_t site) {
+  if (bar_test(bar, parity)) return true;
+  return bar_wait_slow(bar, parity, s_failed, site);
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+#define PAGED_R32(r)                                                                                                   \
+  "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),          \
+      "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),           \
+      "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),          \
+      "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+__device__ __forceinline__ void tld32(uint32_t taddr, uint32_t *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// Waits for the loads issued before it; r is an operand so that no use of it moves ahead.
+__device__ __forceinline__ void tld_wait(uint32_t *r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : PAGED_R32(r) : : "memory");
+}
+__device__ __forceinline__ void tst32(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tst16(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tst_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory matrix descriptors, 128-byte swizzle. K-major (Q, K): rows of
+// 64 values, 8-row groups 1024 bytes apart. MN-major (V): 8 keys x 64 dims an
+// atom, 8-key groups 1024 bytes apart (stride), 64-dim blocks `lead` apart.
+__device__ __forceinline__ uint64_t desc_k(uint32_t a) {
+  return (uint64_t)((a & 0x3FFFFu) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t a, uint32_t lead) {
+  return (uint64_t)((a & 0x3FFFFu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+         (2ull << 61);
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(*reinterpret_cast<uint64_t *>(&d))
+      : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)), "l"(*reinterpret_cast<uint64_t *>(&c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(*reinterpret_cast<uint64_t *>(&d))
+      : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+  return d;
+}
+
+// ---- the line of units
+// Blocks of rows have places x: request r's from place(r) on, where place(r)
+// = floor(rows before r / 256) + r leaves room for its last, partial block
+// (some places stay empty). A place's segments, one a key/value head, follow
+// one another; a segment's units are the key tiles its 256 rows can see.
+__device__ __forceinline__ int place(const AttnParams &p, int start, int r) {
+  return (int)((int64_t)start * p.group / QB) + r;
+}
+struct Block {
+  Request rq;
+  Tiles<KT> tl;
+  int qt, units;  // 0 units: the place is empty
+};
+__device__ __forceinline__ Block block_at(const AttnParams &p, const Request &rq, int qt) {
+  Block b;
+  b.rq = rq;
+  b.qt = qt;
+  const int64_t rows = (int64_t)rq.n * p.group;
+  b.units = 0;
+  b.tl = Tiles<KT>{0, 0, 0};
+  if (rq.n == 0 || !takes(p, rq.n) || (int64_t)qt * QB >= rows) return b;
+  const int last = (int)(min(rows, (int64_t)(qt + 1) * QB) - 1);
+  b.tl = visible_tiles<KT>(p, rq.first + qt * QB / p.group, rq.first + last / p.group);
+  b.units = max(1, b.tl.count());
+  return b;
+}
+// Within a request the last blocks, which see the most keys, come first.
+__device__ __forceinline__ Block block_of_place(const AttnParams &p, int r, int x) {
+  const Request rq = load_request(p, r);
+  const int64_t n = ((int64_t)rq.n * p.group + QB - 1) / QB;
+  const int i = x - place(p, rq.start, r);
+  if (i < 0 || i >= n) {
+    Block b;
+    b.rq = rq, b.qt = 0, b.units = 0;
+    b.tl = Tiles<KT>{0, 0, 0};
+    return b;
+  }
+  return block_at(p, rq, (int)(n - 1) - i);
+}
+
+// One CTA's walk through its share [u, u_end): every role takes the same steps.
+struct Walk {
+  long long u, u_end, before;  // before: units before place x
+  int x, r;
+  // the segment in hand
+  Block b;
+  int h, t_begin, t_end;
+  long long seg_start;
+};
+__device__ __forceinline__ bool next_segment(const AttnParams &p, Walk &w) {
+  while (w.u < w.u_end && w.r < p.requests) {
+    const Block b = block_of_place(p, w.r, w.x);
+    const long long n = (long long)b.units * p.hk;
+    if (w.u >= w.before + n) {
+      w.before += n;
+      w.x++;
+      while (w.r + 1 < p.requests && w.x >= place(p, load_request(p, w.r + 1).start, w.r + 1)) w.r++;
+      // behind the last request's places: nothing is left
+      if (w.r + 1 == p.requests && b.units == 0 && (long long)(w.x - place(p, b.rq.start, w.r)) * QB > (long long)b.rq.n * p.group + QB)
+        return false;
+      continue;
+    }
+    const long long local = w.u - w.before;
+    w.b = b;
+    w.h = (int)(local / b.units);
+    w.t_begin = (int)(local - (long long)w.h * b.units);
+    w.t_end = (int)min((long long)b.units, w.t_begin + (w.u_end - w.u));
+    w.seg_start = w.u - w.t_begin;
+    w.u += w.t_end - w.t_begin;
+    return true;
+  }
+  return false;
+}
+
+template <bool F16, int KV, int DP>
+__global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const AttnParams p) {
+  using C = Tc<F16, KV, DP>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base_a = saddr(smem);
+  const uint32_t kv_a = base_a + C::OFF_KV, raw_a = base_a + C::OFF_RAW;
+  long long *s_off = reinterpret_cast<long long *>(smem + C::OFF_OFFS);   // [2][KT]
+  uint32_t *s_hide = reinterpret_cast<uint32_t *>(smem + C::OFF_HIDE);    // [HIDE_RING][4]
+  const uint32_t bars = base_a + C::OFF_BARS;
+  uint32_t *s_misc = reinterpret_cast<uint32_t *>(smem + C::OFF_BARS + C::BARS * 8);  // tensor memory base, failed flag
+  volatile uint32_t *s_failed = s_misc + 1;
+  auto kv_full = [&](int s) { return bars + 8u * s; };
+  auto kv_empty = [&](int s) { return bars + 8u * (C::SLOTS + s); };
+  const uint32_t q_full = bars + 8u * (2 * C::SLOTS), s_full = q_full + 16, p_full = q_full + 32, pv_done = q_full + 48;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+
+  if (base_a & 1023u) {  // the swizzled tiles need it; the same for every CTA
+    if (tid == 0) atomicCAS(&g_paged_status, 0u, 0x80000000u | 99u);
+    return;
+  }
+  if (tid == 0) {
+    for (int s = 0; s < C::SLOTS; s++) {
+      bar_init(kv_full(s), PRODUCERS);
+      bar_init(kv_empty(s), 1);
+    }
+    for (int g = 0; g < 2; g++) {
+      bar_init(q_full + 8 * g, QT);
+      bar_init(s_full + 8 * g, 1);
+      bar_init(p_full + 8 * g, QT);
+      bar_init(pv_done + 8 * g, 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    *s_failed = 0;
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(s_misc)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // ---- this CTA's share; the requests' first rows in shared memory that Q and K take over later
+  int *s_start = reinterpret_cast<int *>(smem);  // [requests + 1]
+  long long *s_sum = s_off;                      // [warps]
+  long long(*s_found)[4] = reinterpret_cast<long long(*)[4]>(s_off + TC_THREADS / 32);  // cut, place, units before it, request
+  for (int r = tid; r <= p.requests; r += TC_THREADS) s_start[r] = r < p.requests ? load_request(p, r).start : p.tokens;
+  if (tid < 2) s_found[tid][0] = -1;
+  __syncthreads();
+  const int places = p.requests == 0 ? 0 : place(p, min(max(__ldg(p.cu + p.requests), 0), p.tokens), p.requests);
+  auto request_of = [&](int x) {
+    int lo = 0, hi = p.requests;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (place(p, s_start[mid], mid) <= x) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  };
+  long long total = 0;
+  for (int x = tid; x < places; x += TC_THREADS) total += (long long)block_of_place(p, request_of(x), x).units * p.hk;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
+  if (lane == 0) s_sum[warp] = total;
+  __syncthreads();
+  total = 0;
+  for (int i = 0; i < TC_THREADS / 32; i++) total += s_sum[i];
+  __syncthreads();
+  if (p.zero_rest) zero_rest(p, blockIdx.x, gridDim.x);
+  const long long ctas = min((long long)gridDim.x, total), c = blockIdx.x;
+  if (tid == 0) p.desc[c] = make_int4(-1, 0, 0, 0);
+  const long long slack = ctas > 0 ? total / ctas / 16 : 0;
+  Walk walk0;
+  walk0.u = walk0.u_end = 0;
+  walk0.before = 0;
+  walk0.x = walk0.r = 0;
+  if (c < ctas) {
+    const long long raw[2] = {c * total / ctas, (c + 1) * total / ctas};
+    long long before = 0;
+    for (int x0 = 0; x0 < places; x0 += TC_THREADS) {
+      const int x = x0 + tid;
+      const int r = x < places ? request_of(x) : 0;
+      const int units = x < places ? block_of_place(p, r, x).units : 0;
+      const long long mine = (long long)units * p.hk;
+      long long inc = mine;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long a = __shfl_up_sync(~0u, inc, d);
+        if (lane >= d) inc += a;
+      }
+      if (lane == 31) s_sum[warp] = inc;
+      __syncthreads();
+      long long b = before + inc - mine, all = before;
+      for (int w = 0; w < TC_THREADS / 32; w++) {
+        if (w < warp) b += s_sum[w];
+        all += s_sum[w];
+      }
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+        if (raw[k] >= b && raw[k] < b + mine) {
+          const long long in = (raw[k] - b) % units;  // of the segment that the cut falls into
+          long long cut = raw[k];
+          if (in <= slack) cut -= in;
+          else if (units - in <= slack) cut += units - in;
+          s_found[k][0] = cut, s_found[k][1] = x, s_found[k][2] = b, s_found[k][3] = r;
+        }
+      __syncthreads();
+      before = all;
+      if (before > raw[1]) break;
+    }
+    walk0.u = s_found[0][0];
+    walk0.u_end = raw[1] >= total ? total : s_found[1][0];
+    walk0.x = (int)s_found[0][1];
+    walk0.before = s_found[0][2];
+    walk0.r = (int)s_found[0][3];
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(s_misc);
+  // tensor memory columns: S (P) of tile g at 128 g, O of tile g at 256 + DP g
+
+  if (warp >= 8) {
+    Walk w = walk0;
+    if (warp == 8) {
+      // ================================================= MMA issue
+      if (lane == 0) {
+        int slot = 0;
+        uint32_t phase = 0, segs = 0, tiles = 0;
+        bool ok = true;
+        auto step = [&]() {
+          if (++slot == C::SLOTS) slot = 0, phase ^= 1;
+        };
+        auto issue_s = [&](int g, int s) {
+#pragma unroll
+          for (int k = 0; k < DP / 16; k++) {
+            const uint32_t at = (uint32_t)((k >> 2) * (KT * 128) + (k & 3) * 32);
+            mma_ss(tmem + 128 * g, desc_k(base_a + g * C::TILE + at), desc_k(kv_a + s * C::TILE + at), C::IDESC_S, k > 0);
+          }
+          commit(s_full + 8 * g);
+        };
+        while (ok && next_segment(p, w)) {
+          const int n = w.t_end - w.t_begin;
+          ok = bar_wait(q_full, segs & 1, s_failed, 1) && bar_wait(q_full + 8, segs & 1, s_failed, 2) &&
+               bar_wait(kv_full(slot), phase, s_failed, 3);
+          if (!ok) break;
+          fence_after();
+          issue_s(0, slot);
+          issue_s(1, slot);
+          commit(kv_empty(slot));
+          step();
+          for (int j = 0; j < n && ok; j++) {
+            const bool more = j + 1 < n;
+            const int ks = slot;
+            if (more) {
+              ok = bar_wait(kv_full(ks), phase, s_failed, 4);
+              step();
+            }
+            const int vs = slot;
+            ok = ok && bar_wait(kv_full(vs), phase, s_failed, 5);
+            step();
+            if (!ok) break;
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+              ok = ok && bar_wait(p_full + 8 * g, tiles & 1, s_failed, 6 + g);
+              if (!ok) break;
+              fence_after();
+#pragma unroll
+              for (int k = 0; k < KT / 16; k++)
+                mma_ts(tmem + 256 + DP * g, tmem + 128 * g + 8 * k, desc_mn(kv_a + vs * C::TILE + k * 2048, KT * 128),
+                       C::IDESC_O, j > 0 || k > 0);
+              commit(pv_done + 8 * g);
+              if (more) issue_s(g, ks);
+            }
+            if (!ok) break;
+            commit(kv_empty(vs));
+            if (more) commit(kv_empty(ks));
+            tiles++;
+          }
+          segs++;
+        }
+      }
+      __syncwarp();
+    } else {
+      // ================================================= K and V tiles
+      const int pt = tid - 9 * 32;
+      const int used = p.d / (C::FP8 ? 16 : 8);           // 16-byte units of a cached row
+      constexpr int CPR = DP / (C::FP8 ? 16 : 8);         // and with the padding
+      int slot = 0, filled = 0;                           // slot of the next tile to load, tiles loaded
+      uint32_t phase = 0, tiles = 0;
+      bool ok = true;
+      int pend_slot = 0;                                  // slot of the oldest tile not yet announced
+      int pending = 0;
+      // tile loaded by cp.async: announce the oldest one once it has landed
+      auto announce = [&]() {
+        if constexpr (C::FP8) {
+          const uint32_t raw = raw_a + (uint32_t)((filled - pending) & 1) * C::RAW;
+          const uint32_t dst = kv_a + pend_slot * C::TILE;
+          for (int i = pt; i < KT * CPR; i += PRODUCERS) {
+            const int row = i / CPR, cu = i % CPR;
+            uint32_t q[4];
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(raw + i * 16));
+            if (cu >= used) q[0] = q[1] = q[2] = q[3] = 0u;
+            const uint32_t at = dst + (uint32_t)((cu >> 2) * (KT * 128) + row * 128);
+            const int u = (cu & 3) * 2, x = row & 7;
+            sts16(at + ((u ^ x) << 4), fp8x2_to_f16x2<KV>(q[0] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[0] >> 16),
+                  fp8x2_to_f16x2<KV>(q[1] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[1] >> 16));
+            sts16(at + (((u + 1) ^ x) << 4), fp8x2_to_f16x2<KV>(q[2] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[2] >> 16),
+                  fp8x2_to_f16x2<KV>(q[3] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[3] >> 16));
+          }
+        }
+        fence_async();
+        bar_arrive(kv_full(pend_slot));
+        if (++pend_slot == C::SLOTS) pend_slot = 0;
+        pending--;
+      };
+      auto load = [&](const uint8_t *src, int entry, int h) {
+        // float8: the raw ring has two tiles, so the one before the last is converted first
+        if constexpr (C::FP8) {
+          if (pending == 2) {
+            cp_wait<1>();
+            announce();
+          }
+        } else if (pending == 2) {
+          cp_wait<1>();
+          announce();
+        }
+        // the slot must be free (for float8 only before the conversion, but the wait is the same)
+        if (filled >= C::SLOTS && !bar_wait(kv_empty(slot), phase ^ 1, s_failed, 10)) {
+          ok = false;
+          return;
+        }
+        for (int i = pt; i < KT * CPR; i += PRODUCERS) {
+          const int row = i / CPR, cu = i % CPR;
+          const long long off = s_off[entry * KT + row];
+          const bool valid = off >= 0 && cu < used;
+          const uint8_t *at = valid ? src + (off + (long long)h * p.s_head) * (C::FP8 ? 1 : 2) + cu * 16 : src;
+          uint32_t dst;
+          if constexpr (C::FP8) dst = raw_a + (uint32_t)(filled & 1) * C::RAW + i * 16;
+          else dst = kv_a + slot * C::TILE + (cu >> 3) * (KT * 128) + row * 128 + (((cu & 7) ^ (row & 7)) << 4);
+          cp16(dst, at, valid);
+        }
+        cp_commit();
+        filled++;
+        pending++;
+        if (++slot == C::SLOTS) slot = 0, phase ^= 1;
+      };
+      // A thread whose wait ran out (ok false) goes on through the barriers of
+      // the group without loading: nobody is left waiting in them.
+      while (next_segment(p, w)) {
+        const int hi = w.b.rq.first + (int)((min((int64_t)w.b.rq.n * p.group, (int64_t)(w.b.qt + 1) * QB) - 1) / p.group);
+        for (int t = w.t_begin; t <= w.t_end; t++) {
+          if (t < w.t_end) {
+            const int k0 = w.b.tl.at(t) * KT, entry = tiles & 1;
+            __syncwarp();
+            asm volatile("bar.sync 1, 96;" ::: "memory");  // the entry's readers are done
+            for (int i = pt; i < KT; i += PRODUCERS) {
+              const int j = k0 + i;
+              long long off = -1;
+              bool hide = false;
+              if (j <= hi) {
+                off = slot_offset(p, w.r, j);
+                hide = off < 0;
+              }
+              s_off[entry * KT + i] = off;
+              const uint32_t word = __ballot_sync(~0u, hide);
+              if (lane == 0) s_hide[(tiles % HIDE_RING) * 4 + (i >> 5)] = word;
+            }
+            __syncwarp();
+            asm volatile("bar.sync 1, 96;" ::: "memory");
+            if (ok) load(p.k, entry, w.h);
+            tiles++;
+          }
+          if (ok && t > w.t_begin) load(p.v, (tiles - (t < w.t_end ? 2 : 1)) & 1, w.h);
+        }
+      }
+      while (pending > 0) {
+        if (pending == 2) cp_wait<1>();
+        else cp_wait<0>();
+        if (ok) announce();
+        else pending--;
+      }
+      cp_wait<0>();
+    }
+  } else {
+    // =================================================== softmax, one row a thread
+    Walk w = walk0;
+    const int g = warp >> 2;
+    const int my = (warp & 3) * 32 + lane;                 // row of the tile
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lanes + 128 * g, t_o = tmem + lanes + 256 + DP * g;
+    const uint32_t q_a = base_a + g * C::TILE;
+    uint32_t tiles = 0;
+    bool ok = true;
+    while (ok && next_segment(p, w)) {
+      const Request rq = w.b.rq;
+      const int64_t all_rows = (int64_t)rq.n * p.group;
+      const int64_t row0 = (int64_t)w.b.qt * QB + g * QT;  // the tile's first row; it may lie behind the request's last
+      const int64_t row = row0 + my;
+      const bool mine = row < all_rows;
+      const int clipped = (int)min(row, all_rows - 1);
+      const int tok = clipped / p.group, head = w.h * p.group + clipped % p.group;
+      const int pos = rq.first + tok;
+      const int pos_lo = rq.first + (int)(min(row0, all_rows - 1) / p.group);
+      const int pos_hi = rq.first + (int)(min(row0 + QT, all_rows) - 1 < 0 ? 0 : (min(row0 + QT, all_rows) - 1) / p.group);
+      // ---- the row of Q (the previous segment's products with this tile are complete: its last S was waited for)
+      // its sign takes that of the scale, so that the maximum of the products is the maximum of the scores
+      float qscale = 1.0f;
+      const float scale = p.scale_log2 * (C::FP8 && p.ks ? __ldg(p.ks + p.ks_step * w.h) : 1.0f);
+      const float sign = scale < 0.0f ? -1.0f : 1.0f;
+      {
+        const uint16_t *qp = p.q + (int64_t)(rq.start + tok) * p.q_tok + (int64_t)head * p.q_head;
+        float mul = sign;
+        if constexpr (C::FP8 && !F16) {                    // bf16 to f16, the largest value in [1, 2)
+          float a = 0.0f;
+          for (int i = 0; i < p.d / 8; i++) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(qp) + i);
+            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++) a = fmaxf(a, fmaxf(fabsf(u2f(x[e] << 16)), fabsf(u2f(x[e] & 0xFFFF0000u))));
+          }
+          uint32_t eb = f2u(a) >> 23;
+          eb = (eb == 255u || a == 0.0f) ? 127u : min(max(eb, 1u), 253u);
+          mul = u2f((254u - eb) << 23) * sign;
+          qscale = u2f(eb << 23);
+        }
+#pragma unroll 4
+        for (int i = 0; i < DP / 8; i++) {
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (mine && i * 8 < p.d) v = __ldg(reinterpret_cast<const uint4 *>(qp) + i);
+          uint32_t x[4] = {v.x, v.y, v.z, v.w};
+          if constexpr (C::FP8 && !F16) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = pack2<true>(u2f(x[e] << 16) * mul, u2f(x[e] & 0xFFFF0000u) * mul);
+          } else if (sign < 0.0f) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] ^= 0x80008000u;
+          }
+          sts16(q_a + (i >> 3) * (QT * 128) + my * 128 + (((i & 7) ^ (my & 7)) << 4), x[0], x[1], x[2], x[3]);
+        }
+        fence_async();
+        bar_arrive(q_full + 8 * g);
+      }
+      // a scale of 0 weighs all keys alike; kept above 0 so that a hidden key's -inf stays one
+      float sc = fabsf(scale) * qscale;
+      if (sc == 0.0f) sc = 1e-30f;
+      float base = -INFINITY, sum = 0.0f;                  // of this row: weights are 2^(score - base + SHIFT)
+      for (int t = w.t_begin; t < w.t_end; t++) {
+        const int k0 = w.b.tl.at(t) * KT;
+        ok = bar_wait(s_full + 8 * g, tiles & 1, s_failed, 20 + g);
+        if (!__all_sync(~0u, ok)) {
+          ok = false;
+          break;
+        }
+        fence_after();
+        // S is read twice, 32 columns at a time and one read ahead: first for the maximum, then for the weights
+        const uint4 hide = *reinterpret_cast<const uint4 *>(s_hide + (tiles % HIDE_RING) * 4);
+        const bool any_hide = (hide.x | hide.y | hide.z | hide.w) != 0u;
+        const bool masked = k0 + KT - 1 > pos_lo || any_hide ||
+                            (p.window > 0 && pos_hi - k0 >= p.window && k0 + KT - 1 >= p.sinks);
+        const int lim = pos - k0;
+        const int wlo = p.window > 0 ? (int)max((int64_t)pos - p.window - k0, (int64_t)-1) : -1;  // hidden up to here
+        const int sk = (int)min(max((int64_t)p.sinks - k0, (int64_t)0), (int64_t)KT);
+        auto mask = [&](uint32_t *s, int c4) {
+          if (masked) {
+            const uint32_t hw = c4 == 0 ? hide.x : c4 == 1 ? hide.y : c4 == 2 ? hide.z : hide.w;
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+              const int k = c4 * 32 + i;
+              if (!(k <= lim && (k > wlo || k < sk)) || ((hw >> i) & 1u)) s[i] = 0xFF800000u;
+            }
+          }
+        };
+        uint32_t s[2][32];
+        tld32(t_s, s[0]);
+        tld_wait(s[0]);
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c4 = 0; c4 < 4; c4++) {
+          if (c4 < 3) tld32(t_s + 32 * (c4 + 1), s[(c4 + 1) & 1]);
+          mask(s[c4 & 1], c4);
+#pragma unroll
+          for (int i = 0; i < 32; i++) mx[i & 3] = fmaxf(mx[i & 3], u2f(s[c4 & 1][i]));
+          if (c4 < 3) tld_wait(s[(c4 + 1) & 1]);
+        }
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
+        const bool grow = top > base + 8.0f;               // also the first key of the row (base -inf)
+        if (__any_sync(~0u, grow)) {
+          const float nb = grow ? top : base;
+          const float f = base == -INFINITY ? 0.0f : ex2(base - nb);
+          sum *= f;
+          base = nb;
+          if (t > w.t_begin) {                             // O holds the tiles before: wait for the last one, rescale
+            ok = bar_wait(pv_done + 8 * g, (tiles - 1) & 1, s_failed, 30 + g);
+            if (!__all_sync(~0u, ok)) {
+              ok = false;
+              break;
+            }
+            fence_after();
+#pragma unroll 1
+            for (int i = 0; i < DP / 32; i++) {
+              uint32_t o[32];
+              tld32(t_o + 32 * i, o);
+              tld_wait(o);
+#pragma unroll
+              for (int e = 0; e < 32; e++) o[e] = f2u(u2f(o[e]) * f);
+              tst32(t_o + 32 * i, o);
+            }
+          }
+        }
+        const float off = C::SHIFT - (base == -INFINITY ? 0.0f : base);
+        const float2 sc2 = make_float2(sc, sc), off2 = make_float2(off, off);
+        float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        tld32(t_s, s[0]);
+        tld_wait(s[0]);
+#pragma unroll
+        for (int c4 = 0; c4 < 4; c4++) {                   // P overwrites columns of S that have been read
+          if (c4 < 3) tld32(t_s + 32 * (c4 + 1), s[(c4 + 1) & 1]);
+          mask(s[c4 & 1], c4);
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            float2 e = fma2(make_float2(u2f(s[c4 & 1][2 * i]), u2f(s[c4 & 1][2 * i + 1])), sc2, off2);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            acc[i & 1] = add2(acc[i & 1], e);
+            pk[i] = pack2<C::MF16>(e.x, e.y);
+          }
+          if (c4 < 3) tld_wait(s[(c4 + 1) & 1]);
+          tst16(t_s + 16 * c4, pk);
+        }
+        tst_wait();
+        fence_before();
+        bar_arrive(p_full + 8 * g);
+        const float2 a2 = add2(acc[0], acc[1]);
+        sum += a2.x + a2.y;
+        tiles++;
+      }
+      if (!__all_sync(~0u, ok)) {
+        ok = false;
+        break;
+      }
+      // ---- the segment's end
+      ok = bar_wait(pv_done + 8 * g, (tiles - 1) & 1, s_failed, 40 + g);
+      if (!__all_sync(~0u, ok)) {
+        ok = false;
+        break;
+      }
+      fence_after();
+      const bool begins = w.t_begin == 0, ends = w.t_end == w.b.units;
+      const bool whole = begins && ends;
+      if (tid == 0 && begins && !ends) {
+        const long long seg_end = w.seg_start + w.b.units;
+        long long last = c + 1;                            // the CTA whose share reaches the segment's end
+        while (last + 1 < ctas && (last + 1) * total / ctas < seg_end - slack) last++;
+        p.desc[c] = make_int4(w.r, w.b.qt, w.h, (int)last);
+      }
+      const float vs = C::FP8 && p.vs ? __ldg(p.vs + p.vs_step * w.h) : 1.0f;
+      const float inv = sum == 0.0f ? 0.0f : vs / sum;
+      const float mine_base = base - C::SHIFT;
+      float *part = p.part + (c * 2 + (begins ? 1 : 0)) * (int64_t)(QB * (DP + 2));
+      const int brow = g * QT + my;
+      uint16_t *out = p.out + (int64_t)(rq.start + tok) * p.o_tok + (int64_t)head * p.o_head;
+      bool odd = false;
+#pragma unroll 1
+      for (int i = 0; i < DP / 32; i++) {
+        uint32_t o[32];
+        __syncwarp();
+        tld32(t_o + 32 * i, o);
+        tld_wait(o);
+        if (mine) {
+#pragma unroll
+          for (int e = 0; e < 32; e++) odd |= !(fabsf(u2f(o[e])) < INFINITY);
+        }
+        if (mine && whole) {
+#pragma unroll
+          for (int q = 0; q < 4; q++)
+            if (i * 32 + q * 8 < p.d) {
+              uint32_t x[4];
+#pragma unroll
+              for (int e = 0; e < 4; e++) x[e] = pack2<F16>(u2f(o[q * 8 + 2 * e]) * inv, u2f(o[q * 8 + 2 * e + 1]) * inv);
+              *reinterpret_cast<uint4 *>(out + i * 32 + q * 8) = make_uint4(x[0], x[1], x[2], x[3]);
+            }
+        } else if (mine) {
+#pragma unroll
+          for (int q = 0; q < 8; q++)
+            *reinterpret_cast<uint4 *>(part + brow * DP + i * 32 + q * 4) = make_uint4(o[q * 4], o[q * 4 + 1], o[q * 4 + 2], o[q * 4 + 3]);
+        }
+      }
+      fence_before();
+      if (mine && !whole) {
+        part[QB * DP + brow] = mine_base;
+        part[QB * DP + QB + brow] = sum;
+      }
+      uint32_t redo = __ballot_sync(~0u, odd);             // see careful_row
+      while (redo) {
+        const int src = __ffs(redo) - 1;
+        redo &= redo - 1;
+        const int tok_s = __shfl_sync(~0u, tok, src), head_s = __shfl_sync(~0u, head, src), brow_s = __shfl_sync(~0u, brow, src);
+        float m, l, ov[DP / 32];
+        __syncwarp();
+        careful_row<F16, KV, DP, KT>(p, w.r, rq.start + tok_s, head_s, rq.first + tok_s, w.b.tl, w.t_begin, w.t_end, m, l, ov);
+        const float li = l == 0.0f ? 0.0f : vs / l;
+        uint16_t *os = p.out + (int64_t)(rq.start + tok_s) * p.o_tok + (int64_t)head_s * p.o_head;
+#pragma unroll
+        for (int i = 0; i < DP / 32; i++) {
+          const int d = lane + 32 * i;
+          if (whole) {
+            if (d < p.d) os[d] = (uint16_t)pack2<F16>(ov[i] * li, 0.0f);
+          } else {
+            part[brow_s * DP + d] = ov[i];
+          }
+        }
+        if (!whole && lane == 0) {
+          part[QB * DP + brow_s] = m;
+          part[QB * DP + QB + brow_s] = l;
+        }
+      }
+    }
+  }
+  // ---- teardown, reached by every role whether or not a wait ran out
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+// Joins the parts of cut segments, as paged_merge_kernel does; blockIdx.y
+// takes a share of the rows.
+template <bool F16, int DP>
+__global__ void __launch_bounds__(128) paged_merge_tc_kernel(const AttnParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const long long c = blockIdx.x;
+  const int4 d = p.desc[c];
+  if (d.x < 0) return;
+  const Request rq = load_request(p, d.x);
+  const int64_t row0 = (int64_t)d.y * QB;
+  const int h = d.z;
+  const int rows = (int)min((int64_t)QB, (int64_t)rq.n * p.group - row0);
+  const float vs = p.vs ? __ldg(p.vs + p.vs_step * h) : 1.0f;
+  constexpr int64_t SLOT = QB * (DP + 2);
+  for (int i = blockIdx.y * 128 + threadIdx.x; i < rows * (DP / 4); i += gridDim.y * 128) {
+    const int row = i / (DP / 4), d4 = (i % (DP / 4)) * 4;
+    if (d4 >= p.d) continue;
+    float base = -INFINITY, l = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (long long b = c; b <= d.w; b++) {
+      const float *part = p.part + (b * 2 + (b == c ? 1 : 0)) * SLOT;
+      const float bb = part[QB * DP + row], bl = part[QB * DP + QB + row];
+      const float4 v = *reinterpret_cast<const float4 *>(part + row * DP + d4);
+      const float nb = fmaxf(base, bb), ref = nb == -INFINITY ? 0.0f : nb;
+      const float f = ex2(base - ref), e = ex2(bb - ref);
+      base = nb;
+      l = l * f + bl * e;
+      x[0] = x[0] * f + v.x * e, x[1] = x[1] * f + v.y * e, x[2] = x[2] * f + v.z * e, x[3] = x[3] * f + v.w * e;
+    }
+    const float inv = l == 0.0f ? 0.0f : vs / l;
+    const int qr = (int)(row0 + row), tok = rq.start + qr / p.group, head = h * p.group + qr % p.group;
+    uint16_t *out = p.out + (int64_t)tok * p.o_tok + (int64_t)head * p.o_head + d4;
+    *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<F16>(x[0] * inv, x[1] * inv), pack2<F16>(x[2] * inv, x[3] * inv));
+  }
+}
+
+struct TcVariant {
+  void (*main)(AttnParams);
+  void (*merge)(AttnParams);
+  int smem;
+};
+template <bool F16, int KV>
+TcVariant pick_tc(int dp) {
+  if (dp == 64) return {paged_attention_tc_kernel<F16, KV, 64>, paged_merge_tc_kernel<F16, 64>, Tc<F16, KV, 64>::SMEM};
+  return {paged_attention_tc_kernel<F16, KV, 128>, paged_merge_tc_kernel<F16, 128>, Tc<F16, KV, 128>::SMEM};
+}
+
+}  // namespace
+
+int64_t tc_workspace(int dp, int sms) { return (int64_t)sms * (2 * QB * (int64_t)(dp + 2) * 4 + 16); }
+
+int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int sms, uint8_t *workspace, cudaStream_t st) {
+  AttnParams p = params;
+  p.desc = (int4 *)workspace;
+  p.part = (float *)(workspace + (int64_t)sms * 16);
+  TcVariant v;
+  if (cache_dtype == FP8B200_E4M3) v = f16 ? pick_tc<true, FP8B200_E4M3>(dp) : pick_tc<false, FP8B200_E4M3>(dp);
+  else if (cache_dtype == FP8B200_E5M2) v = f16 ? pick_tc<true, FP8B200_E5M2>(dp) : pick_tc<false, FP8B200_E5M2>(dp);
+  else v = f16 ? pick_tc<true, FP8B200_F16>(dp) : pick_tc<false, FP8B200_BF16>(dp);
+  if (cudaFuncSetAttribute(v.main, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem) != cudaSuccess)
+    return check_launch("paged_attention");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)sms);
+  cfg.blockDim = dim3(TC_THREADS);
+  cfg.dynamicSmemBytes = (size_t)v.smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, v.main, p);
+  cfg.gridDim = dim3((unsigned)sms, 8);
+  cfg.blockDim = dim3(128);
+  cfg.dynamicSmemBytes = 0;
+  cudaLaunchKernelEx(&cfg, v.merge, p);
+  count_launch(2);
+  return check_launch("paged_attention");
+}
+
+}  // namespace paged
+}  // namespace fp8b200
+
+extern "C" int fp8b200_paged_status(uint32_t *status_out, int reset) {
+  using namespace fp8b200;
+  int dev;
+  if (int rc = check_device(&dev)) return rc;
+  uint32_t s = 0;
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&s, paged::g_paged_status, sizeof(s));
+  if (e == cudaSuccess && reset && s) {
+    const uint32_t zero = 0;
+    e = cudaMemcpyToSymbol(paged::g_paged_status, &zero, sizeof(zero));
+  }
+  if (e != cudaSuccess) return set_error(FP8B200_ELAUNCH, "paged_status: %s", cudaGetErrorString(e));
+  if (status_out) *status_out = s;
+  return s ? set_error(FP8B200_ETIMEOUT, "paged_attention: a wait ran out (site %u)", s & 0x7FFFFFFFu) : FP8B200_OK;
+}

@@ -68,6 +68,7 @@ def _declare(L):
         "fp8b200_paged_attention": [vp, i32, i64, i64, i64, i32, i32, i32, vp, vp, i32, i64, i64, i64, i64, i64,
                                     vp, i64, i64, vp, vp, i64, f32, vp, i32, vp, i32, i32, i32, i64, vp, i64,
                                     i64, i32, vp, i64, vp],
+        "fp8b200_paged_status": [ctypes.POINTER(ctypes.c_uint32), i32],
         "fp8b200_gemm_status": [ctypes.POINTER(ctypes.c_uint32), i32],
         "fp8b200_debug_gemm": [i32, ctypes.c_ulonglong],
         "fp8b200_gemm_set_path": [i32],
@@ -77,7 +78,7 @@ def _declare(L):
             fn = getattr(L, name)
             fn.argtypes = args
             fn.restype = i32
-    L.fp8b200_paged_attention_workspace.argtypes = [i32]
+    L.fp8b200_paged_attention_workspace.argtypes = [i32, i64]
     L.fp8b200_paged_attention_workspace.restype = i64
 
 

@@ -37,7 +37,7 @@ class PagedStep(NamedTuple):
     free_head: torch.Tensor   # (1,) int32: first free page not taken
 
 
-_workspace_bytes: dict[tuple[int, int], int] = {}
+_workspace_bytes: dict[tuple[int, int, int], int] = {}
 
 
 def _check(t: torch.Tensor, name: str, what: str, dtype: torch.dtype, dim: int, dev: torch.device) -> None:
@@ -246,13 +246,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or (out.numel() and out.stride(2) != 1):
         raise RuntimeError(f"{what}: `out` must be a {q.dtype} tensor of q's shape on {dev} with contiguous heads")
-    size = _workspace_bytes.get((dev.index, d), 0)
+    max_rows = min(t if max_new is None else max_new, t) * (hq // hk)
+    size = _workspace_bytes.get((dev.index, d, max_rows), 0)
     if size == 0 and dev.type == "cuda":
         with torch.cuda.device(dev):
-            size = L.lib().fp8b200_paged_attention_workspace(d)
+            size = L.lib().fp8b200_paged_attention_workspace(d, max_rows)
         if size < 0:
             L.check(size, what)
-        _workspace_bytes[dev.index, d] = size
+        _workspace_bytes[dev.index, d, max_rows] = size
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
     sp, ss, sh, _ = k_cache.stride()
     q_tok, q_head, _ = q.stride()

@@ -10,7 +10,11 @@ f16 2^-11 otherwise), ds bounds the error of a score: (d + 8) 2^-24 of
 scale sum |q||k| for the float32 sums, plus, for bf16 queries of a float8
 cache, 2^-24 of the row's largest |q| times scale sum |k| (values far below
 the row's largest, held in f16); it enters the numerator and the denominator.
-2^-17 covers exp2 and the float32 sums over the keys (up to 2^7 joins)."""
+2^-17 covers exp2 and the float32 sums over the keys (up to 2^7 joins).
+f16 weights have an absolute step too: at most 2^-25 is lost of each (half of
+the least subnormal) while the weight of the key that set the row's base is
+2^7 and part of the sum, so n keys lose at most n 2^-32 max |v| of the output
+(seen where the key with nearly all the weight holds a 0 in that place)."""
 import itertools
 import math
 
@@ -329,7 +333,8 @@ def reference(s, window=0, sinks=0, scale=None):
             ds = (d + 8) * 2.0 ** -24 * mag
             if fp8 and q.dtype == BF16:
                 ds = ds + 2.0 ** -24 * qq.abs().amax(1, keepdim=True) * torch.where(seen, kk.abs().sum(1)[None], 0.0).amax(1, keepdim=True) * abs(scale)
-            tol[a:b, h] = u_out * out[a:b, h].abs() + (u_w + 2 * ds + 2.0 ** -17) * big + 1e-30
+            lost = m * 2.0 ** -32 * vv_abs.max() if u_w == half_step(F16) else 0.0
+            tol[a:b, h] = u_out * out[a:b, h].abs() + (u_w + 2 * ds + 2.0 ** -17) * big + lost + 1e-30
     return out, tol
 
 
