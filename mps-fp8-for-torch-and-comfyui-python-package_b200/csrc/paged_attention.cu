@@ -761,7 +761,7 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
   p.part = (float *)((uint8_t *)workspace + (int64_t)blocks_max * 16);
   const int dp = padded_dim(head_dim);
   const bool f16 = dtype == FP8B200_F16;
-  if (dp <= 128 && most > TC_FROM && requests > 0) {
+  if (dp <= 128 && most > TC_FROM && requests > 0 && tc_takes(p)) {
     // all requests alike: one launch; else the short ones (decoding among chunks) keep the kernel made for them
     const bool alike = max_new > 0 && max_new * requests == tokens;
     AttnParams t = p;

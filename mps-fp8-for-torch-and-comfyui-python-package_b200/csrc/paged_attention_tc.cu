@@ -3,14 +3,18 @@
 //
 // The mathematics, the masks and the segments are those of paged_attention.cu;
 // a block of rows is 256 (two tiles of 128: one row per tensor-memory lane),
-// a key tile 128. One persistent CTA an SM, 12 warps:
-//   warps 0-3, 4-7  one softmax group per row tile, a thread a row: S from
-//                   tensor memory, weights back to it as the second product's
-//                   A operand, running maximum and sum in registers
-//   warp 8          issues the MMAs (one thread): S = Q K^T and O += P V
-//   warps 9-11      bring K and V tiles into shared memory: cp.async gathers
-//                   the rows of the pages (any page size); float8 codes are
-//                   staged raw and converted to f16 (exact)
+// a key tile 128. One persistent CTA an SM; its warps:
+//   0-7      two softmax groups, one per row tile, a thread a row: S from
+//            tensor memory, weights back to it as the second product's A
+//            operand, running maximum and sum in registers
+//   8-11     float8 caches only: turn the raw codes of a tile into f16 (exact)
+// and a warpgroup for control:
+//   MMA      issues S = Q K^T and O += P V (a uniform warp, one lane's
+//            instructions: the descriptors stay in uniform registers)
+//   segments walks the CTA's share of the work and hands its segments on
+//   2 x TMA  in turn bring K and V tiles in, four rows of any pages a copy
+//            (tile::gather4), so every page size is alike; rows without a key
+//            are out of the map's bounds and arrive as zeros
 // While one group computes its weights the tensor core works for the other.
 // Tensor memory: S of either tile (128 columns each, P over its first 64) and
 // O of either tile.
@@ -30,8 +34,11 @@
 // No counterpart in the reference.
 #include "paged_attention.cuh"
 
+#include <cuda.h>
+
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 
 namespace fp8b200 {
 namespace paged {
@@ -40,35 +47,46 @@ namespace {
 constexpr int KT = 128;          // keys a tile
 constexpr int QT = 128;          // rows a tile
 constexpr int QB = 2 * QT;       // rows a block
-constexpr int TC_THREADS = 384;
-constexpr int PRODUCERS = 96;
+constexpr int SEGS = 4;           // segments in the ring
 constexpr int HIDE_RING = 8;     // tiles whose page masks are kept: more than the producers run ahead of the softmax
 constexpr unsigned long long WAIT_NS = 2000000000ull;
 
 __device__ uint32_t g_paged_status;  // 0, or the site of a wait that ran out
+
+// The pool as the tensor maps see it: rows of `pitch` elements, one per slot
+// and head. Slot s of page g under head h is row g * page + s * slot + h * head.
+struct RowMap {
+  int page, slot, head, rows;
+};
 
 template <bool F16, int KV, int DP>
 struct Tc {
   static constexpr bool FP8 = KV == FP8B200_E4M3 || KV == FP8B200_E5M2;
   static constexpr bool MF16 = F16 || FP8;
   static constexpr int TILE = KT * DP * 2;                // K or V tile, Q tile (16-bit)
-  static constexpr int SLOTS = FP8 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 5 : 8);
-  static constexpr int RAW = FP8 ? KT * DP : 0;
-  static constexpr int RAWS = FP8 ? 2 : 0;
+  static constexpr int CTRL = FP8 ? 12 : 8;               // first warp of the control group
+  static constexpr int THREADS = (CTRL + 4) * 32;
+  // registers a thread: 128 (168) at launch, moved to the softmax by warpgroup: 2 x 184 + 72 + 72 = 4 x 128
+  // (float8), 2 x 216 + 72 = 3 x 168
+  static constexpr int REGS_SOFTMAX = FP8 ? 184 : 216, REGS_OTHER = 72;
+  static constexpr int SLOTS = DP == 128 ? (FP8 ? 4 : 5) : 8;
+  static constexpr int RAWS = FP8 ? (DP == 128 ? 2 : 4) : 0;  // float8: raw tiles on their way
+  static constexpr int RAW = KT * DP;
   static constexpr int OFF_KV = 2 * TILE;
   static constexpr int OFF_RAW = OFF_KV + SLOTS * TILE;
-  static constexpr int OFF_OFFS = OFF_RAW + RAWS * RAW;   // slot offsets of two tiles
-  static constexpr int OFF_HIDE = OFF_OFFS + 2 * KT * 8;  // page masks, 128 bits a tile
+  static constexpr int OFF_PLAN = OFF_RAW + RAWS * RAW;   // the plan's scratch
+  static constexpr int OFF_HIDE = OFF_PLAN + 256;         // page masks, 128 bits a tile
   static constexpr int OFF_BARS = OFF_HIDE + HIDE_RING * 16;
-  static constexpr int BARS = 2 * SLOTS + 8;
-  static constexpr int SMEM = OFF_BARS + BARS * 8 + 16;
+  static constexpr int BARS = 2 * SLOTS + 2 * RAWS + 8 + 2 * SEGS;
+  static constexpr int OFF_SEGS = OFF_BARS + BARS * 8;
+  static constexpr int SMEM = OFF_SEGS + SEGS * 48 + 16;
   static constexpr float SHIFT = MF16 ? 7.0f : 0.0f;      // weights are scaled by 2^SHIFT and stay below 2^(SHIFT + 8)
   static constexpr uint32_t FMT = MF16 ? 0u : 1u;
   // f32 accumulator, A and B of one type, M = 128; S: N = 128 keys, B K-major; O: N = DP, B (V) MN-major
   static constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t)(KT >> 3) << 17) | ((128u >> 4) << 24);
   static constexpr uint32_t IDESC_O =
       (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((128u >> 4) << 24);
-  static_assert(OFF_OFFS >= (16384 + 1) * 4, "the requests' first rows fit in front of it");
+  static_assert(OFF_PLAN >= (16384 + 1) * 4, "the requests' first rows fit in front of it");
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
 
@@ -97,7 +115,7 @@ __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
 // Bounded: a wait that runs out records its site, tells the CTA's other roles
 // (s_failed) and holds its thread for 200 us so that copies and MMAs issued
 // before it have landed when the CTA tears down.
-__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t *s_failed, uint32_t site) {
+__device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t *s_failed, uint32_t site) {
   const uint64_t t0 = now_ns();
   for (uint32_t n = 1;; n++) {
     if (bar_test(bar, parity)) return true;
@@ -121,23 +139,31 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// MMA and commit by the lane whose `lead` is set, in code that the whole warp runs.
+__device__ __forceinline__ void commit(uint32_t lead, uint32_t bar) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(lead)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
       : "memory");
 }
 #define PAGED_R32(r)                                                                                                   \
@@ -190,13 +216,16 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t a, uint32_t lead) {
   return (uint64_t)((a & 0x3FFFFu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
          (2ull << 61);
 }
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+// Columns x .. of four rows, each the map's box wide and one high.
+__device__ __forceinline__ void gather4(uint32_t dst, const CUtensorMap *map, int x, const int (&row)[4], uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+      "%6}], [%7];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
+      : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
@@ -257,54 +286,38 @@ __device__ __forceinline__ Block block_of_place(const AttnParams &p, int r, int 
   return block_at(p, rq, (int)(n - 1) - i);
 }
 
-// One CTA's walk through its share [u, u_end): every role takes the same steps.
-struct Walk {
-  long long u, u_end, before;  // before: units before place x
-  int x, r;
-  // the segment in hand
-  Block b;
-  int h, t_begin, t_end;
-  long long seg_start;
+// A segment, or the part of it that falls into this CTA's share.
+struct alignas(16) Segment {
+  int r, h, qt;                // request (-1: no more segments), key/value head, block of rows
+  int start, n, first;         // the request's new tokens (see Request)
+  int t_begin, t_end, units;   // key tiles [t_begin, t_end) of `units`
+  int sinks, from;             // list entry i is key tile i < sinks ? i : from + i - sinks
+  int last;                    // if the part begins the segment and does not end it: the CTA that ends it
+  __device__ __forceinline__ int tile(int i) const { return i < sinks ? i : from + i - sinks; }
+  __device__ __forceinline__ Tiles<KT> tiles() const { return Tiles<KT>{sinks, from, 0}; }
 };
-__device__ __forceinline__ bool next_segment(const AttnParams &p, Walk &w) {
-  while (w.u < w.u_end && w.r < p.requests) {
-    const Block b = block_of_place(p, w.r, w.x);
-    const long long n = (long long)b.units * p.hk;
-    if (w.u >= w.before + n) {
-      w.before += n;
-      w.x++;
-      while (w.r + 1 < p.requests && w.x >= place(p, load_request(p, w.r + 1).start, w.r + 1)) w.r++;
-      // behind the last request's places: nothing is left
-      if (w.r + 1 == p.requests && b.units == 0 && (long long)(w.x - place(p, b.rq.start, w.r)) * QB > (long long)b.rq.n * p.group + QB)
-        return false;
-      continue;
-    }
-    const long long local = w.u - w.before;
-    w.b = b;
-    w.h = (int)(local / b.units);
-    w.t_begin = (int)(local - (long long)w.h * b.units);
-    w.t_end = (int)min((long long)b.units, w.t_begin + (w.u_end - w.u));
-    w.seg_start = w.u - w.t_begin;
-    w.u += w.t_end - w.t_begin;
-    return true;
-  }
-  return false;
-}
+static_assert(sizeof(Segment) == 48, "SEGS * 48 bytes");
 
 template <bool F16, int KV, int DP>
-__global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const AttnParams p) {
+__global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
+    paged_attention_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                              const RowMap rm) {
   using C = Tc<F16, KV, DP>;
+  constexpr int TC_THREADS = C::THREADS;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t base_a = saddr(smem);
   const uint32_t kv_a = base_a + C::OFF_KV, raw_a = base_a + C::OFF_RAW;
-  long long *s_off = reinterpret_cast<long long *>(smem + C::OFF_OFFS);   // [2][KT]
   uint32_t *s_hide = reinterpret_cast<uint32_t *>(smem + C::OFF_HIDE);    // [HIDE_RING][4]
   const uint32_t bars = base_a + C::OFF_BARS;
-  uint32_t *s_misc = reinterpret_cast<uint32_t *>(smem + C::OFF_BARS + C::BARS * 8);  // tensor memory base, failed flag
+  Segment *s_seg = reinterpret_cast<Segment *>(smem + C::OFF_SEGS);
+  uint32_t *s_misc = reinterpret_cast<uint32_t *>(smem + C::OFF_SEGS + SEGS * 48);  // tensor memory base, failed flag
   volatile uint32_t *s_failed = s_misc + 1;
   auto kv_full = [&](int s) { return bars + 8u * s; };
   auto kv_empty = [&](int s) { return bars + 8u * (C::SLOTS + s); };
-  const uint32_t q_full = bars + 8u * (2 * C::SLOTS), s_full = q_full + 16, p_full = q_full + 32, pv_done = q_full + 48;
+  auto raw_full = [&](int s) { return bars + 8u * (2 * C::SLOTS + s); };
+  auto raw_empty = [&](int s) { return bars + 8u * (2 * C::SLOTS + C::RAWS + s); };
+  const uint32_t q_full = bars + 8u * (2 * C::SLOTS + 2 * C::RAWS), s_full = q_full + 16, p_full = q_full + 32, pv_done = q_full + 48;
+  const uint32_t seg_full = q_full + 64, seg_empty = seg_full + 8 * SEGS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   if (base_a & 1023u) {  // the swizzled tiles need it; the same for every CTA
@@ -313,8 +326,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
   }
   if (tid == 0) {
     for (int s = 0; s < C::SLOTS; s++) {
-      bar_init(kv_full(s), PRODUCERS);
+      bar_init(kv_full(s), C::FP8 ? 128 : 1);
       bar_init(kv_empty(s), 1);
+    }
+    for (int s = 0; s < C::RAWS; s++) {
+      bar_init(raw_full(s), 1);
+      bar_init(raw_empty(s), 128);
     }
     for (int g = 0; g < 2; g++) {
       bar_init(q_full + 8 * g, QT);
@@ -322,10 +339,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
       bar_init(p_full + 8 * g, QT);
       bar_init(pv_done + 8 * g, 1);
     }
+    for (int i = 0; i < SEGS; i++) {
+      bar_init(seg_full + 8 * i, 1);
+      bar_init(seg_empty + 8 * i, C::FP8 ? 15 : 11);  // the warps that read it: softmax, converting, MMA, TMA
+    }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     *s_failed = 0;
   }
-  if (warp == 8) {
+  if (warp == C::CTRL) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(saddr(s_misc)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -334,8 +355,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
 
   // ---- this CTA's share; the requests' first rows in shared memory that Q and K take over later
   int *s_start = reinterpret_cast<int *>(smem);  // [requests + 1]
-  long long *s_sum = s_off;                      // [warps]
-  long long(*s_found)[4] = reinterpret_cast<long long(*)[4]>(s_off + TC_THREADS / 32);  // cut, place, units before it, request
+  long long *s_sum = reinterpret_cast<long long *>(smem + C::OFF_PLAN);                 // [warps]
+  long long(*s_found)[4] = reinterpret_cast<long long(*)[4]>(s_sum + TC_THREADS / 32);  // cut, place, units before it, request
   for (int r = tid; r <= p.requests; r += TC_THREADS) s_start[r] = r < p.requests ? load_request(p, r).start : p.tokens;
   if (tid < 2) s_found[tid][0] = -1;
   __syncthreads();
@@ -362,10 +383,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
   const long long ctas = min((long long)gridDim.x, total), c = blockIdx.x;
   if (tid == 0) p.desc[c] = make_int4(-1, 0, 0, 0);
   const long long slack = ctas > 0 ? total / ctas / 16 : 0;
-  Walk walk0;
-  walk0.u = walk0.u_end = 0;
-  walk0.before = 0;
-  walk0.x = walk0.r = 0;
+  long long u = 0, u_end = 0, u_before = 0;      // the share, and the units before place x
+  int u_x = 0, u_r = 0;
   if (c < ctas) {
     const long long raw[2] = {c * total / ctas, (c + 1) * total / ctas};
     long long before = 0;
@@ -400,11 +419,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
       before = all;
       if (before > raw[1]) break;
     }
-    walk0.u = s_found[0][0];
-    walk0.u_end = raw[1] >= total ? total : s_found[1][0];
-    walk0.x = (int)s_found[0][1];
-    walk0.before = s_found[0][2];
-    walk0.r = (int)s_found[0][3];
+    u = s_found[0][0];
+    u_end = raw[1] >= total ? total : s_found[1][0];
+    u_x = (int)s_found[0][1];
+    u_before = s_found[0][2];
+    u_r = (int)s_found[0][3];
   }
   fence_before();
   __syncthreads();
@@ -412,171 +431,223 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(s_misc);
   // tensor memory columns: S (P) of tile g at 128 g, O of tile g at 256 + DP g
 
-  if (warp >= 8) {
-    Walk w = walk0;
-    if (warp == 8) {
-      // ================================================= MMA issue
+  // The segment in ring place n % SEGS once it is there; 0 if the wait ran out.
+  auto seg_at = [&](uint32_t n, uint32_t site) -> const Segment * {
+    if (!bar_wait(seg_full + 8 * (n % SEGS), (n / SEGS) & 1, s_failed, site)) return nullptr;
+    return s_seg + n % SEGS;
+  };
+  if (warp >= C::CTRL) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_OTHER));
+    if (warp == C::CTRL + 1) {
+      // ================================================= the share's segments
       if (lane == 0) {
-        int slot = 0;
-        uint32_t phase = 0, segs = 0, tiles = 0;
-        bool ok = true;
-        auto step = [&]() {
-          if (++slot == C::SLOTS) slot = 0, phase ^= 1;
-        };
-        auto issue_s = [&](int g, int s) {
-#pragma unroll
-          for (int k = 0; k < DP / 16; k++) {
-            const uint32_t at = (uint32_t)((k >> 2) * (KT * 128) + (k & 3) * 32);
-            mma_ss(tmem + 128 * g, desc_k(base_a + g * C::TILE + at), desc_k(kv_a + s * C::TILE + at), C::IDESC_S, k > 0);
-          }
-          commit(s_full + 8 * g);
-        };
-        while (ok && next_segment(p, w)) {
-          const int n = w.t_end - w.t_begin;
-          ok = bar_wait(q_full, segs & 1, s_failed, 1) && bar_wait(q_full + 8, segs & 1, s_failed, 2) &&
-               bar_wait(kv_full(slot), phase, s_failed, 3);
-          if (!ok) break;
-          fence_after();
-          issue_s(0, slot);
-          issue_s(1, slot);
-          commit(kv_empty(slot));
-          step();
-          for (int j = 0; j < n && ok; j++) {
-            const bool more = j + 1 < n;
-            const int ks = slot;
-            if (more) {
-              ok = bar_wait(kv_full(ks), phase, s_failed, 4);
-              step();
+        uint32_t n = 0;
+        bool more = true;
+        while (more) {
+          Segment sg;
+          sg.r = -1;
+          while (u < u_end && u_r < p.requests) {
+            const Block b = block_of_place(p, u_r, u_x);
+            const long long all = (long long)b.units * p.hk;
+            if (u < u_before + all) {
+              const int local = (int)(u - u_before);       // units of one place: below 2^31
+              sg.r = u_r, sg.h = local / b.units, sg.qt = b.qt;
+              sg.start = b.rq.start, sg.n = b.rq.n, sg.first = b.rq.first;
+              sg.t_begin = local - sg.h * b.units;
+              sg.t_end = (int)min((long long)b.units, sg.t_begin + (u_end - u));
+              sg.units = b.units, sg.sinks = b.tl.sinks, sg.from = b.tl.from;
+              const long long seg_end = u - sg.t_begin + b.units;
+              sg.last = 0;
+              if (sg.t_begin == 0 && sg.t_end < sg.units) {
+                long long last = c + 1;                    // the CTA whose share reaches the segment's end
+                while (last + 1 < ctas && (last + 1) * total / ctas < seg_end - slack) last++;
+                sg.last = (int)last;
+              }
+              u += sg.t_end - sg.t_begin;
+              break;
             }
-            const int vs = slot;
-            ok = ok && bar_wait(kv_full(vs), phase, s_failed, 5);
-            step();
-            if (!ok) break;
-#pragma unroll
-            for (int g = 0; g < 2; g++) {
-              ok = ok && bar_wait(p_full + 8 * g, tiles & 1, s_failed, 6 + g);
-              if (!ok) break;
-              fence_after();
-#pragma unroll
-              for (int k = 0; k < KT / 16; k++)
-                mma_ts(tmem + 256 + DP * g, tmem + 128 * g + 8 * k, desc_mn(kv_a + vs * C::TILE + k * 2048, KT * 128),
-                       C::IDESC_O, j > 0 || k > 0);
-              commit(pv_done + 8 * g);
-              if (more) issue_s(g, ks);
-            }
-            if (!ok) break;
-            commit(kv_empty(vs));
-            if (more) commit(kv_empty(ks));
-            tiles++;
+            u_before += all;
+            u_x++;
+            while (u_r + 1 < p.requests && u_x >= place(p, load_request(p, u_r + 1).start, u_r + 1)) u_r++;
+            // behind the last request's places nothing is left (only if the offsets make no sense)
+            if (u_r + 1 == p.requests && b.units == 0 &&
+                (long long)(u_x - place(p, b.rq.start, u_r)) * QB > (long long)b.rq.n * p.group + QB)
+              break;
           }
-          segs++;
+          if (n >= SEGS && !bar_wait(seg_empty + 8 * (n % SEGS), ((n / SEGS) & 1) ^ 1, s_failed, 50)) break;
+          s_seg[n % SEGS] = sg;
+          bar_arrive(seg_full + 8 * (n % SEGS));
+          more = sg.r >= 0;
+          n++;
         }
       }
       __syncwarp();
-    } else {
-      // ================================================= K and V tiles
-      const int pt = tid - 9 * 32;
-      const int used = p.d / (C::FP8 ? 16 : 8);           // 16-byte units of a cached row
-      constexpr int CPR = DP / (C::FP8 ? 16 : 8);         // and with the padding
-      int slot = 0, filled = 0;                           // slot of the next tile to load, tiles loaded
-      uint32_t phase = 0, tiles = 0;
+    } else if (warp == C::CTRL) {
+      // ================================================= MMA issue
+      const uint32_t lead = lane == 0;
+      int slot = 0;
+      uint32_t phase = 0, segs = 0, tiles = 0;
       bool ok = true;
-      int pend_slot = 0;                                  // slot of the oldest tile not yet announced
-      int pending = 0;
-      // tile loaded by cp.async: announce the oldest one once it has landed
-      auto announce = [&]() {
-        if constexpr (C::FP8) {
-          const uint32_t raw = raw_a + (uint32_t)((filled - pending) & 1) * C::RAW;
-          const uint32_t dst = kv_a + pend_slot * C::TILE;
-          for (int i = pt; i < KT * CPR; i += PRODUCERS) {
-            const int row = i / CPR, cu = i % CPR;
-            uint32_t q[4];
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(raw + i * 16));
-            if (cu >= used) q[0] = q[1] = q[2] = q[3] = 0u;
-            const uint32_t at = dst + (uint32_t)((cu >> 2) * (KT * 128) + row * 128);
-            const int u = (cu & 3) * 2, x = row & 7;
-            sts16(at + ((u ^ x) << 4), fp8x2_to_f16x2<KV>(q[0] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[0] >> 16),
-                  fp8x2_to_f16x2<KV>(q[1] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[1] >> 16));
-            sts16(at + (((u + 1) ^ x) << 4), fp8x2_to_f16x2<KV>(q[2] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[2] >> 16),
-                  fp8x2_to_f16x2<KV>(q[3] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[3] >> 16));
-          }
-        }
-        fence_async();
-        bar_arrive(kv_full(pend_slot));
-        if (++pend_slot == C::SLOTS) pend_slot = 0;
-        pending--;
-      };
-      auto load = [&](const uint8_t *src, int entry, int h) {
-        // float8: the raw ring has two tiles, so the one before the last is converted first
-        if constexpr (C::FP8) {
-          if (pending == 2) {
-            cp_wait<1>();
-            announce();
-          }
-        } else if (pending == 2) {
-          cp_wait<1>();
-          announce();
-        }
-        // the slot must be free (for float8 only before the conversion, but the wait is the same)
-        if (filled >= C::SLOTS && !bar_wait(kv_empty(slot), phase ^ 1, s_failed, 10)) {
-          ok = false;
-          return;
-        }
-        for (int i = pt; i < KT * CPR; i += PRODUCERS) {
-          const int row = i / CPR, cu = i % CPR;
-          const long long off = s_off[entry * KT + row];
-          const bool valid = off >= 0 && cu < used;
-          const uint8_t *at = valid ? src + (off + (long long)h * p.s_head) * (C::FP8 ? 1 : 2) + cu * 16 : src;
-          uint32_t dst;
-          if constexpr (C::FP8) dst = raw_a + (uint32_t)(filled & 1) * C::RAW + i * 16;
-          else dst = kv_a + slot * C::TILE + (cu >> 3) * (KT * 128) + row * 128 + (((cu & 7) ^ (row & 7)) << 4);
-          cp16(dst, at, valid);
-        }
-        cp_commit();
-        filled++;
-        pending++;
+      auto step = [&]() {
         if (++slot == C::SLOTS) slot = 0, phase ^= 1;
       };
-      // A thread whose wait ran out (ok false) goes on through the barriers of
-      // the group without loading: nobody is left waiting in them.
-      while (next_segment(p, w)) {
-        const int hi = w.b.rq.first + (int)((min((int64_t)w.b.rq.n * p.group, (int64_t)(w.b.qt + 1) * QB) - 1) / p.group);
-        for (int t = w.t_begin; t <= w.t_end; t++) {
-          if (t < w.t_end) {
-            const int k0 = w.b.tl.at(t) * KT, entry = tiles & 1;
-            __syncwarp();
-            asm volatile("bar.sync 1, 96;" ::: "memory");  // the entry's readers are done
-            for (int i = pt; i < KT; i += PRODUCERS) {
-              const int j = k0 + i;
-              long long off = -1;
-              bool hide = false;
-              if (j <= hi) {
-                off = slot_offset(p, w.r, j);
-                hide = off < 0;
-              }
-              s_off[entry * KT + i] = off;
-              const uint32_t word = __ballot_sync(~0u, hide);
-              if (lane == 0) s_hide[(tiles % HIDE_RING) * 4 + (i >> 5)] = word;
-            }
-            __syncwarp();
-            asm volatile("bar.sync 1, 96;" ::: "memory");
-            if (ok) load(p.k, entry, w.h);
-            tiles++;
-          }
-          if (ok && t > w.t_begin) load(p.v, (tiles - (t < w.t_end ? 2 : 1)) & 1, w.h);
+      auto issue_s = [&](int g, int s) {
+        const uint64_t qd = desc_k(base_a + g * C::TILE), kd = desc_k(kv_a + s * C::TILE);
+#pragma unroll
+        for (int k = 0; k < DP / 16; k++) {
+          const uint64_t at = (uint64_t)((k >> 2) * (KT * 128 / 16) + (k & 3) * 2);  // 16-byte units
+          mma_ss(lead, tmem + 128 * g, qd + at, kd + at, C::IDESC_S, k > 0);
         }
+        commit(lead, s_full + 8 * g);
+      };
+      while (ok) {
+        const Segment *sg = seg_at(segs, 51);
+        if (!__all_sync(~0u, sg != nullptr) || sg->r < 0) break;
+        const int n = sg->t_end - sg->t_begin;
+        __syncwarp();
+        if (lane == 0) bar_arrive(seg_empty + 8 * (segs % SEGS));
+        ok = bar_wait(q_full, segs & 1, s_failed, 1) && bar_wait(q_full + 8, segs & 1, s_failed, 2) &&
+             bar_wait(kv_full(slot), phase, s_failed, 3);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        fence_after();
+        issue_s(0, slot);
+        issue_s(1, slot);
+        commit(lead, kv_empty(slot));
+        step();
+        for (int j = 0; j < n && ok; j++) {
+          const bool more = j + 1 < n;
+          const int ks = slot;
+          if (more) {
+            ok = bar_wait(kv_full(ks), phase, s_failed, 4);
+            step();
+          }
+          const int vs = slot;
+          ok = ok && bar_wait(kv_full(vs), phase, s_failed, 5);
+          step();
+#pragma unroll 1
+          for (int g = 0; g < 2; g++) {
+            ok = ok && bar_wait(p_full + 8 * g, tiles & 1, s_failed, 6 + g);
+            ok = __all_sync(~0u, ok);
+            if (!ok) break;
+            fence_after();
+            const uint64_t vd = desc_mn(kv_a + vs * C::TILE, KT * 128);
+#pragma unroll
+            for (int k = 0; k < KT / 16; k++)
+              mma_ts(lead, tmem + 256 + DP * g, tmem + 128 * g + 8 * k, vd + k * (2048 / 16), C::IDESC_O, j > 0 || k > 0);
+            commit(lead, pv_done + 8 * g);
+            if (more) issue_s(g, ks);
+          }
+          if (!ok) break;
+          commit(lead, kv_empty(vs));
+          if (more) commit(lead, kv_empty(ks));
+          tiles++;
+        }
+        segs++;
       }
-      while (pending > 0) {
-        if (pending == 2) cp_wait<1>();
-        else cp_wait<0>();
-        if (ok) announce();
-        else pending--;
+    } else {
+      // ================================================= K and V tiles, in turn: K 0, K 1, V 0, K 2, V 1, ...
+      const uint32_t turn = warp - (C::CTRL + 2);
+      // float8 tiles go to the raw ring, 16-bit ones straight to the operands' ring
+      constexpr int RING = C::FP8 ? C::RAWS : C::SLOTS;
+      uint32_t filled = 0, tiles = 0;
+      bool ok = true;
+      for (uint32_t segs = 0; ok; segs++) {
+        const Segment *sg = seg_at(segs, 52);
+        if (!__all_sync(~0u, sg != nullptr) || sg->r < 0) break;
+        const int r = sg->r, n = sg->t_end - sg->t_begin;
+        const int hi = sg->first + (int)((min((int64_t)sg->n * p.group, (int64_t)(sg->qt + 1) * QB) - 1) / p.group);
+        const int head_row = sg->h * rm.head;
+#pragma unroll 1
+        for (int i = 0; i < 2 * n; i++, filled++) {
+          const bool keys = i == 0 || ((i & 1) && i < 2 * n - 1);
+          const uint32_t number = tiles;
+          tiles += keys;
+          if ((filled & 1u) != turn) continue;
+          const int t = sg->t_begin + (keys ? (i + 1) / 2 : i == 2 * n - 1 ? n - 1 : i / 2 - 1);
+          const int k0 = sg->tile(t) * KT + 4 * lane;
+          int row[4];
+          uint32_t hide[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int j = k0 + e;
+            row[e] = rm.rows;                             // out of bounds: zeros
+            if (j <= hi) {
+              const uint32_t col = (uint32_t)j / (uint32_t)p.page;
+              int page = -1;
+              if (col < (uint32_t)p.table_cols) page = __ldg(p.table + (int64_t)r * p.table_ld + col);
+              if (page >= 0 && page < p.pages) row[e] = page * rm.page + (int)((uint32_t)j - col * (uint32_t)p.page) * rm.slot + head_row;
+            }
+            hide[e] = __ballot_sync(~0u, j <= hi && row[e] == rm.rows);
+          }
+          const uint32_t at = filled % RING, turns = filled / RING;
+          if (filled >= RING) ok = bar_wait(C::FP8 ? raw_empty(at) : kv_empty(at), (turns & 1) ^ 1, s_failed, 10);
+          ok = __all_sync(~0u, ok);
+          if (!ok) break;
+          const uint32_t bar = C::FP8 ? raw_full(at) : kv_full(at);
+          const uint32_t dst = C::FP8 ? raw_a + at * C::RAW : kv_a + at * C::TILE;
+          if (lane == 0) {
+            if (keys) {                                   // key 4 i + e is bit i of word e
+#pragma unroll
+              for (int e = 0; e < 4; e++) s_hide[(number % HIDE_RING) * 4 + e] = hide[e];
+            }
+            bar_expect(bar, C::FP8 ? C::RAW : C::TILE);
+          }
+          __syncwarp();
+          const CUtensorMap *map = keys ? &map_k : &map_v;
+          if constexpr (C::FP8) {
+            gather4(dst + lane * 4 * DP, map, 0, row, bar);
+          } else {
+#pragma unroll
+            for (int b = 0; b < DP / 64; b++) gather4(dst + b * (KT * 128) + lane * 512, map, b * 64, row, bar);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) bar_arrive(seg_empty + 8 * (segs % SEGS));
       }
-      cp_wait<0>();
+    }
+  } else if (C::FP8 && warp >= 8) {
+    // =================================================== float8 codes to f16
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_OTHER));
+    if constexpr (C::FP8) {
+      const int pt = tid - 8 * 32;
+      constexpr int CPR = DP / 16, STEP = 128 / CPR, UNITS = KT / STEP;  // a thread's units lie STEP rows apart
+      static_assert(STEP % 8 == 0, "a thread's rows share their place in the swizzle");
+      const int cu = pt % CPR, row0 = pt / CPR, x = row0 & 7, u8 = (cu & 3) * 2;
+      const uint32_t at8 = (uint32_t)((cu >> 2) * (KT * 128) + row0 * 128);
+      uint32_t done = 0;
+      bool ok = true;
+      for (uint32_t segs = 0; ok; segs++) {
+        const Segment *sg = seg_at(segs, 54);
+        if (!__all_sync(~0u, sg != nullptr) || sg->r < 0) break;
+        const int n = 2 * (sg->t_end - sg->t_begin);
+#pragma unroll 1
+        for (int i = 0; i < n && ok; i++, done++) {
+          const uint32_t rs = done % C::RAWS, ks = done % C::SLOTS;
+          ok = bar_wait(raw_full(rs), (done / C::RAWS) & 1, s_failed, 11);
+          if (done >= C::SLOTS) ok = ok && bar_wait(kv_empty(ks), ((done / C::SLOTS) & 1) ^ 1, s_failed, 12);
+          if (!ok) break;
+          const uint32_t raw = raw_a + rs * C::RAW + pt * 16, dst = kv_a + ks * C::TILE + at8;
+#pragma unroll
+          for (int k = 0; k < UNITS; k++) {
+            uint32_t q[4];
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(raw + k * 2048));
+            sts16(dst + k * (STEP * 128) + ((u8 ^ x) << 4), fp8x2_to_f16x2<KV>(q[0] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[0] >> 16),
+                  fp8x2_to_f16x2<KV>(q[1] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[1] >> 16));
+            sts16(dst + k * (STEP * 128) + (((u8 + 1) ^ x) << 4), fp8x2_to_f16x2<KV>(q[2] & 0xFFFFu),
+                  fp8x2_to_f16x2<KV>(q[2] >> 16), fp8x2_to_f16x2<KV>(q[3] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[3] >> 16));
+          }
+          bar_arrive(raw_empty(rs));
+          fence_async();
+          bar_arrive(kv_full(ks));
+        }
+        __syncwarp();
+        if (lane == 0) bar_arrive(seg_empty + 8 * (segs % SEGS));
+      }
     }
   } else {
     // =================================================== softmax, one row a thread
-    Walk w = walk0;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REGS_SOFTMAX));
     const int g = warp >> 2;
     const int my = (warp & 3) * 32 + lane;                 // row of the tile
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -584,24 +655,26 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
     const uint32_t q_a = base_a + g * C::TILE;
     uint32_t tiles = 0;
     bool ok = true;
-    while (ok && next_segment(p, w)) {
-      const Request rq = w.b.rq;
-      const int64_t all_rows = (int64_t)rq.n * p.group;
-      const int64_t row0 = (int64_t)w.b.qt * QB + g * QT;  // the tile's first row; it may lie behind the request's last
-      const int64_t row = row0 + my;
-      const bool mine = row < all_rows;
-      const int clipped = (int)min(row, all_rows - 1);
-      const int tok = clipped / p.group, head = w.h * p.group + clipped % p.group;
-      const int pos = rq.first + tok;
-      const int pos_lo = rq.first + (int)(min(row0, all_rows - 1) / p.group);
-      const int pos_hi = rq.first + (int)(min(row0 + QT, all_rows) - 1 < 0 ? 0 : (min(row0 + QT, all_rows) - 1) / p.group);
+    for (uint32_t segs = 0; ok; segs++) {
+      const Segment *sg = seg_at(segs, 53);
+      if (!__all_sync(~0u, sg != nullptr) || sg->r < 0) break;
+      const int h = sg->h, first = sg->first, t_begin = sg->t_begin, t_end = sg->t_end;
+      const int all_rows = sg->n * p.group;                // below 2^31: tokens x query heads are
+      const int row0 = sg->qt * QB + g * QT;               // the tile's first row; it may lie behind the request's last
+      const bool mine = row0 + my < all_rows;
+      const int clipped = min(row0 + my, all_rows - 1);
+      const int tok = clipped / p.group, head = h * p.group + clipped - tok * p.group;
+      const int pos = first + tok;
+      const int pos_lo = first + min(row0, all_rows - 1) / p.group;
+      const int pos_hi = first + (min(row0 + QT, all_rows) - 1) / p.group;
+      const int64_t q_row = (int64_t)(sg->start + tok) * p.q_tok + (int64_t)head * p.q_head;
       // ---- the row of Q (the previous segment's products with this tile are complete: its last S was waited for)
       // its sign takes that of the scale, so that the maximum of the products is the maximum of the scores
       float qscale = 1.0f;
-      const float scale = p.scale_log2 * (C::FP8 && p.ks ? __ldg(p.ks + p.ks_step * w.h) : 1.0f);
+      const float scale = p.scale_log2 * (C::FP8 && p.ks ? __ldg(p.ks + p.ks_step * h) : 1.0f);
       const float sign = scale < 0.0f ? -1.0f : 1.0f;
       {
-        const uint16_t *qp = p.q + (int64_t)(rq.start + tok) * p.q_tok + (int64_t)head * p.q_head;
+        const uint16_t *qp = p.q + q_row;
         float mul = sign;
         if constexpr (C::FP8 && !F16) {                    // bf16 to f16, the largest value in [1, 2)
           float a = 0.0f;
@@ -637,44 +710,43 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
       float sc = fabsf(scale) * qscale;
       if (sc == 0.0f) sc = 1e-30f;
       float base = -INFINITY, sum = 0.0f;                  // of this row: weights are 2^(score - base + SHIFT)
-      for (int t = w.t_begin; t < w.t_end; t++) {
-        const int k0 = w.b.tl.at(t) * KT;
+      for (int t = t_begin; t < t_end; t++) {
+        const int k0 = sg->tile(t) * KT;
         ok = bar_wait(s_full + 8 * g, tiles & 1, s_failed, 20 + g);
         if (!__all_sync(~0u, ok)) {
           ok = false;
           break;
         }
         fence_after();
-        // S is read twice, 32 columns at a time and one read ahead: first for the maximum, then for the weights
+        uint32_t s[128];
+#pragma unroll
+        for (int i = 0; i < 4; i++) tld32(t_s + 32 * i, s + 32 * i);
+#pragma unroll
+        for (int i = 0; i < 4; i++) tld_wait(s + 32 * i);
         const uint4 hide = *reinterpret_cast<const uint4 *>(s_hide + (tiles % HIDE_RING) * 4);
         const bool any_hide = (hide.x | hide.y | hide.z | hide.w) != 0u;
-        const bool masked = k0 + KT - 1 > pos_lo || any_hide ||
-                            (p.window > 0 && pos_hi - k0 >= p.window && k0 + KT - 1 >= p.sinks);
-        const int lim = pos - k0;
-        const int wlo = p.window > 0 ? (int)max((int64_t)pos - p.window - k0, (int64_t)-1) : -1;  // hidden up to here
-        const int sk = (int)min(max((int64_t)p.sinks - k0, (int64_t)0), (int64_t)KT);
-        auto mask = [&](uint32_t *s, int c4) {
-          if (masked) {
-            const uint32_t hw = c4 == 0 ? hide.x : c4 == 1 ? hide.y : c4 == 2 ? hide.z : hide.w;
+        if (k0 + KT - 1 > pos_lo || any_hide || (p.window > 0 && pos_hi - k0 >= p.window && k0 + KT - 1 >= p.sinks)) {
+          const int lim = pos - k0;
+          const int wlo = p.window > 0 ? (int)max((int64_t)pos - p.window - k0, (int64_t)-1) : -1;  // hidden up to here
+          const int sk = (int)min(max((int64_t)p.sinks - k0, (int64_t)0), (int64_t)KT);
 #pragma unroll
-            for (int i = 0; i < 32; i++) {
-              const int k = c4 * 32 + i;
-              if (!(k <= lim && (k > wlo || k < sk)) || ((hw >> i) & 1u)) s[i] = 0xFF800000u;
+          for (int i = 0; i < 128; i++)
+            if (!(i <= lim && (i > wlo || i < sk))) s[i] = 0xFF800000u;
+          if (any_hide) {
+#pragma unroll
+            for (int i = 0; i < 128; i++) {
+              const uint32_t word = (i & 3) == 0 ? hide.x : (i & 3) == 1 ? hide.y : (i & 3) == 2 ? hide.z : hide.w;
+              if ((word >> (i >> 2)) & 1u) s[i] = 0xFF800000u;
             }
           }
-        };
-        uint32_t s[2][32];
-        tld32(t_s, s[0]);
-        tld_wait(s[0]);
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c4 = 0; c4 < 4; c4++) {
-          if (c4 < 3) tld32(t_s + 32 * (c4 + 1), s[(c4 + 1) & 1]);
-          mask(s[c4 & 1], c4);
-#pragma unroll
-          for (int i = 0; i < 32; i++) mx[i & 3] = fmaxf(mx[i & 3], u2f(s[c4 & 1][i]));
-          if (c4 < 3) tld_wait(s[(c4 + 1) & 1]);
         }
+        float mx[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) mx[k] = fmaxf(u2f(s[k]), u2f(s[4 + k]));
+#pragma unroll
+        for (int i = 8; i < 128; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; k++) mx[k] = fmaxf(mx[k], fmaxf(u2f(s[i + k]), u2f(s[i + 4 + k])));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * sc;
         const bool grow = top > base + 8.0f;               // also the first key of the row (base -inf)
         if (__any_sync(~0u, grow)) {
@@ -682,7 +754,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
           const float f = base == -INFINITY ? 0.0f : ex2(base - nb);
           sum *= f;
           base = nb;
-          if (t > w.t_begin) {                             // O holds the tiles before: wait for the last one, rescale
+          if (t > t_begin) {                               // O holds the tiles before: wait for the last one, rescale
             ok = bar_wait(pv_done + 8 * g, (tiles - 1) & 1, s_failed, 30 + g);
             if (!__all_sync(~0u, ok)) {
               ok = false;
@@ -703,22 +775,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
         const float off = C::SHIFT - (base == -INFINITY ? 0.0f : base);
         const float2 sc2 = make_float2(sc, sc), off2 = make_float2(off, off);
         float2 acc[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-        tld32(t_s, s[0]);
-        tld_wait(s[0]);
 #pragma unroll
-        for (int c4 = 0; c4 < 4; c4++) {                   // P overwrites columns of S that have been read
-          if (c4 < 3) tld32(t_s + 32 * (c4 + 1), s[(c4 + 1) & 1]);
-          mask(s[c4 & 1], c4);
+        for (int c4 = 0; c4 < 4; c4++) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; i++) {
-            float2 e = fma2(make_float2(u2f(s[c4 & 1][2 * i]), u2f(s[c4 & 1][2 * i + 1])), sc2, off2);
+            float2 e = fma2(make_float2(u2f(s[c4 * 32 + 2 * i]), u2f(s[c4 * 32 + 2 * i + 1])), sc2, off2);
             e.x = ex2(e.x);
             e.y = ex2(e.y);
             acc[i & 1] = add2(acc[i & 1], e);
             pk[i] = pack2<C::MF16>(e.x, e.y);
           }
-          if (c4 < 3) tld_wait(s[(c4 + 1) & 1]);
           tst16(t_s + 16 * c4, pk);
         }
         tst_wait();
@@ -739,20 +806,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
         break;
       }
       fence_after();
-      const bool begins = w.t_begin == 0, ends = w.t_end == w.b.units;
-      const bool whole = begins && ends;
-      if (tid == 0 && begins && !ends) {
-        const long long seg_end = w.seg_start + w.b.units;
-        long long last = c + 1;                            // the CTA whose share reaches the segment's end
-        while (last + 1 < ctas && (last + 1) * total / ctas < seg_end - slack) last++;
-        p.desc[c] = make_int4(w.r, w.b.qt, w.h, (int)last);
-      }
-      const float vs = C::FP8 && p.vs ? __ldg(p.vs + p.vs_step * w.h) : 1.0f;
+      const bool begins = t_begin == 0, whole = begins && t_end == sg->units;
+      if (tid == 0 && begins && !whole) p.desc[c] = make_int4(sg->r, sg->qt, h, sg->last);
+      const float vs = C::FP8 && p.vs ? __ldg(p.vs + p.vs_step * h) : 1.0f;
       const float inv = sum == 0.0f ? 0.0f : vs / sum;
       const float mine_base = base - C::SHIFT;
       float *part = p.part + (c * 2 + (begins ? 1 : 0)) * (int64_t)(QB * (DP + 2));
       const int brow = g * QT + my;
-      uint16_t *out = p.out + (int64_t)(rq.start + tok) * p.o_tok + (int64_t)head * p.o_head;
+      uint16_t *out = p.out + (int64_t)(sg->start + tok) * p.o_tok + (int64_t)head * p.o_head;
       bool odd = false;
 #pragma unroll 1
       for (int i = 0; i < DP / 32; i++) {
@@ -791,9 +852,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
         const int tok_s = __shfl_sync(~0u, tok, src), head_s = __shfl_sync(~0u, head, src), brow_s = __shfl_sync(~0u, brow, src);
         float m, l, ov[DP / 32];
         __syncwarp();
-        careful_row<F16, KV, DP, KT>(p, w.r, rq.start + tok_s, head_s, rq.first + tok_s, w.b.tl, w.t_begin, w.t_end, m, l, ov);
+        careful_row<F16, KV, DP, KT>(p, sg->r, sg->start + tok_s, head_s, first + tok_s, sg->tiles(), t_begin, t_end, m, l, ov);
         const float li = l == 0.0f ? 0.0f : vs / l;
-        uint16_t *os = p.out + (int64_t)(rq.start + tok_s) * p.o_tok + (int64_t)head_s * p.o_head;
+        uint16_t *os = p.out + (int64_t)(sg->start + tok_s) * p.o_tok + (int64_t)head_s * p.o_head;
 #pragma unroll
         for (int i = 0; i < DP / 32; i++) {
           const int d = lane + 32 * i;
@@ -808,13 +869,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_attention_tc_kernel(const
           part[QB * DP + QB + brow_s] = l;
         }
       }
+      __syncwarp();
+      if (lane == 0) bar_arrive(seg_empty + 8 * (segs % SEGS));
     }
   }
   // ---- teardown, reached by every role whether or not a wait ran out
   fence_before();
   __syncthreads();
   fence_after();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (warp == C::CTRL) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
 // Joins the parts of cut segments, as paged_merge_kernel does; blockIdx.y
@@ -853,29 +916,86 @@ __global__ void __launch_bounds__(128) paged_merge_tc_kernel(const AttnParams p)
   }
 }
 
+using TcKernel = void (*)(AttnParams, CUtensorMap, CUtensorMap, RowMap);
 struct TcVariant {
-  void (*main)(AttnParams);
+  TcKernel main;
   void (*merge)(AttnParams);
-  int smem;
+  int smem, threads;
 };
+template <bool F16, int KV, int DP>
+TcVariant tc_variant() {
+  return {paged_attention_tc_kernel<F16, KV, DP>, paged_merge_tc_kernel<F16, DP>, Tc<F16, KV, DP>::SMEM, Tc<F16, KV, DP>::THREADS};
+}
 template <bool F16, int KV>
 TcVariant pick_tc(int dp) {
-  if (dp == 64) return {paged_attention_tc_kernel<F16, KV, 64>, paged_merge_tc_kernel<F16, 64>, Tc<F16, KV, 64>::SMEM};
-  return {paged_attention_tc_kernel<F16, KV, 128>, paged_merge_tc_kernel<F16, 128>, Tc<F16, KV, 128>::SMEM};
+  return dp == 64 ? tc_variant<F16, KV, 64>() : tc_variant<F16, KV, 128>();
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static std::once_flag once;
+  static EncodeTiled fn = nullptr;
+  std::call_once(once, [] {
+    void *ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiled>(ptr);
+  });
+  return fn;
+}
+
+// The pool's rows: the common pitch of its slots, heads and pages.
+bool row_map(const AttnParams &p, RowMap &rm, int64_t &pitch) {
+  pitch = p.hk > 1 ? std::min(p.s_slot, p.s_head) : p.s_slot;
+  if (p.page == 1) pitch = p.hk > 1 ? std::min(p.s_page, p.s_head) : p.s_page;
+  if (p.pages < 1 || pitch < p.d || p.s_page % pitch || (p.page > 1 && p.s_slot % pitch) || (p.hk > 1 && p.s_head % pitch))
+    return false;
+  const int64_t page = p.s_page / pitch, slot = p.page > 1 ? p.s_slot / pitch : 0, head = p.hk > 1 ? p.s_head / pitch : 0;
+  const __int128 rows = (__int128)(p.pages - 1) * page + (__int128)(p.page - 1) * slot + (__int128)(p.hk - 1) * head + 1;
+  if (page < 0 || slot < 0 || head < 0 || rows >= INT32_MAX) return false;
+  rm = RowMap{(int)page, (int)slot, (int)head, (int)rows};
+  return true;
 }
 
 }  // namespace
 
 int64_t tc_workspace(int dp, int sms) { return (int64_t)sms * (2 * QB * (int64_t)(dp + 2) * 4 + 16); }
 
+bool tc_takes(const AttnParams &p) {
+  RowMap rm;
+  int64_t pitch;
+  return row_map(p, rm, pitch);
+}
+
 int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int sms, uint8_t *workspace, cudaStream_t st) {
   AttnParams p = params;
   p.desc = (int4 *)workspace;
   p.part = (float *)(workspace + (int64_t)sms * 16);
+  const bool fp8 = cache_dtype == FP8B200_E4M3 || cache_dtype == FP8B200_E5M2;
   TcVariant v;
   if (cache_dtype == FP8B200_E4M3) v = f16 ? pick_tc<true, FP8B200_E4M3>(dp) : pick_tc<false, FP8B200_E4M3>(dp);
   else if (cache_dtype == FP8B200_E5M2) v = f16 ? pick_tc<true, FP8B200_E5M2>(dp) : pick_tc<false, FP8B200_E5M2>(dp);
   else v = f16 ? pick_tc<true, FP8B200_F16>(dp) : pick_tc<false, FP8B200_BF16>(dp);
+  RowMap rm;
+  int64_t pitch;
+  if (!row_map(p, rm, pitch)) return set_error(FP8B200_EINVAL, "paged_attention: the cache's strides have no common row pitch");
+  EncodeTiled encode = encode_tiled();
+  if (!encode) return set_error(FP8B200_ELAUNCH, "paged_attention: cuTensorMapEncodeTiled not available");
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; i++) {
+    // a box is one row high: 64 16-bit values (one swizzled 128-byte row) or a head's float8 codes
+    const cuuint64_t dims[2] = {(cuuint64_t)p.d, (cuuint64_t)rm.rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)(pitch * (fp8 ? 1 : 2))};
+    const cuuint32_t box[2] = {(cuuint32_t)(fp8 ? dp : 64), 1}, step[2] = {1, 1};
+    const CUresult r = encode(&maps[i], fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
+                              const_cast<uint8_t *>(i ? p.v : p.k), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              fp8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(FP8B200_ELAUNCH, "paged_attention: tensor map encode failed (%d)", (int)r);
+  }
   if (cudaFuncSetAttribute(v.main, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem) != cudaSuccess)
     return check_launch("paged_attention");
   cudaLaunchConfig_t cfg = {};
@@ -883,12 +1003,12 @@ int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int s
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3((unsigned)sms);
-  cfg.blockDim = dim3(TC_THREADS);
+  cfg.blockDim = dim3((unsigned)v.threads);
   cfg.dynamicSmemBytes = (size_t)v.smem;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, v.main, p);
+  cudaLaunchKernelEx(&cfg, v.main, p, maps[0], maps[1], rm);
   cfg.gridDim = dim3((unsigned)sms, 8);
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = 0;
