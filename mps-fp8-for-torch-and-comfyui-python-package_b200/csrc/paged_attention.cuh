@@ -150,8 +150,7 @@ __device__ __forceinline__ float cache_value(const uint8_t *base, int64_t elem) 
 }
 
 // The kernel for many query rows (paged_attention_tc.cu): head sizes up to
-// 128, caches whose pages, slots and heads are all a multiple of one row pitch
-// apart (tc_takes).
+// 128, caches that a tensor map can describe (tc_takes).
 bool tc_takes(const AttnParams &p);
 int64_t tc_workspace(int dp, int sms);
 int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int sms, uint8_t *workspace, cudaStream_t st);

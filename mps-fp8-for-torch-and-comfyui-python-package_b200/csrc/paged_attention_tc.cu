@@ -12,9 +12,13 @@
 //   MMA      issues S = Q K^T and O += P V (a uniform warp, one lane's
 //            instructions: the descriptors stay in uniform registers)
 //   segments walks the CTA's share of the work and hands its segments on
-//   2 x TMA  in turn bring K and V tiles in, four rows of any pages a copy
-//            (tile::gather4), so every page size is alike; rows without a key
-//            are out of the map's bounds and arrive as zeros
+//   2 x TMA  in turn bring K and V tiles in, boxes of as many slots as divide
+//            both the page and the tile (16 for pages of 16 or 48 slots); boxes
+//            without a key are out of the map's bounds and arrive as zeros, a
+//            box that runs past the request's last key goes slot by slot, so
+//            that what an unwritten slot holds is never multiplied. (Gathering
+//            four rows a copy, tile::gather4, for all pages alike took 53
+//            cycles a copy: half the speed at 8 x 2048.)
 // While one group computes its weights the tensor core works for the other.
 // Tensor memory: S of either tile (128 columns each, P over its first 64) and
 // O of either tile.
@@ -53,10 +57,10 @@ constexpr unsigned long long WAIT_NS = 2000000000ull;
 
 __device__ uint32_t g_paged_status;  // 0, or the site of a wait that ran out
 
-// The pool as the tensor maps see it: rows of `pitch` elements, one per slot
-// and head. Slot s of page g under head h is row g * page + s * slot + h * head.
-struct RowMap {
-  int page, slot, head, rows;
+// Tensor maps of the caches, 4-D (head_dim, heads, slots of a page, pages):
+// boxes of 2^box_log slots, and of one.
+struct TcMaps {
+  CUtensorMap box[2], one[2];  // K, V
 };
 
 template <bool F16, int KV, int DP>
@@ -71,7 +75,7 @@ struct Tc {
   static constexpr int REGS_SOFTMAX = FP8 ? 184 : 216, REGS_OTHER = 72;
   static constexpr int SLOTS = DP == 128 ? (FP8 ? 4 : 5) : 8;
   static constexpr int RAWS = FP8 ? (DP == 128 ? 2 : 4) : 0;  // float8: raw tiles on their way
-  static constexpr int RAW = KT * DP;
+  static constexpr int RAW = KT * 128;                    // rows of 128 bytes: a copy's target must be 128-byte aligned
   static constexpr int OFF_KV = 2 * TILE;
   static constexpr int OFF_RAW = OFF_KV + SLOTS * TILE;
   static constexpr int OFF_PLAN = OFF_RAW + RAWS * RAW;   // the plan's scratch
@@ -219,12 +223,11 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t a, uint32_t lead) {
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// Columns x .. of four rows, each the map's box wide and one high.
-__device__ __forceinline__ void gather4(uint32_t dst, const CUtensorMap *map, int x, const int (&row)[4], uint32_t bar) {
+// A box of the pool: columns x .., key/value head h, slots off .. of one page.
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, int x, int h, int off, int page, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
-      "%6}], [%7];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(bar)
+      "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(h), "r"(off), "r"(page), "r"(bar)
       : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -300,8 +303,7 @@ static_assert(sizeof(Segment) == 48, "SEGS * 48 bytes");
 
 template <bool F16, int KV, int DP>
 __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
-    paged_attention_tc_kernel(const AttnParams p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                              const RowMap rm) {
+    paged_attention_tc_kernel(const AttnParams p, const __grid_constant__ TcMaps maps, const int box_log) {
   using C = Tc<F16, KV, DP>;
   constexpr int TC_THREADS = C::THREADS;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -555,9 +557,9 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
       for (uint32_t segs = 0; ok; segs++) {
         const Segment *sg = seg_at(segs, 52);
         if (!__all_sync(~0u, sg != nullptr) || sg->r < 0) break;
-        const int r = sg->r, n = sg->t_end - sg->t_begin;
-        const int hi = sg->first + (int)((min((int64_t)sg->n * p.group, (int64_t)(sg->qt + 1) * QB) - 1) / p.group);
-        const int head_row = sg->h * rm.head;
+        const int r = sg->r, h = sg->h, n = sg->t_end - sg->t_begin;
+        const int last = sg->first + sg->n - 1;           // the request's last key
+        const int B = 1 << box_log, boxes = KT >> box_log;
 #pragma unroll 1
         for (int i = 0; i < 2 * n; i++, filled++) {
           const bool keys = i == 0 || ((i & 1) && i < 2 * n - 1);
@@ -565,42 +567,53 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
           tiles += keys;
           if ((filled & 1u) != turn) continue;
           const int t = sg->t_begin + (keys ? (i + 1) / 2 : i == 2 * n - 1 ? n - 1 : i / 2 - 1);
-          const int k0 = sg->tile(t) * KT + 4 * lane;
-          int row[4];
-          uint32_t hide[4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int j = k0 + e;
-            row[e] = rm.rows;                             // out of bounds: zeros
-            if (j <= hi) {
-              const uint32_t col = (uint32_t)j / (uint32_t)p.page;
-              int page = -1;
-              if (col < (uint32_t)p.table_cols) page = __ldg(p.table + (int64_t)r * p.table_ld + col);
-              if (page >= 0 && page < p.pages) row[e] = page * rm.page + (int)((uint32_t)j - col * (uint32_t)p.page) * rm.slot + head_row;
-            }
-            hide[e] = __ballot_sync(~0u, j <= hi && row[e] == rm.rows);
-          }
+          const int k0 = sg->tile(t) * KT;
           const uint32_t at = filled % RING, turns = filled / RING;
-          if (filled >= RING) ok = bar_wait(C::FP8 ? raw_empty(at) : kv_empty(at), (turns & 1) ^ 1, s_failed, 10);
-          ok = __all_sync(~0u, ok);
-          if (!ok) break;
           const uint32_t bar = C::FP8 ? raw_full(at) : kv_full(at);
           const uint32_t dst = C::FP8 ? raw_a + at * C::RAW : kv_a + at * C::TILE;
-          if (lane == 0) {
-            if (keys) {                                   // key 4 i + e is bit i of word e
-#pragma unroll
-              for (int e = 0; e < 4; e++) s_hide[(number % HIDE_RING) * 4 + e] = hide[e];
+          const CUtensorMap *map = &maps.box[keys ? 0 : 1], *one = &maps.one[keys ? 0 : 1];
+          constexpr uint32_t row_bytes = 128;
+#pragma unroll 1
+          for (int b0 = 0; b0 < boxes; b0 += 32) {        // once, unless a page's slots are odd or twice odd
+            const int b = b0 + lane, j = k0 + (b << box_log);
+            int page = -1, off = 0;
+            if (b < boxes && j <= last) {
+              const uint32_t col = (uint32_t)j / (uint32_t)p.page;
+              off = (int)((uint32_t)j - col * (uint32_t)p.page);
+              if (col < (uint32_t)p.table_cols) page = __ldg(p.table + (int64_t)r * p.table_ld + col);
+              if (page >= p.pages) page = -1;
             }
-            bar_expect(bar, C::FP8 ? C::RAW : C::TILE);
-          }
-          __syncwarp();
-          const CUtensorMap *map = keys ? &map_k : &map_v;
-          if constexpr (C::FP8) {
-            gather4(dst + lane * 4 * DP, map, 0, row, bar);
-          } else {
+            const uint32_t hide = __ballot_sync(~0u, b < boxes && j <= last && page < 0);
+            if (b0 == 0) {
+              if (filled >= RING) ok = bar_wait(C::FP8 ? raw_empty(at) : kv_empty(at), (turns & 1) ^ 1, s_failed, 10);
+              ok = __all_sync(~0u, ok);
+              if (!ok) break;
+              if (lane == 0) {
+                if (keys) {
 #pragma unroll
-            for (int b = 0; b < DP / 64; b++) gather4(dst + b * (KT * 128) + lane * 512, map, b * 64, row, bar);
+                  for (int e = 1; e < 4; e++) s_hide[(number % HIDE_RING) * 4 + e] = 0;
+                }
+                bar_expect(bar, C::FP8 ? C::RAW : C::TILE);
+              }
+            }
+            if (lane == 0 && keys) s_hide[(number % HIDE_RING) * 4 + (b0 >> 5)] = hide;  // bit b: box b
+            __syncwarp();
+            if (b < boxes) {
+              const uint32_t to = dst + (uint32_t)(b << box_log) * row_bytes;
+              const int pg = page < 0 ? (int)p.pages : page;  // behind the last page: zeros
+              if (page < 0 || j + B - 1 <= last) {
+                load_box(to, map, 0, h, off, pg, bar);
+                if constexpr (!C::FP8 && DP == 128) load_box(to + KT * 128, map, 64, h, off, pg, bar);
+              } else {
+                for (int e = 0; e < B; e++) {
+                  const int pe = j + e <= last ? page : (int)p.pages;
+                  load_box(to + e * row_bytes, one, 0, h, off + e, pe, bar);
+                  if constexpr (!C::FP8 && DP == 128) load_box(to + e * row_bytes + KT * 128, one, 64, h, off + e, pe, bar);
+                }
+              }
+            }
           }
+          if (!ok) break;
         }
         __syncwarp();
         if (lane == 0) bar_arrive(seg_empty + 8 * (segs % SEGS));
@@ -627,11 +640,11 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
           ok = bar_wait(raw_full(rs), (done / C::RAWS) & 1, s_failed, 11);
           if (done >= C::SLOTS) ok = ok && bar_wait(kv_empty(ks), ((done / C::SLOTS) & 1) ^ 1, s_failed, 12);
           if (!ok) break;
-          const uint32_t raw = raw_a + rs * C::RAW + pt * 16, dst = kv_a + ks * C::TILE + at8;
+          const uint32_t raw = raw_a + rs * C::RAW + row0 * 128 + cu * 16, dst = kv_a + ks * C::TILE + at8;
 #pragma unroll
           for (int k = 0; k < UNITS; k++) {
             uint32_t q[4];
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(raw + k * 2048));
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(raw + k * (STEP * 128)));
             sts16(dst + k * (STEP * 128) + ((u8 ^ x) << 4), fp8x2_to_f16x2<KV>(q[0] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[0] >> 16),
                   fp8x2_to_f16x2<KV>(q[1] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[1] >> 16));
             sts16(dst + k * (STEP * 128) + (((u8 + 1) ^ x) << 4), fp8x2_to_f16x2<KV>(q[2] & 0xFFFFu),
@@ -735,8 +748,9 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
           if (any_hide) {
 #pragma unroll
             for (int i = 0; i < 128; i++) {
-              const uint32_t word = (i & 3) == 0 ? hide.x : (i & 3) == 1 ? hide.y : (i & 3) == 2 ? hide.z : hide.w;
-              if ((word >> (i >> 2)) & 1u) s[i] = 0xFF800000u;
+              const int b = i >> box_log;
+              const uint32_t word = b < 32 ? hide.x : b < 64 ? hide.y : b < 96 ? hide.z : hide.w;
+              if ((word >> (b & 31)) & 1u) s[i] = 0xFF800000u;
             }
           }
         }
@@ -916,7 +930,7 @@ __global__ void __launch_bounds__(128) paged_merge_tc_kernel(const AttnParams p)
   }
 }
 
-using TcKernel = void (*)(AttnParams, CUtensorMap, CUtensorMap, RowMap);
+using TcKernel = void (*)(AttnParams, TcMaps, int);
 struct TcVariant {
   TcKernel main;
   void (*merge)(AttnParams);
@@ -947,27 +961,15 @@ EncodeTiled encode_tiled() {
   return fn;
 }
 
-// The pool's rows: the common pitch of its slots, heads and pages.
-bool row_map(const AttnParams &p, RowMap &rm, int64_t &pitch) {
-  pitch = p.hk > 1 ? std::min(p.s_slot, p.s_head) : p.s_slot;
-  if (p.page == 1) pitch = p.hk > 1 ? std::min(p.s_page, p.s_head) : p.s_page;
-  if (p.pages < 1 || pitch < p.d || p.s_page % pitch || (p.page > 1 && p.s_slot % pitch) || (p.hk > 1 && p.s_head % pitch))
-    return false;
-  const int64_t page = p.s_page / pitch, slot = p.page > 1 ? p.s_slot / pitch : 0, head = p.hk > 1 ? p.s_head / pitch : 0;
-  const __int128 rows = (__int128)(p.pages - 1) * page + (__int128)(p.page - 1) * slot + (__int128)(p.hk - 1) * head + 1;
-  if (page < 0 || slot < 0 || head < 0 || rows >= INT32_MAX) return false;
-  rm = RowMap{(int)page, (int)slot, (int)head, (int)rows};
-  return true;
-}
-
 }  // namespace
 
 int64_t tc_workspace(int dp, int sms) { return (int64_t)sms * (2 * QB * (int64_t)(dp + 2) * 4 + 16); }
 
+// What a tensor map can describe: strides above 0 (below 2^40 bytes), extents below 2^31.
 bool tc_takes(const AttnParams &p) {
-  RowMap rm;
-  int64_t pitch;
-  return row_map(p, rm, pitch);
+  const int64_t most = (int64_t)1 << 38;
+  auto fits = [&](int64_t n, int64_t stride) { return n == 1 || (stride > 0 && stride < most); };
+  return p.pages > 0 && p.pages < INT32_MAX && fits(p.hk, p.s_head) && fits(p.page, p.s_slot) && fits(p.pages, p.s_page);
 }
 
 int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int sms, uint8_t *workspace, cudaStream_t st) {
@@ -979,19 +981,20 @@ int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int s
   if (cache_dtype == FP8B200_E4M3) v = f16 ? pick_tc<true, FP8B200_E4M3>(dp) : pick_tc<false, FP8B200_E4M3>(dp);
   else if (cache_dtype == FP8B200_E5M2) v = f16 ? pick_tc<true, FP8B200_E5M2>(dp) : pick_tc<false, FP8B200_E5M2>(dp);
   else v = f16 ? pick_tc<true, FP8B200_F16>(dp) : pick_tc<false, FP8B200_BF16>(dp);
-  RowMap rm;
-  int64_t pitch;
-  if (!row_map(p, rm, pitch)) return set_error(FP8B200_EINVAL, "paged_attention: the cache's strides have no common row pitch");
   EncodeTiled encode = encode_tiled();
   if (!encode) return set_error(FP8B200_ELAUNCH, "paged_attention: cuTensorMapEncodeTiled not available");
-  CUtensorMap maps[2];
-  for (int i = 0; i < 2; i++) {
-    // a box is one row high: 64 16-bit values (one swizzled 128-byte row) or a head's float8 codes
-    const cuuint64_t dims[2] = {(cuuint64_t)p.d, (cuuint64_t)rm.rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)(pitch * (fp8 ? 1 : 2))};
-    const cuuint32_t box[2] = {(cuuint32_t)(fp8 ? dp : 64), 1}, step[2] = {1, 1};
-    const CUresult r = encode(&maps[i], fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2,
-                              const_cast<uint8_t *>(i ? p.v : p.k), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+  int box_log = 0;  // slots a box: the largest power of two that divides the page and the tile
+  while (box_log < 7 && !((p.page >> box_log) & 1)) box_log++;
+  TcMaps maps;
+  for (int i = 0; i < 4; i++) {
+    // 64 16-bit values (one swizzled 128-byte row) or a head's float8 codes wide
+    const int64_t esz = fp8 ? 1 : 2, any = (int64_t)p.d * esz;
+    const cuuint64_t dims[4] = {(cuuint64_t)p.d, (cuuint64_t)p.hk, (cuuint64_t)p.page, (cuuint64_t)p.pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)(p.hk > 1 ? p.s_head * esz : any), (cuuint64_t)(p.page > 1 ? p.s_slot * esz : any),
+                                   (cuuint64_t)(p.pages > 1 ? p.s_page * esz : any)};
+    const cuuint32_t box[4] = {fp8 ? 128u : 64u, 1, i < 2 ? 1u << box_log : 1u, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = encode(i < 2 ? &maps.box[i] : &maps.one[i - 2], fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_UINT16,
+                              4, const_cast<uint8_t *>(i & 1 ? p.v : p.k), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               fp8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(FP8B200_ELAUNCH, "paged_attention: tensor map encode failed (%d)", (int)r);
@@ -1008,7 +1011,7 @@ int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int s
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, v.main, p, maps[0], maps[1], rm);
+  cudaLaunchKernelEx(&cfg, v.main, p, maps, box_log);
   cfg.gridDim = dim3((unsigned)sms, 8);
   cfg.blockDim = dim3(128);
   cfg.dynamicSmemBytes = 0;
