@@ -28,9 +28,10 @@
 // nothing overflows and the quotient is the same): after the first tiles that
 // is rare, and the O accumulator stays in tensor memory.
 //
-// Work: the units (key tiles) of all segments in one line, cut into one share
-// a CTA; a cut within a sixteenth of a share of a segment's edge moves there,
-// so with many segments none is split, and with few all SMs still work.
+// Work: the units (key tiles, and SEG_COST more for its start and end) of all
+// segments in one line, cut into one share a CTA; a cut within a sixteenth of a
+// share of a segment's edge moves there, so with many segments none is split,
+// and with few all SMs still work.
 //
 // Bound by the tensor core and the exponentials alike: 256 x 128 scores cost
 // 2048 cycles of MMA at head size 128 and 2048 cycles of ex2 (16 a cycle).
@@ -51,6 +52,7 @@ namespace {
 constexpr int KT = 128;          // keys a tile
 constexpr int QT = 128;          // rows a tile
 constexpr int QB = 2 * QT;       // rows a block
+constexpr int SEG_COST = 2;       // what a segment's start and end cost, in key tiles
 constexpr int SEGS = 4;           // segments in the ring
 constexpr int HIDE_RING = 8;     // tiles whose page masks are kept: more than the producers run ahead of the softmax
 constexpr unsigned long long WAIT_NS = 2000000000ull;
@@ -253,26 +255,28 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 // Blocks of rows have places x: request r's from place(r) on, where place(r)
 // = floor(rows before r / 256) + r leaves room for its last, partial block
 // (some places stay empty). A place's segments, one a key/value head, follow
-// one another; a segment's units are the key tiles its 256 rows can see.
+// one another; a segment's units are the key tiles its 256 rows can see, and
+// SEG_COST behind them.
 __device__ __forceinline__ int place(const AttnParams &p, int start, int r) {
   return (int)((int64_t)start * p.group / QB) + r;
 }
 struct Block {
   Request rq;
   Tiles<KT> tl;
-  int qt, units;  // 0 units: the place is empty
+  int qt, tiles;  // 0 tiles: the place is empty
+  __device__ __forceinline__ int units() const { return tiles ? tiles + SEG_COST : 0; }
 };
 __device__ __forceinline__ Block block_at(const AttnParams &p, const Request &rq, int qt) {
   Block b;
   b.rq = rq;
   b.qt = qt;
   const int64_t rows = (int64_t)rq.n * p.group;
-  b.units = 0;
+  b.tiles = 0;
   b.tl = Tiles<KT>{0, 0, 0};
   if (rq.n == 0 || !takes(p, rq.n) || (int64_t)qt * QB >= rows) return b;
   const int last = (int)(min(rows, (int64_t)(qt + 1) * QB) - 1);
   b.tl = visible_tiles<KT>(p, rq.first + qt * QB / p.group, rq.first + last / p.group);
-  b.units = max(1, b.tl.count());
+  b.tiles = max(1, b.tl.count());
   return b;
 }
 // Within a request the last blocks, which see the most keys, come first.
@@ -282,7 +286,7 @@ __device__ __forceinline__ Block block_of_place(const AttnParams &p, int r, int 
   const int i = x - place(p, rq.start, r);
   if (i < 0 || i >= n) {
     Block b;
-    b.rq = rq, b.qt = 0, b.units = 0;
+    b.rq = rq, b.qt = 0, b.tiles = 0;
     b.tl = Tiles<KT>{0, 0, 0};
     return b;
   }
@@ -293,7 +297,7 @@ __device__ __forceinline__ Block block_of_place(const AttnParams &p, int r, int 
 struct alignas(16) Segment {
   int r, h, qt;                // request (-1: no more segments), key/value head, block of rows
   int start, n, first;         // the request's new tokens (see Request)
-  int t_begin, t_end, units;   // key tiles [t_begin, t_end) of `units`
+  int t_begin, t_end, units;   // key tiles [t_begin, t_end) of `units` tiles
   int sinks, from;             // list entry i is key tile i < sinks ? i : from + i - sinks
   int last;                    // if the part begins the segment and does not end it: the CTA that ends it
   __device__ __forceinline__ int tile(int i) const { return i < sinks ? i : from + i - sinks; }
@@ -373,7 +377,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
     return lo;
   };
   long long total = 0;
-  for (int x = tid; x < places; x += TC_THREADS) total += (long long)block_of_place(p, request_of(x), x).units * p.hk;
+  for (int x = tid; x < places; x += TC_THREADS) total += (long long)block_of_place(p, request_of(x), x).units() * p.hk;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
   if (lane == 0) s_sum[warp] = total;
@@ -393,7 +397,10 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
     for (int x0 = 0; x0 < places; x0 += TC_THREADS) {
       const int x = x0 + tid;
       const int r = x < places ? request_of(x) : 0;
-      const int units = x < places ? block_of_place(p, r, x).units : 0;
+      Block blk;
+      blk.tiles = 0;
+      if (x < places) blk = block_of_place(p, r, x);
+      const int units = blk.units();
       const long long mine = (long long)units * p.hk;
       long long inc = mine;
 #pragma unroll
@@ -414,7 +421,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
           const long long in = (raw[k] - b) % units;  // of the segment that the cut falls into
           long long cut = raw[k];
           if (in <= slack) cut -= in;
-          else if (units - in <= slack) cut += units - in;
+          else if (in >= blk.tiles - slack) cut += units - in;
           s_found[k][0] = cut, s_found[k][1] = x, s_found[k][2] = b, s_found[k][3] = r;
         }
       __syncthreads();
@@ -450,29 +457,30 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
           sg.r = -1;
           while (u < u_end && u_r < p.requests) {
             const Block b = block_of_place(p, u_r, u_x);
-            const long long all = (long long)b.units * p.hk;
+            const int units = b.units();
+            const long long all = (long long)units * p.hk;
             if (u < u_before + all) {
               const int local = (int)(u - u_before);       // units of one place: below 2^31
-              sg.r = u_r, sg.h = local / b.units, sg.qt = b.qt;
+              sg.r = u_r, sg.h = local / units, sg.qt = b.qt;
               sg.start = b.rq.start, sg.n = b.rq.n, sg.first = b.rq.first;
-              sg.t_begin = local - sg.h * b.units;
-              sg.t_end = (int)min((long long)b.units, sg.t_begin + (u_end - u));
-              sg.units = b.units, sg.sinks = b.tl.sinks, sg.from = b.tl.from;
-              const long long seg_end = u - sg.t_begin + b.units;
+              sg.t_begin = local - sg.h * units;
+              sg.t_end = (int)min((long long)b.tiles, sg.t_begin + (u_end - u));
+              sg.units = b.tiles, sg.sinks = b.tl.sinks, sg.from = b.tl.from;
+              const long long tiles_end = u - sg.t_begin + b.tiles;
               sg.last = 0;
-              if (sg.t_begin == 0 && sg.t_end < sg.units) {
+              if (sg.t_begin == 0 && sg.t_end < b.tiles) {
                 long long last = c + 1;                    // the CTA whose share reaches the segment's end
-                while (last + 1 < ctas && (last + 1) * total / ctas < seg_end - slack) last++;
+                while (last + 1 < ctas && (last + 1) * total / ctas < tiles_end - slack) last++;
                 sg.last = (int)last;
               }
-              u += sg.t_end - sg.t_begin;
+              u = sg.t_end == b.tiles ? tiles_end + SEG_COST : u + (sg.t_end - sg.t_begin);
               break;
             }
             u_before += all;
             u_x++;
             while (u_r + 1 < p.requests && u_x >= place(p, load_request(p, u_r + 1).start, u_r + 1)) u_r++;
             // behind the last request's places nothing is left (only if the offsets make no sense)
-            if (u_r + 1 == p.requests && b.units == 0 &&
+            if (u_r + 1 == p.requests && b.tiles == 0 &&
                 (long long)(u_x - place(p, b.rq.start, u_r)) * QB > (long long)b.rq.n * p.group + QB)
               break;
           }
@@ -626,7 +634,9 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
       const int pt = tid - 8 * 32;
       constexpr int CPR = DP / 16, STEP = 128 / CPR, UNITS = KT / STEP;  // a thread's units lie STEP rows apart
       static_assert(STEP % 8 == 0, "a thread's rows share their place in the swizzle");
-      const int cu = pt % CPR, row0 = pt / CPR, x = row0 & 7, u8 = (cu & 3) * 2;
+      const int cu = pt % CPR, row0 = pt / CPR, x = row0 & 7;
+      // the halves' order alternates between the column blocks, so that the eight lanes of a row meet eight bank groups
+      const int swap = cu >> 2, u0 = (cu & 3) * 2 + swap, u1 = (cu & 3) * 2 + 1 - swap;
       const uint32_t at8 = (uint32_t)((cu >> 2) * (KT * 128) + row0 * 128);
       uint32_t done = 0;
       bool ok = true;
@@ -645,10 +655,11 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
           for (int k = 0; k < UNITS; k++) {
             uint32_t q[4];
             asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]) : "r"(raw + k * (STEP * 128)));
-            sts16(dst + k * (STEP * 128) + ((u8 ^ x) << 4), fp8x2_to_f16x2<KV>(q[0] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[0] >> 16),
-                  fp8x2_to_f16x2<KV>(q[1] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[1] >> 16));
-            sts16(dst + k * (STEP * 128) + (((u8 + 1) ^ x) << 4), fp8x2_to_f16x2<KV>(q[2] & 0xFFFFu),
-                  fp8x2_to_f16x2<KV>(q[2] >> 16), fp8x2_to_f16x2<KV>(q[3] & 0xFFFFu), fp8x2_to_f16x2<KV>(q[3] >> 16));
+            const uint32_t a0 = swap ? q[2] : q[0], a1 = swap ? q[3] : q[1], b0 = swap ? q[0] : q[2], b1 = swap ? q[1] : q[3];
+            sts16(dst + k * (STEP * 128) + ((u0 ^ x) << 4), fp8x2_to_f16x2<KV>(a0 & 0xFFFFu), fp8x2_to_f16x2<KV>(a0 >> 16),
+                  fp8x2_to_f16x2<KV>(a1 & 0xFFFFu), fp8x2_to_f16x2<KV>(a1 >> 16));
+            sts16(dst + k * (STEP * 128) + ((u1 ^ x) << 4), fp8x2_to_f16x2<KV>(b0 & 0xFFFFu), fp8x2_to_f16x2<KV>(b0 >> 16),
+                  fp8x2_to_f16x2<KV>(b1 & 0xFFFFu), fp8x2_to_f16x2<KV>(b1 >> 16));
           }
           bar_arrive(raw_empty(rs));
           fence_async();
@@ -668,9 +679,66 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
     const uint32_t q_a = base_a + g * C::TILE;
     uint32_t tiles = 0;
     bool ok = true;
-    for (uint32_t segs = 0; ok; segs++) {
-      const Segment *sg = seg_at(segs, 53);
-      if (!__all_sync(~0u, sg != nullptr) || sg->r < 0) break;
+    // The group's rows of Q for a segment. A row takes DP / 8 lanes, so that a
+    // warp reads whole rows; the owner of row r gets its scale from them.
+    float qscale = 1.0f;
+    auto load_q = [&](const Segment *sg) {
+      constexpr int LPR = DP / 8, RPI = 32 / LPR;          // lanes a row, rows an instruction
+      const int cu = lane % LPR, sub = lane / LPR;
+      const int all_rows = sg->n * p.group, row0 = sg->qt * QB + g * QT + (warp & 3) * 32;
+      const int own = min(row0 + lane, all_rows - 1), own_tok = own / p.group;
+      const int64_t own_at = (int64_t)(sg->start + own_tok) * p.q_tok + (int64_t)(sg->h * p.group + own - own_tok * p.group) * p.q_head;
+      // its sign takes that of the scale, so that the maximum of the products is the maximum of the scores
+      const uint32_t flip = p.scale_log2 * (C::FP8 && p.ks ? __ldg(p.ks + p.ks_step * sg->h) : 1.0f) < 0.0f ? 0x80008000u : 0u;
+      constexpr int BATCH = C::FP8 || DP == 64 ? 8 : 16;   // loads in flight
+#pragma unroll 1
+      for (int i0 = 0; i0 < 32 / RPI; i0 += BATCH) {
+        uint4 v[BATCH];
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {
+          const int row = (i0 + k) * RPI + sub;
+          const int64_t at = __shfl_sync(~0u, own_at, row);
+          v[k] = make_uint4(0, 0, 0, 0);
+          if (row0 + row < all_rows && cu * 8 < p.d) v[k] = __ldg(reinterpret_cast<const uint4 *>(p.q + at) + cu);
+        }
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {
+          const int row = (i0 + k) * RPI + sub, my_row = (warp & 3) * 32 + row;
+          uint32_t x[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+          if constexpr (C::FP8 && !F16) {                  // bf16 to f16, the largest value in [1, 2)
+            float a = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) a = fmaxf(a, fmaxf(fabsf(u2f(x[e] << 16)), fabsf(u2f(x[e] & 0xFFFF0000u))));
+#pragma unroll
+            for (int d = LPR / 2; d > 0; d >>= 1) a = fmaxf(a, __shfl_xor_sync(~0u, a, d));
+            uint32_t eb = f2u(a) >> 23;
+            eb = (eb == 255u || a == 0.0f) ? 127u : min(max(eb, 1u), 253u);
+            const float mul = u2f((254u - eb) << 23);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = pack2<true>(u2f(x[e] << 16) * mul, u2f(x[e] & 0xFFFF0000u) * mul);
+            const float qs = __shfl_sync(~0u, u2f(eb << 23), (lane % RPI) * LPR);  // of row (i0 + k) * RPI + lane % RPI
+            if (lane / RPI == i0 + k) qscale = qs;
+          }
+          sts16(q_a + (cu >> 3) * (QT * 128) + my_row * 128 + (((cu & 7) ^ (my_row & 7)) << 4), x[0] ^ flip, x[1] ^ flip,
+                x[2] ^ flip, x[3] ^ flip);
+        }
+      }
+      fence_async();
+      bar_arrive(q_full + 8 * g);
+    };
+    // Its rows into L2, a segment ahead.
+    auto prefetch_q = [&](const Segment *sg) {
+      const int row = sg->qt * QB + g * QT + my;
+      if (row < sg->n * p.group) {
+        const int tok = row / p.group;
+        const uint16_t *at = p.q + (int64_t)(sg->start + tok) * p.q_tok + (int64_t)(sg->h * p.group + row - tok * p.group) * p.q_head;
+        for (int d = 0; d < p.d; d += 64) asm volatile("prefetch.global.L2 [%0];" ::"l"(at + d));
+      }
+    };
+    const Segment *sg = seg_at(0, 53);
+    if (!__all_sync(~0u, sg != nullptr)) ok = false;
+    if (ok && sg->r >= 0) load_q(sg);
+    for (uint32_t segs = 0; ok && sg->r >= 0; segs++) {
       const int h = sg->h, first = sg->first, t_begin = sg->t_begin, t_end = sg->t_end;
       const int all_rows = sg->n * p.group;                // below 2^31: tokens x query heads are
       const int row0 = sg->qt * QB + g * QT;               // the tile's first row; it may lie behind the request's last
@@ -680,48 +748,15 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
       const int pos = first + tok;
       const int pos_lo = first + min(row0, all_rows - 1) / p.group;
       const int pos_hi = first + (min(row0 + QT, all_rows) - 1) / p.group;
-      const int64_t q_row = (int64_t)(sg->start + tok) * p.q_tok + (int64_t)head * p.q_head;
-      // ---- the row of Q (the previous segment's products with this tile are complete: its last S was waited for)
-      // its sign takes that of the scale, so that the maximum of the products is the maximum of the scores
-      float qscale = 1.0f;
-      const float scale = p.scale_log2 * (C::FP8 && p.ks ? __ldg(p.ks + p.ks_step * h) : 1.0f);
-      const float sign = scale < 0.0f ? -1.0f : 1.0f;
-      {
-        const uint16_t *qp = p.q + q_row;
-        float mul = sign;
-        if constexpr (C::FP8 && !F16) {                    // bf16 to f16, the largest value in [1, 2)
-          float a = 0.0f;
-          for (int i = 0; i < p.d / 8; i++) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(qp) + i);
-            const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) a = fmaxf(a, fmaxf(fabsf(u2f(x[e] << 16)), fabsf(u2f(x[e] & 0xFFFF0000u))));
-          }
-          uint32_t eb = f2u(a) >> 23;
-          eb = (eb == 255u || a == 0.0f) ? 127u : min(max(eb, 1u), 253u);
-          mul = u2f((254u - eb) << 23) * sign;
-          qscale = u2f(eb << 23);
-        }
-#pragma unroll 4
-        for (int i = 0; i < DP / 8; i++) {
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (mine && i * 8 < p.d) v = __ldg(reinterpret_cast<const uint4 *>(qp) + i);
-          uint32_t x[4] = {v.x, v.y, v.z, v.w};
-          if constexpr (C::FP8 && !F16) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = pack2<true>(u2f(x[e] << 16) * mul, u2f(x[e] & 0xFFFF0000u) * mul);
-          } else if (sign < 0.0f) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[e] ^= 0x80008000u;
-          }
-          sts16(q_a + (i >> 3) * (QT * 128) + my * 128 + (((i & 7) ^ (my & 7)) << 4), x[0], x[1], x[2], x[3]);
-        }
-        fence_async();
-        bar_arrive(q_full + 8 * g);
-      }
       // a scale of 0 weighs all keys alike; kept above 0 so that a hidden key's -inf stays one
-      float sc = fabsf(scale) * qscale;
+      float sc = fabsf(p.scale_log2 * (C::FP8 && p.ks ? __ldg(p.ks + p.ks_step * h) : 1.0f)) * qscale;
       if (sc == 0.0f) sc = 1e-30f;
+      const Segment *next = seg_at(segs + 1, 55);
+      if (!__all_sync(~0u, next != nullptr)) {
+        ok = false;
+        break;
+      }
+      if (next->r >= 0) prefetch_q(next);
       float base = -INFINITY, sum = 0.0f;                  // of this row: weights are 2^(score - base + SHIFT)
       for (int t = t_begin; t < t_end; t++) {
         const int k0 = sg->tile(t) * KT;
@@ -738,20 +773,23 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
         for (int i = 0; i < 4; i++) tld_wait(s + 32 * i);
         const uint4 hide = *reinterpret_cast<const uint4 *>(s_hide + (tiles % HIDE_RING) * 4);
         const bool any_hide = (hide.x | hide.y | hide.z | hide.w) != 0u;
-        if (k0 + KT - 1 > pos_lo || any_hide || (p.window > 0 && pos_hi - k0 >= p.window && k0 + KT - 1 >= p.sinks)) {
+        if (k0 + KT - 1 > pos_lo) {                          // keys behind the query
           const int lim = pos - k0;
-          const int wlo = p.window > 0 ? (int)max((int64_t)pos - p.window - k0, (int64_t)-1) : -1;  // hidden up to here
+#pragma unroll
+          for (int i = 0; i < 128; i++) s[i] = i > lim ? 0xFF800000u : s[i];
+        }
+        if (p.window > 0 && pos_hi - k0 >= p.window && k0 + KT - 1 >= p.sinks) {  // before its window, behind the sinks
+          const int wlo = (int)max((int64_t)pos - p.window - k0, (int64_t)-1);
           const int sk = (int)min(max((int64_t)p.sinks - k0, (int64_t)0), (int64_t)KT);
 #pragma unroll
-          for (int i = 0; i < 128; i++)
-            if (!(i <= lim && (i > wlo || i < sk))) s[i] = 0xFF800000u;
-          if (any_hide) {
+          for (int i = 0; i < 128; i++) s[i] = i <= wlo && i >= sk ? 0xFF800000u : s[i];
+        }
+        if (any_hide) {                                      // without a page
 #pragma unroll
-            for (int i = 0; i < 128; i++) {
-              const int b = i >> box_log;
-              const uint32_t word = b < 32 ? hide.x : b < 64 ? hide.y : b < 96 ? hide.z : hide.w;
-              if ((word >> (b & 31)) & 1u) s[i] = 0xFF800000u;
-            }
+          for (int i = 0; i < 128; i++) {
+            const int b = i >> box_log;
+            const uint32_t word = b < 32 ? hide.x : b < 64 ? hide.y : b < 96 ? hide.z : hide.w;
+            if ((word >> (b & 31)) & 1u) s[i] = 0xFF800000u;
           }
         }
         float mx[4];
@@ -813,6 +851,8 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
         ok = false;
         break;
       }
+      // ---- the next segment's rows of Q: the last S, for which all have waited, was the last reader of these
+      if (next->r >= 0) load_q(next);
       // ---- the segment's end
       ok = bar_wait(pv_done + 8 * g, (tiles - 1) & 1, s_failed, 40 + g);
       if (!__all_sync(~0u, ok)) {
@@ -827,7 +867,10 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
       const float mine_base = base - C::SHIFT;
       float *part = p.part + (c * 2 + (begins ? 1 : 0)) * (int64_t)(QB * (DP + 2));
       const int brow = g * QT + my;
-      uint16_t *out = p.out + (int64_t)(sg->start + tok) * p.o_tok + (int64_t)head * p.o_head;
+      const int64_t out_at = (int64_t)(sg->start + tok) * p.o_tok + (int64_t)head * p.o_head;
+      int64_t to[4];                                       // of the rows that this lane stores, -1 for none
+#pragma unroll
+      for (int q = 0; q < 4; q++) to[q] = __shfl_sync(~0u, mine ? out_at : (int64_t)-1, (lane & ~3) + q);
       bool odd = false;
 #pragma unroll 1
       for (int i = 0; i < DP / 32; i++) {
@@ -839,15 +882,36 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
 #pragma unroll
           for (int e = 0; e < 32; e++) odd |= !(fabsf(u2f(o[e])) < INFINITY);
         }
-        if (mine && whole) {
+        if (whole) {
+          // 16-byte units through a transpose among four lanes: a store then covers 64 bytes of each of eight rows
+          uint4 x[4];
 #pragma unroll
-          for (int q = 0; q < 4; q++)
-            if (i * 32 + q * 8 < p.d) {
-              uint32_t x[4];
+          for (int q = 0; q < 4; q++) {
+            x[q].x = pack2<F16>(u2f(o[q * 8]) * inv, u2f(o[q * 8 + 1]) * inv);
+            x[q].y = pack2<F16>(u2f(o[q * 8 + 2]) * inv, u2f(o[q * 8 + 3]) * inv);
+            x[q].z = pack2<F16>(u2f(o[q * 8 + 4]) * inv, u2f(o[q * 8 + 5]) * inv);
+            x[q].w = pack2<F16>(u2f(o[q * 8 + 6]) * inv, u2f(o[q * 8 + 7]) * inv);
+          }
 #pragma unroll
-              for (int e = 0; e < 4; e++) x[e] = pack2<F16>(u2f(o[q * 8 + 2 * e]) * inv, u2f(o[q * 8 + 2 * e + 1]) * inv);
-              *reinterpret_cast<uint4 *>(out + i * 32 + q * 8) = make_uint4(x[0], x[1], x[2], x[3]);
-            }
+          for (int d = 1; d <= 2; d <<= 1) {               // lane l gives away its units whose bit d differs from l's
+            const bool up = lane & d;
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+              if (!(q & d)) {
+                uint4 &lo = x[q], &hi = x[q | d];
+                uint4 out4 = up ? lo : hi;
+                out4.x = __shfl_xor_sync(~0u, out4.x, d);
+                out4.y = __shfl_xor_sync(~0u, out4.y, d);
+                out4.z = __shfl_xor_sync(~0u, out4.z, d);
+                out4.w = __shfl_xor_sync(~0u, out4.w, d);
+                if (up) lo = out4;
+                else hi = out4;
+              }
+          }
+          const int col = i * 32 + (lane & 3) * 8;
+#pragma unroll
+          for (int q = 0; q < 4; q++)                      // x[q]: unit lane % 4 of the row of lane (lane & ~3) + q
+            if (to[q] >= 0 && col < p.d) *reinterpret_cast<uint4 *>(p.out + to[q] + col) = x[q];
         } else if (mine) {
 #pragma unroll
           for (int q = 0; q < 8; q++)
@@ -885,6 +949,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
       }
       __syncwarp();
       if (lane == 0) bar_arrive(seg_empty + 8 * (segs % SEGS));
+      sg = next;
     }
   }
   // ---- teardown, reached by every role whether or not a wait ran out
