@@ -47,27 +47,6 @@ constexpr int THREADS = 128;  // four warps
 template <int KV>
 constexpr bool is_fp8 = KV == FP8B200_E4M3 || KV == FP8B200_E5M2;
 
-template <bool F16, int KV, int DP, int RW>
-struct Cfg {
-  static constexpr bool FP8 = is_fp8<KV>;
-  static constexpr bool MF16 = F16 || FP8;              // operand type of the matrix instructions
-  static constexpr int ROWB = DP * (FP8 ? 1 : 2);       // bytes of a key's row in shared memory
-  static constexpr int CPR = ROWB / 16;                 // 16-byte units of it
-  static constexpr int TILE = BN * ROWB;                // K or V
-  // two blocks an SM (head size 256: one), the more bytes in flight the better
-  static constexpr int STAGES = FP8 ? (DP == 64 ? 8 : DP == 128 ? (RW == 4 ? 5 : 6) : 3)
-                                    : (DP == 64 ? 6 : DP == 128 ? (RW == 4 ? 2 : 3) : 2);
-  static constexpr int MR = 16 * RW;                    // rows a block
-  static constexpr int KW = 4 / RW;                     // warps that share a tile's keys
-  static constexpr int WN = BN / KW;                    // keys a warp
-  static constexpr int QROW = DP * 2 + 16;              // bytes of a query row (padded: no bank conflicts)
-  static constexpr int RING = STAGES * 2 * TILE;
-  static constexpr int OFFS = STAGES + 1;               // slot offsets are found one tile further ahead
-  static constexpr int SMEM = RING + MR * QROW + OFFS * BN * 8 + OFFS * 2 * 4 + MR * 4 + 64 * 2 * 4 + 64;
-  static constexpr float SHIFT = MF16 ? 15.0f : 0.0f;   // weights are scaled by 2^SHIFT
-  static_assert(64 * DP * 4 <= RING, "the warps' outputs fit the drained ring");
-};
-
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
@@ -125,6 +104,537 @@ __device__ __forceinline__ long long units_of(const AttnParams &p, int r, int &t
   return row_tiles * p.hk * tiles;
 }
 
+// A block's share [u, u_end) of the line of units, found by all its threads:
+// the request that u falls into and the units before that request. At least
+// MIN_UNITS a block: below that the join costs more than the share saves.
+constexpr int MIN_UNITS = 2;
+struct Share {
+  long long u, u_end, before, total, blocks;
+  int r;  // -1: nothing for this block
+};
+template <int MR>
+__device__ __forceinline__ Share find_share(const AttnParams &p, long long *s_scan) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  Share sh;
+  int tiles;
+  const long long first = tid < p.requests ? units_of<MR>(p, tid, tiles) : 0;
+  long long sum = first;
+  for (int r = tid + THREADS; r < p.requests; r += THREADS) sum += units_of<MR>(p, r, tiles);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+  if (lane == 0) s_scan[warp] = sum;
+  __syncthreads();
+  sh.total = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+  sh.blocks = min((long long)gridDim.x, (sh.total + MIN_UNITS - 1) / MIN_UNITS);
+  sh.r = -1;
+  sh.u = sh.u_end = sh.before = 0;
+  const long long c = blockIdx.x;
+  if (tid == 0) p.desc[c].rows = 0;
+  if (c >= sh.blocks) return sh;
+  sh.u = c * sh.total / sh.blocks;
+  sh.u_end = (c + 1) * sh.total / sh.blocks;
+  long long before = 0;
+  for (int r0 = 0; r0 < p.requests; r0 += THREADS) {
+    const int r = r0 + tid;
+    const long long mine = r0 == 0 ? first : r < p.requests ? units_of<MR>(p, r, tiles) : 0;
+    long long inc = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long a = __shfl_up_sync(~0u, inc, d);
+      if (lane >= d) inc += a;
+    }
+    __syncthreads();
+    if (lane == 31) s_scan[warp] = inc;
+    __syncthreads();
+    long long base = before;
+    for (int w = 0; w < warp; w++) base += s_scan[w];
+    before += s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+    if (base + inc > sh.u && base + inc - mine <= sh.u) {
+      s_scan[4] = r;
+      s_scan[5] = base + inc - mine;
+    }
+    if (before > sh.u) break;
+  }
+  __syncthreads();
+  sh.r = (int)s_scan[4];
+  sh.before = s_scan[5];
+  return sh;
+}
+
+// bf16 rows of s_q to f16 with the largest value in [1, 2); `flip` changes the
+// signs (a negative scale: the maximum of the products is then that of the
+// scores). Rows are shared by the block's warps.
+template <bool TO_F16, int DP>
+__device__ __forceinline__ void normalise_rows(uint8_t *s_q, int qrow, int rows, float *s_qscale, uint32_t flip) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int row = warp; row < rows; row += 4) {
+    uint32_t *w = reinterpret_cast<uint32_t *>(s_q + row * qrow);
+    if constexpr (TO_F16) {
+      float a = 0.0f;
+      for (int i = lane; i < DP / 2; i += 32) a = fmaxf(a, fmaxf(fabsf(u2f(w[i] << 16)), fabsf(u2f(w[i] & 0xFFFF0000u))));
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) a = fmaxf(a, __shfl_xor_sync(~0u, a, d));
+      uint32_t eb = f2u(a) >> 23;
+      eb = (eb == 255u || a == 0.0f) ? 127u : min(max(eb, 1u), 253u);
+      const float mul = u2f((254u - eb) << 23);
+      for (int i = lane; i < DP / 2; i += 32)
+        w[i] = pack2<true>(u2f(w[i] << 16) * mul, u2f(w[i] & 0xFFFF0000u) * mul) ^ flip;
+      if (lane == 0) s_qscale[row] = u2f(eb << 23);
+    } else if (flip) {
+      for (int i = lane; i < DP / 2; i += 32) w[i] ^= flip;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ few rows
+//
+// Up to 16 * MG query rows a request (decoding, a few drafted tokens). The
+// four warps of a block share nothing but the queries: each takes 16 of a
+// tile's 64 keys, brings them into a ring of its own and multiplies them with
+// all rows, so there is no block barrier between a segment's ends, a key's
+// codes are converted once whatever the number of rows, and the SM's warps
+// drift apart and cover one another's latencies. O is rescaled only when a
+// row's maximum has grown by more than 2^8 (see paged_attention_tc.cu).
+template <bool F16, int KV, int DP, int MG>
+struct Few {
+  static constexpr bool FP8 = is_fp8<KV>;
+  static constexpr bool MF16 = F16 || FP8;
+  static constexpr int ROWB = DP * (FP8 ? 1 : 2), CPR = ROWB / 16;
+  static constexpr int WK = 16;                           // keys a warp takes of a tile
+  static constexpr int HALF = WK * ROWB;                  // K or V of them
+  static constexpr int ST = DP == 256 && !FP8 ? 2 : DP == 64 ? 4 : 3;
+  static constexpr int RING = ST * 2 * HALF;              // a warp's
+  static constexpr int MR = 16 * MG;
+  static constexpr int QROW = DP * 2 + 16;
+  static constexpr int OFF_Q = 4 * RING;
+  static constexpr int OFF_SCALE = OFF_Q + MR * QROW;     // [MR] query scales, [4][MR] bases, [4][MR] sums
+  static constexpr int OFF_SCAN = OFF_SCALE + 9 * MR * 4;
+  static constexpr int SMEM = OFF_SCAN + 64;
+  static constexpr float SHIFT = MF16 ? 7.0f : 0.0f;
+  static constexpr bool QREG = MG == 1 && DP <= 128;      // query fragments stay in registers
+  static constexpr int PER_SM = DP == 256 ? (FP8 ? 2 : 1) : (DP == 128 && (!FP8 || MG > 1)) ? 2 : MG > 2 ? 2 : DP == 64 && MG == 1 && FP8 ? 4 : 3;
+  static_assert(4 * 16 * DP * 4 <= 4 * RING, "the warps' outputs of one row group fit the drained rings");
+  static_assert(PER_SM * (SMEM + 1024) <= 233472, "blocks an SM");
+};
+
+template <bool F16, int KV, int DP, int MG>
+__global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged_few_kernel(const AttnParams p) {
+  using C = Few<F16, KV, DP, MG>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t *s_q = smem + C::OFF_Q;
+  float *s_qscale = reinterpret_cast<float *>(smem + C::OFF_SCALE), *s_base = s_qscale + C::MR, *s_sum = s_base + 4 * C::MR;
+  long long *s_scan = reinterpret_cast<long long *>(smem + C::OFF_SCAN);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, tg = lane & 3;
+  uint8_t *ring = smem + warp * C::RING;
+  const uint32_t ring_a = saddr(ring);
+  const uint8_t *none = reinterpret_cast<const uint8_t *>(p.q);  // where nothing is read from
+  const int used = (p.d * (C::FP8 ? 1 : 2)) / 16;          // 16-byte units of a key's row that hold values
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Share sh = find_share<C::MR>(p, s_scan);
+  if (p.zero_rest) zero_rest(p, blockIdx.x, gridDim.x);
+  if (sh.r < 0) return;
+  const long long c = blockIdx.x;
+  long long u = sh.u, before = sh.before;
+  int r = sh.r;
+  while (u < sh.u_end) {
+    // ---- the segment that unit u belongs to
+    const Request rq = load_request(p, r);
+    int tiles_n;
+    const long long n_units = units_of<C::MR>(p, r, tiles_n);
+    if (u >= before + n_units) {
+      before += n_units;
+      r++;
+      continue;
+    }
+    const int local = (int)(u - before) % tiles_n;
+    const long long seg = (u - before) / tiles_n;
+    const int t_begin = local, t_end = (int)min((long long)tiles_n, t_begin + (sh.u_end - u));
+    const int h = (int)(seg % p.hk), qt = (int)(seg / p.hk);
+    const long long seg_start = u - t_begin;
+    u += t_end - t_begin;
+    const Tiles<BN> tl = visible_tiles<BN>(p, rq.first, rq.first + rq.n - 1);
+    const int row0 = qt * C::MR;
+    const int rows = (int)min((long long)C::MR, (long long)rq.n * p.group - row0);
+    const int pos_lo = rq.first + row0 / p.group, pos_hi = rq.first + (row0 + rows - 1) / p.group;
+    const float scale = p.scale_log2 * (C::FP8 && p.ks ? __ldg(p.ks + p.ks_step * h) : 1.0f);
+
+    // this warp's keys of list entry i: lane < 16 finds the slot of key `lane`
+    auto find = [&](int i) -> long long {
+      if (i >= t_end || lane >= C::WK) return -1;
+      const int j = tl.at(i) * BN + warp * C::WK + lane;
+      return j <= pos_hi ? slot_offset(p, r, j) : -2;      // -2: no key, -1: a key without a page
+    };
+    unsigned long long hidden = 0;                          // keys without a page, 16 bits a tile, newest last
+    auto issue = [&](int stage, long long off) {            // of the tile whose offsets the lanes hold
+      hidden = (hidden << 16) | (__ballot_sync(~0u, off == -1) & 0xFFFFu);
+      constexpr int STEP = 32 / C::CPR > 0 ? 32 / C::CPR : 1, PASS = C::CPR > 32 ? C::CPR / 32 : 1;
+#pragma unroll
+      for (int k = 0; k < C::WK / STEP; k++) {
+        const int row = k * STEP + (C::CPR < 32 ? lane / C::CPR : 0);
+        const long long o = __shfl_sync(~0u, off, row);
+#pragma unroll
+        for (int q = 0; q < PASS; q++) {
+          const int cu = C::CPR < 32 ? lane % C::CPR : lane + 32 * q;
+          if (cu < used) {
+            const bool valid = o >= 0;
+            const long long byte = valid ? (o + (long long)h * p.s_head) * (C::FP8 ? 1 : 2) + cu * 16 : 0;
+            const uint32_t at = ring_a + stage * 2 * C::HALF;
+            cp16(at + (C::FP8 ? unit_at<C::ROWB, true>(row, cu) : unit_at<C::ROWB, false>(row, cu)), valid ? p.k + byte : none, valid);
+            cp16(at + C::HALF + unit_at<C::ROWB, false>(row, cu), valid ? p.v + byte : none, valid);
+          }
+        }
+      }
+    };
+
+    __syncthreads();  // the previous segment's readers of shared memory are done
+    if (used < C::CPR) {  // units without values are zero while the segment lasts (its end uses the ring for something else)
+      for (int i = lane; i < C::RING / 16; i += 32) {
+        const int half = i / (C::HALF / 16), row = (i % (C::HALF / 16)) / C::CPR, cu = i % C::CPR;
+        if (cu >= used) {
+          const uint32_t at = (C::FP8 && half % 2 == 0) ? unit_at<C::ROWB, true>(row, cu) : unit_at<C::ROWB, false>(row, cu);
+          *reinterpret_cast<uint4 *>(ring + half * C::HALF + at) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      __syncwarp();
+    }
+    long long off[C::ST];
+#pragma unroll
+    for (int k = 0; k < C::ST; k++) off[k] = find(t_begin + k);  // all table reads in flight at once
+    for (int i = tid; i < C::MR * (DP / 8); i += THREADS) {
+      const int row = i / (DP / 8), cu = i % (DP / 8);
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (row < rows && cu * 8 < p.d) {
+        const int qr = row0 + row, tok = rq.start + qr / p.group, head = h * p.group + qr % p.group;
+        v = __ldg(reinterpret_cast<const uint4 *>(p.q + (int64_t)tok * p.q_tok + (int64_t)head * p.q_head + cu * 8));
+      }
+      *reinterpret_cast<uint4 *>(s_q + row * C::QROW + cu * 16) = v;
+    }
+#pragma unroll
+    for (int k = 0; k < C::ST - 1; k++) {
+      issue(k, off[k]);
+      cp_commit();
+    }
+    long long ahead = off[C::ST - 1];                       // offsets of the next tile to load
+    __syncthreads();
+    if ((C::FP8 && !F16) || scale < 0.0f) {
+      normalise_rows<C::FP8 && !F16, DP>(s_q, C::QROW, C::MR, s_qscale, scale < 0.0f ? 0x80008000u : 0u);
+      __syncthreads();
+    }
+    auto load_q = [&](int mg, int ks, uint32_t (&a)[4]) {
+      const uint8_t *q0 = s_q + (mg * 16 + g) * C::QROW, *q1 = q0 + 8 * C::QROW;
+      if constexpr (C::FP8) {                               // k order of a 64-value block: lane tg holds values 16 tg .. 16 tg + 15
+        const int at = ((ks >> 2) * 64 + tg * 16 + (ks & 3) * 4) * 2;
+        const uint2 x = *reinterpret_cast<const uint2 *>(q0 + at), y = *reinterpret_cast<const uint2 *>(q1 + at);
+        a[0] = x.x, a[1] = y.x, a[2] = x.y, a[3] = y.y;
+      } else {
+        const int at = (ks * 16 + tg * 2) * 2;
+        a[0] = *reinterpret_cast<const uint32_t *>(q0 + at);
+        a[1] = *reinterpret_cast<const uint32_t *>(q1 + at);
+        a[2] = *reinterpret_cast<const uint32_t *>(q0 + at + 16);
+        a[3] = *reinterpret_cast<const uint32_t *>(q1 + at + 16);
+      }
+    };
+    uint32_t qf[C::QREG ? DP / 16 : 1][4];
+    if constexpr (C::QREG) {
+#pragma unroll
+      for (int ks = 0; ks < DP / 16; ks++) load_q(0, ks, qf[ks]);
+    }
+    float sc[MG][2];                                        // of rows g and g + 8 of each group; above 0, see paged_attention_tc.cu
+    int pos[MG][2];
+#pragma unroll
+    for (int mg = 0; mg < MG; mg++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const int row = mg * 16 + g + 8 * e;
+        sc[mg][e] = fabsf(scale) * ((C::FP8 && !F16) ? s_qscale[row] : 1.0f);
+        if (sc[mg][e] == 0.0f) sc[mg][e] = 1e-30f;
+        pos[mg][e] = rq.first + min(row0 + row, row0 + rows - 1) / p.group;
+      }
+    float o[MG][DP / 8][4], base[MG][2], sum[MG][2];
+#pragma unroll
+    for (int mg = 0; mg < MG; mg++) {
+#pragma unroll
+      for (int i = 0; i < DP / 8; i++) o[mg][i][0] = o[mg][i][1] = o[mg][i][2] = o[mg][i][3] = 0.0f;
+      base[mg][0] = base[mg][1] = -INFINITY;
+      sum[mg][0] = sum[mg][1] = 0.0f;
+    }
+
+    int stage = 0;
+#pragma unroll 1
+    for (int i = t_begin; i < t_end; i++) {
+      cp_wait<C::ST - 2>();
+      __syncwarp();
+      {
+        int st = stage + C::ST - 1;
+        if (st >= C::ST) st -= C::ST;
+        issue(st, ahead);                                   // behind the last tile: copies nothing that is read
+        cp_commit();
+        ahead = find(i + C::ST);
+      }
+      const uint32_t kt = ring_a + stage * 2 * C::HALF, vt = kt + C::HALF;
+      if (++stage == C::ST) stage = 0;
+      float s[MG][2][4];
+#pragma unroll
+      for (int mg = 0; mg < MG; mg++)
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++) s[mg][nt][0] = s[mg][nt][1] = s[mg][nt][2] = s[mg][nt][3] = 0.0f;
+      if constexpr (C::FP8) {
+#pragma unroll
+        for (int b = 0; b < DP / 64; b++) {
+          uint32_t w[2][4];
+#pragma unroll
+          for (int nt = 0; nt < 2; nt++)
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(w[nt][0]), "=r"(w[nt][1]), "=r"(w[nt][2]), "=r"(w[nt][3])
+                         : "r"(kt + unit_at<C::ROWB, true>(nt * 8 + g, b * 4 + tg)));
+#pragma unroll
+          for (int ks = 0; ks < 4; ks++) {
+            uint32_t a[MG][4];
+#pragma unroll
+            for (int mg = 0; mg < MG; mg++) {
+              if constexpr (C::QREG) a[mg][0] = qf[b * 4 + ks][0], a[mg][1] = qf[b * 4 + ks][1], a[mg][2] = qf[b * 4 + ks][2], a[mg][3] = qf[b * 4 + ks][3];
+              else load_q(mg, b * 4 + ks, a[mg]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < 2; nt++) {
+              const uint32_t b0 = fp8x2_to_f16x2<KV>(w[nt][ks] & 0xFFFFu), b1 = fp8x2_to_f16x2<KV>(w[nt][ks] >> 16);
+#pragma unroll
+              for (int mg = 0; mg < MG; mg++) mma<true>(s[mg][nt], a[mg], b0, b1);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ks++) {
+          uint32_t b[4];
+          ldsm4(kt + unit_at<C::ROWB, false>(((lane >> 4) << 3) + (lane & 7), ks * 2 + ((lane >> 3) & 1)), b);
+#pragma unroll
+          for (int mg = 0; mg < MG; mg++) {
+            uint32_t a[4];
+            if constexpr (C::QREG) a[0] = qf[ks][0], a[1] = qf[ks][1], a[2] = qf[ks][2], a[3] = qf[ks][3];
+            else load_q(mg, ks, a);
+            mma<C::MF16>(s[mg][0], a, b[0], b[1]);
+            mma<C::MF16>(s[mg][1], a, b[2], b[3]);
+          }
+        }
+      }
+      const int k0 = tl.at(i) * BN + warp * C::WK;
+      const uint32_t hide = (uint32_t)(hidden >> (16 * (C::ST - 1))) & 0xFFFFu;
+      if (k0 + C::WK - 1 > pos_lo || hide || (p.window > 0 && pos_hi - k0 >= p.window && k0 + C::WK - 1 >= p.sinks)) {
+#pragma unroll
+        for (int mg = 0; mg < MG; mg++)
+#pragma unroll
+          for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+              const int kk = nt * 8 + tg * 2 + x;
+              const bool gone = (hide >> kk) & 1u;
+              if (gone || !visible(p, k0 + kk, pos[mg][0])) s[mg][nt][x] = -INFINITY;
+              if (gone || !visible(p, k0 + kk, pos[mg][1])) s[mg][nt][2 + x] = -INFINITY;
+            }
+      }
+      float top[MG][2];
+      bool grow = false;
+#pragma unroll
+      for (int mg = 0; mg < MG; mg++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          float m = fmaxf(fmaxf(s[mg][0][2 * e], s[mg][0][2 * e + 1]), fmaxf(s[mg][1][2 * e], s[mg][1][2 * e + 1]));
+          m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
+          m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
+          top[mg][e] = m * sc[mg][e];
+          grow |= top[mg][e] > base[mg][e] + 8.0f;          // also a row's first key
+        }
+      if (__any_sync(~0u, grow)) {
+#pragma unroll
+        for (int mg = 0; mg < MG; mg++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float nb = fmaxf(base[mg][e], top[mg][e]);
+            const float f = base[mg][e] == -INFINITY ? 0.0f : ex2(base[mg][e] - nb);
+            base[mg][e] = nb;
+            sum[mg][e] *= f;
+#pragma unroll
+            for (int j = 0; j < DP / 8; j++) o[mg][j][2 * e] *= f, o[mg][j][2 * e + 1] *= f;
+          }
+      }
+      uint32_t a[MG][4];
+#pragma unroll
+      for (int mg = 0; mg < MG; mg++) {
+        const float o0 = C::SHIFT - (base[mg][0] == -INFINITY ? 0.0f : base[mg][0]);
+        const float o1 = C::SHIFT - (base[mg][1] == -INFINITY ? 0.0f : base[mg][1]);
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++) {
+          const float e0 = ex2(fmaf(s[mg][nt][0], sc[mg][0], o0)), e1 = ex2(fmaf(s[mg][nt][1], sc[mg][0], o0));
+          const float e2 = ex2(fmaf(s[mg][nt][2], sc[mg][1], o1)), e3 = ex2(fmaf(s[mg][nt][3], sc[mg][1], o1));
+          sum[mg][0] += e0 + e1;
+          sum[mg][1] += e2 + e3;
+          a[mg][2 * nt] = pack2<C::MF16>(e0, e1);
+          a[mg][2 * nt + 1] = pack2<C::MF16>(e2, e3);
+        }
+      }
+      const int key = (((lane >> 3) & 1) << 3) + (lane & 7);
+      if constexpr (C::FP8) {
+#pragma unroll
+        for (int cp = 0; cp < DP / 32; cp++) {
+          uint32_t w[4];
+          ldsm4t(vt + unit_at<C::ROWB, false>(key, cp * 2 + (lane >> 4)), w);
+#pragma unroll
+          for (int e = 0; e < 2; e++) {                     // unit cp * 2 + e: its even dims, then its odd dims
+            uint32_t x, y;
+            asm("prmt.b32 %0, %1, 0, 0x3120;" : "=r"(x) : "r"(w[2 * e]));
+            asm("prmt.b32 %0, %1, 0, 0x3120;" : "=r"(y) : "r"(w[2 * e + 1]));
+            const uint32_t x0 = fp8x2_to_f16x2<KV>(x & 0xFFFFu), y0 = fp8x2_to_f16x2<KV>(y & 0xFFFFu);
+            const uint32_t x1 = fp8x2_to_f16x2<KV>(x >> 16), y1 = fp8x2_to_f16x2<KV>(y >> 16);
+#pragma unroll
+            for (int mg = 0; mg < MG; mg++) {
+              mma<true>(o[mg][cp * 4 + e * 2], a[mg], x0, y0);
+              mma<true>(o[mg][cp * 4 + e * 2 + 1], a[mg], x1, y1);
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int dp = 0; dp < DP / 16; dp++) {
+          uint32_t b[4];
+          ldsm4t(vt + unit_at<C::ROWB, false>(key, dp * 2 + (lane >> 4)), b);
+#pragma unroll
+          for (int mg = 0; mg < MG; mg++) {
+            mma<C::MF16>(o[mg][2 * dp], a[mg], b[0], b[1]);
+            mma<C::MF16>(o[mg][2 * dp + 1], a[mg], b[2], b[3]);
+          }
+        }
+      }
+    }
+    cp_wait<0>();
+
+    // ---- the segment's end: the warps' results, a row group at a time, through the drained rings
+    bool odd = false;                                       // infinities or NaN: see careful_row
+#pragma unroll
+    for (int mg = 0; mg < MG; mg++) {
+#pragma unroll
+      for (int j = 0; j < DP / 8; j++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) odd |= !(fabsf(o[mg][j][x]) < INFINITY);
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        sum[mg][e] += __shfl_xor_sync(~0u, sum[mg][e], 1);
+        sum[mg][e] += __shfl_xor_sync(~0u, sum[mg][e], 2);
+        if (tg == 0) {
+          s_base[warp * C::MR + mg * 16 + g + 8 * e] = base[mg][e] - C::SHIFT;
+          s_sum[warp * C::MR + mg * 16 + g + 8 * e] = sum[mg][e];
+        }
+      }
+    }
+    const bool careful = __syncthreads_or(odd);
+    const bool begins = t_begin == 0, ends = t_end == tiles_n;
+    const float vs = C::FP8 && p.vs ? __ldg(p.vs + p.vs_step * h) : 1.0f;
+    float *part = p.part + (c * 2 + (begins ? 1 : 0)) * (int64_t)(C::MR * (DP + 2));
+    if (tid == 0 && begins && !ends)
+      p.desc[c] = PartDesc{rows, row0, h, (int)(((seg_start + tiles_n) * sh.blocks - 1) / sh.total), rq.start};
+    float *s_o = reinterpret_cast<float *>(smem);           // [4 warps][16 rows][DP]
+#pragma unroll
+    for (int mg = 0; mg < MG; mg++) {
+      if (mg * 16 < rows) {
+        if (mg) __syncthreads();
+        if (!careful) {
+          float *x0 = s_o + (warp * 16 + g) * DP, *x1 = x0 + 8 * DP;
+          if constexpr (C::FP8) {
+#pragma unroll
+            for (int k = 0; k < DP / 16; k++) {
+              const float(&e)[4] = o[mg][2 * k], (&f)[4] = o[mg][2 * k + 1];
+              *reinterpret_cast<float4 *>(x0 + k * 16 + tg * 4) = make_float4(e[0], f[0], e[1], f[1]);
+              *reinterpret_cast<float4 *>(x1 + k * 16 + tg * 4) = make_float4(e[2], f[2], e[3], f[3]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < DP / 8; j++) {
+              *reinterpret_cast<float2 *>(x0 + j * 8 + tg * 2) = make_float2(o[mg][j][0], o[mg][j][1]);
+              *reinterpret_cast<float2 *>(x1 + j * 8 + tg * 2) = make_float2(o[mg][j][2], o[mg][j][3]);
+            }
+          }
+        } else {
+          for (int row = warp; row < 16; row += 4) {
+            const bool there = mg * 16 + row < rows;
+            float m = -INFINITY, l = 0.0f, ov[DP / 32];
+#pragma unroll
+            for (int k = 0; k < DP / 32; k++) ov[k] = 0.0f;
+            if (there) {
+              const int qr = row0 + mg * 16 + row, tok = qr / p.group;
+              careful_row<F16, KV, DP, BN>(p, r, rq.start + tok, h * p.group + qr % p.group, rq.first + tok, tl, t_begin, t_end, m, l, ov);
+            }
+            for (int w = 0; w < 4; w++) {
+#pragma unroll
+              for (int k = 0; k < DP / 32; k++) s_o[(w * 16 + row) * DP + lane + 32 * k] = w == 0 ? ov[k] : 0.0f;
+              if (lane == 0) {
+                s_base[w * C::MR + mg * 16 + row] = w == 0 ? m : -INFINITY;
+                s_sum[w * C::MR + mg * 16 + row] = w == 0 ? l : 0.0f;
+              }
+            }
+          }
+        }
+        __syncthreads();
+        const int group_rows = min(16, rows - mg * 16);
+        for (int i = tid; i < group_rows * (DP / 4); i += THREADS) {
+          const int row = i / (DP / 4), d4 = (i % (DP / 4)) * 4, at = mg * 16 + row;
+          float b = fmaxf(fmaxf(s_base[at], s_base[C::MR + at]), fmaxf(s_base[2 * C::MR + at], s_base[3 * C::MR + at]));
+          const float ref = b == -INFINITY ? 0.0f : b;
+          float l = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int w = 0; w < 4; w++) {
+            const float f = ex2(s_base[w * C::MR + at] - ref);
+            const float4 v = *reinterpret_cast<const float4 *>(s_o + (w * 16 + row) * DP + d4);
+            l += f * s_sum[w * C::MR + at];
+            x[0] += f * v.x, x[1] += f * v.y, x[2] += f * v.z, x[3] += f * v.w;
+          }
+          if (begins && ends) {
+            if (d4 < p.d) {
+              const float inv = l == 0.0f ? 0.0f : vs / l;
+              const int qr = row0 + at, tok = rq.start + qr / p.group, head = h * p.group + qr % p.group;
+              uint16_t *out = p.out + (int64_t)tok * p.o_tok + (int64_t)head * p.o_head + d4;
+              *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<F16>(x[0] * inv, x[1] * inv), pack2<F16>(x[2] * inv, x[3] * inv));
+            }
+          } else {
+            *reinterpret_cast<float4 *>(part + at * DP + d4) = make_float4(x[0], x[1], x[2], x[3]);
+            if (d4 == 0) {
+              part[C::MR * DP + at] = b;
+              part[C::MR * DP + C::MR + at] = l;
+            }
+          }
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ more rows
+//
+// Where the tensor-memory kernel does not serve (head sizes above 128, caches
+// that no tensor map describes, a few dozen rows): the block's four warps take
+// 16 rows each and share the tile's keys.
+template <bool F16, int KV, int DP, int RW>
+struct Cfg {
+  static constexpr bool FP8 = is_fp8<KV>;
+  static constexpr bool MF16 = F16 || FP8;              // operand type of the matrix instructions
+  static constexpr int ROWB = DP * (FP8 ? 1 : 2);       // bytes of a key's row in shared memory
+  static constexpr int CPR = ROWB / 16;                 // 16-byte units of it
+  static constexpr int TILE = BN * ROWB;                // K or V
+  // two blocks an SM (head size 256: one), the more bytes in flight the better
+  static constexpr int STAGES = FP8 ? (DP == 64 ? 8 : DP == 128 ? (RW == 4 ? 5 : 6) : 3)
+                                    : (DP == 64 ? 6 : DP == 128 ? (RW == 4 ? 2 : 3) : 2);
+  static constexpr int MR = 16 * RW;                    // rows a block
+  static constexpr int KW = 4 / RW;                     // warps that share a tile's keys
+  static constexpr int WN = BN / KW;                    // keys a warp
+  static constexpr int QROW = DP * 2 + 16;              // bytes of a query row (padded: no bank conflicts)
+  static constexpr int RING = STAGES * 2 * TILE;
+  static constexpr int OFFS = STAGES + 1;               // slot offsets are found one tile further ahead
+  static constexpr int SMEM = RING + MR * QROW + OFFS * BN * 8 + OFFS * 2 * 4 + MR * 4 + 64 * 2 * 4 + 64;
+  static constexpr float SHIFT = MF16 ? 15.0f : 0.0f;   // weights are scaled by 2^SHIFT
+  static_assert(64 * DP * 4 <= RING, "the warps' outputs fit the drained ring");
+};
+
 template <bool F16, int KV, int DP, int RW>
 __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_kernel(const AttnParams p) {
   using C = Cfg<F16, KV, DP, RW>;
@@ -143,52 +653,17 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
   const uint32_t ring_a = saddr(ring), q_a = saddr(s_q);
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const uint8_t *none = reinterpret_cast<const uint8_t *>(p.q);  // where nothing is read from
   const int used = (p.d * (C::FP8 ? 1 : 2)) / 16;  // 16-byte units of a key's row that hold values
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ---- this block's share of the line of units
-  long long total = 0;
-  int tiles_r = 0;
-  for (int r = tid; r < p.requests; r += THREADS) total += units_of<C::MR>(p, r, tiles_r);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
-  if (lane == 0) s_scan[warp] = total;
-  __syncthreads();
-  total = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
-  __syncthreads();
+  const Share sh = find_share<C::MR>(p, s_scan);
   if (p.zero_rest) zero_rest(p, blockIdx.x, gridDim.x);
-  const long long blocks = min((long long)gridDim.x, total);  // no block is left without a unit between two others
-  const long long c = blockIdx.x;
-  if (tid == 0) p.desc[c] = make_int4(-1, 0, 0, 0);
-  if (c >= blocks) return;
-  long long u = c * total / blocks;
-  const long long u_end = (c + 1) * total / blocks;
-  long long before = 0;                                       // units before the requests looked at
-  for (int r0 = 0; r0 < p.requests; r0 += THREADS) {
-    const int r = r0 + tid;
-    const long long mine = r < p.requests ? units_of<C::MR>(p, r, tiles_r) : 0;
-    long long inc = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long a = __shfl_up_sync(~0u, inc, d);
-      if (lane >= d) inc += a;
-    }
-    if (lane == 31) s_scan[warp] = inc;
-    __syncthreads();
-    long long base = before;
-    for (int w = 0; w < warp; w++) base += s_scan[w];
-    const long long all = before + s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
-    if (base + inc > u && base + inc - mine <= u) {
-      s_scan[4] = r;
-      s_scan[5] = base + inc - mine;
-    }
-    __syncthreads();
-    before = all;
-    if (before > u) break;
-  }
-  int r = (int)s_scan[4];
-  before = s_scan[5];
-
+  if (sh.r < 0) return;
+  const long long c = blockIdx.x, u_end = sh.u_end, blocks = sh.blocks, total = sh.total;
+  long long u = sh.u, before = sh.before;
+  int r = sh.r;
   while (u < u_end) {
     // ---- the segment that unit u belongs to
     const Request rq = load_request(p, r);
@@ -251,8 +726,8 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
           const bool valid = off >= 0;
           const uint32_t kd = ring_a + stage * 2 * C::TILE + (C::FP8 ? unit_at<C::ROWB, true>(row, cunit) : unit_at<C::ROWB, false>(row, cunit));
           const uint32_t vd = ring_a + (stage * 2 + 1) * C::TILE + unit_at<C::ROWB, false>(row, cunit);
-          cp16(kd, valid ? p.k + byte : p.k, valid);
-          cp16(vd, valid ? p.v + byte : p.v, valid);
+          cp16(kd, valid ? p.k + byte : none, valid);
+          cp16(vd, valid ? p.v + byte : none, valid);
         }
       }
     };
@@ -562,7 +1037,7 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
     const float vs = C::FP8 && p.vs ? __ldg(p.vs + p.vs_step * h) : 1.0f;
     float *part = p.part + (c * 2 + (begins ? 1 : 0)) * (int64_t)(C::MR * (DP + 2));
     if (tid == 0 && begins && !ends)
-      p.desc[c] = make_int4(r, qt, h, (int)(((seg_start + tiles_n) * blocks - 1) / total));
+      p.desc[c] = PartDesc{rows, row0, h, (int)(((seg_start + tiles_n) * blocks - 1) / total), rq.start};
     for (int i = tid; i < rows * (DP / 4); i += THREADS) {
       const int row = i / (DP / 4), d4 = (i % (DP / 4)) * 4;
       const int at = (row >> 4) * C::KW * 16 + (row & 15);
@@ -596,72 +1071,31 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
   }
 }
 
-// Joins the parts of the segments that were cut: block c the one that began
-// in block c of the attention kernel (its second part), with the first parts
-// of the blocks after it, in their order.
-template <bool F16, int DP, int MR>
-__global__ void __launch_bounds__(THREADS) paged_merge_kernel(const AttnParams p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const long long c = blockIdx.x;
-  const int4 d = p.desc[c];
-  if (d.x < 0) return;
-  const Request rq = load_request(p, d.x);
-  const int row0 = d.y * MR, h = d.z;
-  const int rows = (int)min((long long)MR, (long long)rq.n * p.group - row0);
-  const float vs = p.vs ? __ldg(p.vs + p.vs_step * h) : 1.0f;
-  constexpr int64_t SLOT = MR * (DP + 2);
-  for (int i = threadIdx.x; i < rows * (DP / 4); i += THREADS) {
-    const int row = i / (DP / 4), d4 = (i % (DP / 4)) * 4;
-    if (d4 >= p.d) continue;
-    float base = -INFINITY, l = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (long long b = c; b <= d.w; b++) {
-      const float *part = p.part + (b * 2 + (b == c ? 1 : 0)) * SLOT;
-      const float bb = part[MR * DP + row], bl = part[MR * DP + MR + row];
-      const float4 v = *reinterpret_cast<const float4 *>(part + row * DP + d4);
-      const float nb = fmaxf(base, bb), ref = nb == -INFINITY ? 0.0f : nb;
-      const float f = ex2(base - ref), e = ex2(bb - ref);
-      base = nb;
-      l = l * f + bl * e;
-      x[0] = x[0] * f + v.x * e, x[1] = x[1] * f + v.y * e, x[2] = x[2] * f + v.z * e, x[3] = x[3] * f + v.w * e;
-    }
-    const float inv = l == 0.0f ? 0.0f : vs / l;
-    const int qr = row0 + row, tok = rq.start + qr / p.group, head = h * p.group + qr % p.group;
-    uint16_t *out = p.out + (int64_t)tok * p.o_tok + (int64_t)head * p.o_head + d4;
-    *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<F16>(x[0] * inv, x[1] * inv), pack2<F16>(x[2] * inv, x[3] * inv));
-  }
-}
-
-template <typename P>
-cudaError_t launch_pdl(void (*kernel)(P), int grid, int threads, int smem, cudaStream_t st, const P &p) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 struct Variant {
   void (*main)(AttnParams);
   void (*merge)(AttnParams);
-  int smem, per_sm;
+  int smem, per_sm, rows;
 };
-template <bool F16, int KV, int DP, int RW>
-Variant variant() {
-  return {paged_attention_kernel<F16, KV, DP, RW>, paged_merge_kernel<F16, DP, 16 * RW>, Cfg<F16, KV, DP, RW>::SMEM,
-          DP == 256 ? 1 : 2};
+template <bool F16, int KV, int DP, int MG>
+Variant few() {
+  using C = Few<F16, KV, DP, MG>;
+  return {paged_few_kernel<F16, KV, DP, MG>, paged_merge_kernel<F16, DP, C::MR>, C::SMEM, C::PER_SM, C::MR};
 }
+template <bool F16, int KV, int DP>
+Variant many() {
+  return {paged_attention_kernel<F16, KV, DP, 4>, paged_merge_kernel<F16, DP, 64>, Cfg<F16, KV, DP, 4>::SMEM, DP == 256 ? 1 : 2, 64};
+}
+// `rows`: query rows of the longest request (a request with more is served in several row tiles).
 template <bool F16, int KV>
-Variant pick(int dp, int rw) {
-  if (dp == 64) return rw == 1 ? variant<F16, KV, 64, 1>() : rw == 2 ? variant<F16, KV, 64, 2>() : variant<F16, KV, 64, 4>();
-  if (dp == 128) return rw == 1 ? variant<F16, KV, 128, 1>() : rw == 2 ? variant<F16, KV, 128, 2>() : variant<F16, KV, 128, 4>();
-  return rw == 1 ? variant<F16, KV, 256, 1>() : rw == 2 ? variant<F16, KV, 256, 2>() : variant<F16, KV, 256, 4>();
+Variant pick(int dp, int64_t rows) {
+  if (dp == 64) return rows <= 16 ? few<F16, KV, 64, 1>() : rows <= 32 ? few<F16, KV, 64, 2>() : rows <= 64 ? few<F16, KV, 64, 4>() : many<F16, KV, 64>();
+  if (dp == 128) return rows <= 16 ? few<F16, KV, 128, 1>() : rows <= 32 ? few<F16, KV, 128, 2>() : many<F16, KV, 128>();
+  return rows <= 16 ? few<F16, KV, 256, 1>() : many<F16, KV, 256>();
+}
+Variant variant_for(bool f16, int cache_dtype, int dp, int64_t rows) {
+  if (cache_dtype == FP8B200_E4M3) return f16 ? pick<true, FP8B200_E4M3>(dp, rows) : pick<false, FP8B200_E4M3>(dp, rows);
+  if (cache_dtype == FP8B200_E5M2) return f16 ? pick<true, FP8B200_E5M2>(dp, rows) : pick<false, FP8B200_E5M2>(dp, rows);
+  return f16 ? pick<true, FP8B200_F16>(dp, rows) : pick<false, FP8B200_BF16>(dp, rows);
 }
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
@@ -674,7 +1108,8 @@ int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 // tensor-memory kernel when the longest has more than TC_FROM and the head
 // size is at most 128.
 static constexpr int64_t TC_FROM = 64, TC_OVER = 16;
-static int64_t paged_generic_workspace(int dp, int sms) { return 2 * (int64_t)sms * (2 * 64 * (int64_t)(dp + 2) * 4 + 16); }
+// Two parts a block (64 rows by two blocks an SM, 16 by four, ...: at most 128 rows an SM) and a descriptor.
+static int64_t paged_generic_workspace(int dp, int sms) { return (int64_t)sms * (2 * 128 * (int64_t)(dp + 2) * 4 + 4 * (int64_t)sizeof(fp8b200::paged::PartDesc)); }
 
 extern "C" int64_t fp8b200_paged_attention_workspace(int head_dim, int64_t max_rows) {
   using namespace fp8b200;
@@ -733,7 +1168,7 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
                      (long long)need);
   int dev;
   if (int rc = check_device(&dev)) return rc;
-  const int blocks_max = 2 * current_sm_count();
+  const int blocks_max = 4 * current_sm_count();
   AttnParams p{};
   p.q = (const uint16_t *)q;
   p.q_tok = q_stride_token, p.q_head = q_stride_head;
@@ -757,8 +1192,8 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
   p.zero_rest = zero_rest;
   p.rows_over = 0;
   p.rows_upto = INT32_MAX;
-  p.desc = (int4 *)workspace;
-  p.part = (float *)((uint8_t *)workspace + (int64_t)blocks_max * 16);
+  p.desc = (PartDesc *)workspace;
+  p.part = (float *)((uint8_t *)workspace + (int64_t)blocks_max * sizeof(PartDesc));
   const int dp = padded_dim(head_dim);
   const bool f16 = dtype == FP8B200_F16;
   if (dp <= 128 && most > TC_FROM && requests > 0 && tc_takes(p)) {
@@ -775,16 +1210,11 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
     if (alike) return FP8B200_OK;
     p.zero_rest = 0;
   }
-  const int rw = p.rows_upto <= 16 || most <= 16 ? 1 : most <= 32 ? 2 : 4;
-  Variant v;
-  if (cache_dtype == FP8B200_E4M3) v = f16 ? pick<true, FP8B200_E4M3>(dp, rw) : pick<false, FP8B200_E4M3>(dp, rw);
-  else if (cache_dtype == FP8B200_E5M2) v = f16 ? pick<true, FP8B200_E5M2>(dp, rw) : pick<false, FP8B200_E5M2>(dp, rw);
-  else v = f16 ? pick<true, FP8B200_F16>(dp, rw) : pick<false, FP8B200_BF16>(dp, rw);
-  cudaError_t e = cudaFuncSetAttribute(v.main, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem);
-  if (e != cudaSuccess) return check_launch("paged_attention");
+  const Variant v = variant_for(f16, cache_dtype, dp, std::min<int64_t>(most, p.rows_upto));
+  if (int rc = launch_attributes((const void *)v.main, v.smem)) return rc;
   const int grid = current_sm_count() * v.per_sm;
-  launch_pdl(v.main, grid, THREADS, v.smem, (cudaStream_t)stream, p);
-  launch_pdl(v.merge, grid, THREADS, 0, (cudaStream_t)stream, p);
+  launch_dependent(v.main, dim3((unsigned)grid), THREADS, v.smem, (cudaStream_t)stream, p);
+  launch_dependent(v.merge, dim3((unsigned)grid, 4), MERGE_THREADS, 0, (cudaStream_t)stream, p);
   count_launch(2);
   return check_launch("paged_attention");
 }

@@ -9,6 +9,14 @@
 namespace fp8b200 {
 namespace paged {
 
+// A segment that was cut, for the merge: written by the block that begins it.
+struct alignas(16) PartDesc {
+  int rows;                   // of the row tile; 0: this block began no such segment
+  int row0, h, last;          // the tile's first row in its request, the key/value head, the block that ends the segment
+  int start;                  // the request's first row of q
+};
+static_assert(sizeof(PartDesc) == 32, "two 16-byte words");
+
 // One call. Element strides throughout; the two caches share their strides.
 struct AttnParams {
   const uint16_t *q;
@@ -34,7 +42,7 @@ struct AttnParams {
   int rows_over, rows_upto;   // requests whose query rows (tokens x group) lie in (rows_over, rows_upto] are taken
   // split segments: partial results and which block continues what
   float *part;
-  int4 *desc;
+  PartDesc *desc;
 };
 
 // The new tokens of request r: rows [start, start + n) of q, the last at
@@ -200,6 +208,105 @@ __device__ __noinline__ void careful_row(const AttnParams &p, int r, int tok, in
   m_out = m;
   l_out = l;
 }
+
+// Joins the parts of the segments that were cut: block c the one that began
+// in block c of the attention kernel (its second part), with the first parts
+// of the blocks after it, in their order. A warp a row: its lanes fetch the
+// parts' bases and sums together, then the rows' values, whose loads do not
+// wait for one another. MR: rows a part has room for.
+constexpr int MERGE_THREADS = 128;
+template <bool F16, int DP, int MR>
+__global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t c = blockIdx.x;
+  const PartDesc d = p.desc[c];
+  if (d.rows == 0) return;
+  const int lane = threadIdx.x & 31;
+  const int n = d.last - (int)c + 1;                        // parts
+  constexpr int64_t SLOT = MR * (DP + 2);
+  const float *parts = p.part + (c * 2 + 1) * SLOT;         // the first; part k > 0 is the first of block c + k
+  auto part_at = [&](int k) { return parts + (k == 0 ? 0 : (2 * (int64_t)k - 1) * SLOT); };
+  const float vs = p.vs ? __ldg(p.vs + p.vs_step * d.h) : 1.0f;
+  constexpr int V = DP / 4;                                 // float4 a row
+  constexpr int SPLIT = V < 32 ? 32 / V : 1, PASS = V > 32 ? V / 32 : 1;  // parts side by side, float4 a lane
+  for (int row = blockIdx.y * (MERGE_THREADS / 32) + (threadIdx.x >> 5); row < d.rows; row += gridDim.y * (MERGE_THREADS / 32)) {
+    float base = -INFINITY;
+    for (int k = lane; k < n; k += 32) base = fmaxf(base, part_at(k)[MR * DP + row]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) base = fmaxf(base, __shfl_xor_sync(~0u, base, x));
+    const float ref = base == -INFINITY ? 0.0f : base;
+    float l = 0.0f;
+    float4 acc[PASS];
+#pragma unroll
+    for (int q = 0; q < PASS; q++) acc[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k0 = 0; k0 < n; k0 += 32) {
+      float w = 0.0f;
+      if (k0 + lane < n) {
+        const float *part = part_at(k0 + lane);
+        w = ex2(part[MR * DP + row] - ref);
+        l += w * part[MR * DP + MR + row];
+      }
+#pragma unroll 4
+      for (int j = 0; j < 32; j += SPLIT) {
+        if (k0 + j >= n) break;
+        const int mine = j + (SPLIT > 1 ? lane / V : 0);
+        const float wj = __shfl_sync(~0u, w, mine);
+        if (k0 + mine < n) {
+#pragma unroll
+          for (int q = 0; q < PASS; q++) {
+            const float4 v = *reinterpret_cast<const float4 *>(part_at(k0 + mine) + row * DP + ((SPLIT > 1 ? lane % V : lane) + 32 * q) * 4);
+            acc[q].x += wj * v.x, acc[q].y += wj * v.y, acc[q].z += wj * v.z, acc[q].w += wj * v.w;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(~0u, l, x);
+    if constexpr (SPLIT > 1) {
+#pragma unroll
+      for (int x = V; x < 32; x <<= 1) {
+        acc[0].x += __shfl_xor_sync(~0u, acc[0].x, x);
+        acc[0].y += __shfl_xor_sync(~0u, acc[0].y, x);
+        acc[0].z += __shfl_xor_sync(~0u, acc[0].z, x);
+        acc[0].w += __shfl_xor_sync(~0u, acc[0].w, x);
+      }
+    }
+    const float inv = l == 0.0f ? 0.0f : vs / l;
+    const int qr = d.row0 + row, tok = d.start + qr / p.group, head = d.h * p.group + qr % p.group;
+#pragma unroll
+    for (int q = 0; q < PASS; q++) {
+      const int d4 = ((SPLIT > 1 ? lane % V : lane) + 32 * q) * 4;
+      if (lane < V && d4 < p.d) {
+        uint16_t *out = p.out + (int64_t)tok * p.o_tok + (int64_t)head * p.o_head + d4;
+        *reinterpret_cast<uint2 *>(out) =
+            make_uint2(pack2<F16>(acc[q].x * inv, acc[q].y * inv), pack2<F16>(acc[q].z * inv, acc[q].w * inv));
+      }
+    }
+  }
+}
+
+// Launch with programmatic stream serialization: the kernel's prologue may
+// overlap the previous kernel's end (griddepcontrol.wait before the first
+// global access).
+template <typename... Params, typename... Args>
+inline void launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, int smem, cudaStream_t st, const Args &...args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+// Dynamic shared memory above 48 KB, and all of the SM's memory as shared:
+// without it an SM that has just run a kernel without shared memory may split
+// its memory for one block.
+int launch_attributes(const void *kernel, int smem);
 
 }  // namespace paged
 }  // namespace fp8b200

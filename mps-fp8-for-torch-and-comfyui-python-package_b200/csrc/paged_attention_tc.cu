@@ -387,7 +387,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
   __syncthreads();
   if (p.zero_rest) zero_rest(p, blockIdx.x, gridDim.x);
   const long long ctas = min((long long)gridDim.x, total), c = blockIdx.x;
-  if (tid == 0) p.desc[c] = make_int4(-1, 0, 0, 0);
+  if (tid == 0) p.desc[c].rows = 0;
   const long long slack = ctas > 0 ? total / ctas / 16 : 0;
   long long u = 0, u_end = 0, u_before = 0;      // the share, and the units before place x
   int u_x = 0, u_r = 0;
@@ -861,7 +861,8 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
       }
       fence_after();
       const bool begins = t_begin == 0, whole = begins && t_end == sg->units;
-      if (tid == 0 && begins && !whole) p.desc[c] = make_int4(sg->r, sg->qt, h, sg->last);
+      if (tid == 0 && begins && !whole)
+        p.desc[c] = PartDesc{min(QB, all_rows - sg->qt * QB), sg->qt * QB, h, sg->last, sg->start};
       const float vs = C::FP8 && p.vs ? __ldg(p.vs + p.vs_step * h) : 1.0f;
       const float inv = sum == 0.0f ? 0.0f : vs / sum;
       const float mine_base = base - C::SHIFT;
@@ -959,42 +960,6 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
   if (warp == C::CTRL) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-// Joins the parts of cut segments, as paged_merge_kernel does; blockIdx.y
-// takes a share of the rows.
-template <bool F16, int DP>
-__global__ void __launch_bounds__(128) paged_merge_tc_kernel(const AttnParams p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const long long c = blockIdx.x;
-  const int4 d = p.desc[c];
-  if (d.x < 0) return;
-  const Request rq = load_request(p, d.x);
-  const int64_t row0 = (int64_t)d.y * QB;
-  const int h = d.z;
-  const int rows = (int)min((int64_t)QB, (int64_t)rq.n * p.group - row0);
-  const float vs = p.vs ? __ldg(p.vs + p.vs_step * h) : 1.0f;
-  constexpr int64_t SLOT = QB * (DP + 2);
-  for (int i = blockIdx.y * 128 + threadIdx.x; i < rows * (DP / 4); i += gridDim.y * 128) {
-    const int row = i / (DP / 4), d4 = (i % (DP / 4)) * 4;
-    if (d4 >= p.d) continue;
-    float base = -INFINITY, l = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (long long b = c; b <= d.w; b++) {
-      const float *part = p.part + (b * 2 + (b == c ? 1 : 0)) * SLOT;
-      const float bb = part[QB * DP + row], bl = part[QB * DP + QB + row];
-      const float4 v = *reinterpret_cast<const float4 *>(part + row * DP + d4);
-      const float nb = fmaxf(base, bb), ref = nb == -INFINITY ? 0.0f : nb;
-      const float f = ex2(base - ref), e = ex2(bb - ref);
-      base = nb;
-      l = l * f + bl * e;
-      x[0] = x[0] * f + v.x * e, x[1] = x[1] * f + v.y * e, x[2] = x[2] * f + v.z * e, x[3] = x[3] * f + v.w * e;
-    }
-    const float inv = l == 0.0f ? 0.0f : vs / l;
-    const int qr = (int)(row0 + row), tok = rq.start + qr / p.group, head = h * p.group + qr % p.group;
-    uint16_t *out = p.out + (int64_t)tok * p.o_tok + (int64_t)head * p.o_head + d4;
-    *reinterpret_cast<uint2 *>(out) = make_uint2(pack2<F16>(x[0] * inv, x[1] * inv), pack2<F16>(x[2] * inv, x[3] * inv));
-  }
-}
-
 using TcKernel = void (*)(AttnParams, TcMaps, int);
 struct TcVariant {
   TcKernel main;
@@ -1003,7 +968,7 @@ struct TcVariant {
 };
 template <bool F16, int KV, int DP>
 TcVariant tc_variant() {
-  return {paged_attention_tc_kernel<F16, KV, DP>, paged_merge_tc_kernel<F16, DP>, Tc<F16, KV, DP>::SMEM, Tc<F16, KV, DP>::THREADS};
+  return {paged_attention_tc_kernel<F16, KV, DP>, paged_merge_kernel<F16, DP, QB>, Tc<F16, KV, DP>::SMEM, Tc<F16, KV, DP>::THREADS};
 }
 template <bool F16, int KV>
 TcVariant pick_tc(int dp) {
@@ -1028,7 +993,27 @@ EncodeTiled encode_tiled() {
 
 }  // namespace
 
-int64_t tc_workspace(int dp, int sms) { return (int64_t)sms * (2 * QB * (int64_t)(dp + 2) * 4 + 16); }
+// The attributes last as long as the process: set once a kernel and device.
+int launch_attributes(const void *kernel, int smem) {
+  static std::mutex m;
+  static const void *done[256];
+  static int devices[256], n = 0;
+  int dev;
+  if (int rc = check_device(&dev)) return rc;
+  std::lock_guard<std::mutex> lock(m);
+  for (int i = 0; i < n; i++)
+    if (done[i] == kernel && devices[i] == dev) return FP8B200_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess ||
+      cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared) != cudaSuccess)
+    return check_launch("paged_attention");
+  if (n < 256) {
+    done[n] = kernel;
+    devices[n++] = dev;
+  }
+  return FP8B200_OK;
+}
+
+int64_t tc_workspace(int dp, int sms) { return (int64_t)sms * (2 * QB * (int64_t)(dp + 2) * 4 + (int64_t)sizeof(PartDesc)); }
 
 // What a tensor map can describe: strides above 0 (below 2^40 bytes), extents below 2^31.
 bool tc_takes(const AttnParams &p) {
@@ -1039,8 +1024,8 @@ bool tc_takes(const AttnParams &p) {
 
 int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int sms, uint8_t *workspace, cudaStream_t st) {
   AttnParams p = params;
-  p.desc = (int4 *)workspace;
-  p.part = (float *)(workspace + (int64_t)sms * 16);
+  p.desc = (PartDesc *)workspace;
+  p.part = (float *)(workspace + (int64_t)sms * sizeof(PartDesc));
   const bool fp8 = cache_dtype == FP8B200_E4M3 || cache_dtype == FP8B200_E5M2;
   TcVariant v;
   if (cache_dtype == FP8B200_E4M3) v = f16 ? pick_tc<true, FP8B200_E4M3>(dp) : pick_tc<false, FP8B200_E4M3>(dp);
@@ -1064,23 +1049,9 @@ int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int s
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(FP8B200_ELAUNCH, "paged_attention: tensor map encode failed (%d)", (int)r);
   }
-  if (cudaFuncSetAttribute(v.main, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem) != cudaSuccess)
-    return check_launch("paged_attention");
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)sms);
-  cfg.blockDim = dim3((unsigned)v.threads);
-  cfg.dynamicSmemBytes = (size_t)v.smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, v.main, p, maps, box_log);
-  cfg.gridDim = dim3((unsigned)sms, 8);
-  cfg.blockDim = dim3(128);
-  cfg.dynamicSmemBytes = 0;
-  cudaLaunchKernelEx(&cfg, v.merge, p);
+  if (int rc = launch_attributes((const void *)v.main, v.smem)) return rc;
+  launch_dependent(v.main, dim3((unsigned)sms), v.threads, v.smem, st, p, maps, box_log);
+  launch_dependent(v.merge, dim3((unsigned)sms, 16), MERGE_THREADS, 0, st, p);
   count_launch(2);
   return check_launch("paged_attention");
 }
