@@ -200,6 +200,13 @@ __device__ __noinline__ void careful_row(const AttnParams &p, int r, int tok, in
       const float keep = exp2f(m - base), w = exp2f(s - base);
       m = mn;
       l = l * keep + w;
+      if (l != l) {            // a score is NaN, or +inf: so is every output
+#pragma unroll
+        for (int i = 0; i < DMAX / 32; i++) o[i] = l;
+        m_out = m;
+        l_out = l;
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < DMAX / 32; i++)
         if (lane + 32 * i < p.d) o[i] = o[i] * keep + w * cache_value<F16, KV>(p.v, e + lane + 32 * i);

@@ -52,7 +52,7 @@ namespace {
 constexpr int KT = 128;          // keys a tile
 constexpr int QT = 128;          // rows a tile
 constexpr int QB = 2 * QT;       // rows a block
-constexpr int SEG_COST = 2;       // what a segment's start and end cost, in key tiles
+constexpr int SEG_COST = 3;       // what a segment's start and end cost, in key tiles
 constexpr int SEGS = 4;           // segments in the ring
 constexpr int HIDE_RING = 8;     // tiles whose page masks are kept: more than the producers run ahead of the softmax
 constexpr unsigned long long WAIT_NS = 2000000000ull;
@@ -83,7 +83,7 @@ struct Tc {
   static constexpr int OFF_PLAN = OFF_RAW + RAWS * RAW;   // the plan's scratch
   static constexpr int OFF_HIDE = OFF_PLAN + 256;         // page masks, 128 bits a tile
   static constexpr int OFF_BARS = OFF_HIDE + HIDE_RING * 16;
-  static constexpr int BARS = 2 * SLOTS + 2 * RAWS + 8 + 2 * SEGS;
+  static constexpr int BARS = 2 * SLOTS + 2 * RAWS + 10 + 2 * SEGS;
   static constexpr int OFF_SEGS = OFF_BARS + BARS * 8;
   static constexpr int SMEM = OFF_SEGS + SEGS * 48 + 16;
   static constexpr float SHIFT = MF16 ? 7.0f : 0.0f;      // weights are scaled by 2^SHIFT and stay below 2^(SHIFT + 8)
@@ -145,31 +145,48 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// MMA and commit by the lane whose `lead` is set, in code that the whole warp runs.
-__device__ __forceinline__ void commit(uint32_t lead, uint32_t bar) {
+// MMAs and commits are issued by one thread of a warp that runs the code as a
+// whole, elected in the same statement: with any other predicate each MMA took
+// 100 cycles to issue, more than an MMA of 128 x 128 x 16 takes to run (64).
+__device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile(
       "{\n\t.reg .pred q;\n\t"
-      "setp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
-      "r"(lead)
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Four K steps of 16 along a 128-byte swizzled row: A and B advance by 32 bytes.
+__device__ __forceinline__ void mma_ss4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
+      "{\n\t.reg .pred p, t, q;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "add.u64 a1, %1, 2;\n\tadd.u64 b1, %2, 2;\n\t"
+      "add.u64 a2, %1, 4;\n\tadd.u64 b2, %2, 4;\n\t"
+      "add.u64 a3, %1, 6;\n\tadd.u64 b3, %2, 6;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Four K steps of 16 keys: A (tensor memory) advances by 8 columns, B by 16 rows of 128 bytes.
+__device__ __forceinline__ void mma_ts4(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
+      "{\n\t.reg .pred p, t, q;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+      "setp.eq.b32 t, 0, 0;\n\t"
+      "add.u32 a1, %1, 8;\n\tadd.u64 b1, %2, 128;\n\t"
+      "add.u32 a2, %1, 16;\n\tadd.u64 b2, %2, 256;\n\t"
+      "add.u32 a3, %1, 24;\n\tadd.u64 b3, %2, 384;\n\t"
+      "elect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
 #define PAGED_R32(r)                                                                                                   \
@@ -323,7 +340,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
   auto raw_full = [&](int s) { return bars + 8u * (2 * C::SLOTS + s); };
   auto raw_empty = [&](int s) { return bars + 8u * (2 * C::SLOTS + C::RAWS + s); };
   const uint32_t q_full = bars + 8u * (2 * C::SLOTS + 2 * C::RAWS), s_full = q_full + 16, p_full = q_full + 32, pv_done = q_full + 48;
-  const uint32_t seg_full = q_full + 64, seg_empty = seg_full + 8 * SEGS;
+  const uint32_t p_half = q_full + 64, seg_full = q_full + 80, seg_empty = seg_full + 8 * SEGS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   if (base_a & 1023u) {  // the swizzled tiles need it; the same for every CTA
@@ -342,6 +359,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
     for (int g = 0; g < 2; g++) {
       bar_init(q_full + 8 * g, QT);
       bar_init(s_full + 8 * g, 1);
+      bar_init(p_half + 8 * g, QT);
       bar_init(p_full + 8 * g, QT);
       bar_init(pv_done + 8 * g, 1);
     }
@@ -494,7 +512,6 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
       __syncwarp();
     } else if (warp == C::CTRL) {
       // ================================================= MMA issue
-      const uint32_t lead = lane == 0;
       int slot = 0;
       uint32_t phase = 0, segs = 0, tiles = 0;
       bool ok = true;
@@ -504,11 +521,9 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
       auto issue_s = [&](int g, int s) {
         const uint64_t qd = desc_k(base_a + g * C::TILE), kd = desc_k(kv_a + s * C::TILE);
 #pragma unroll
-        for (int k = 0; k < DP / 16; k++) {
-          const uint64_t at = (uint64_t)((k >> 2) * (KT * 128 / 16) + (k & 3) * 2);  // 16-byte units
-          mma_ss(lead, tmem + 128 * g, qd + at, kd + at, C::IDESC_S, k > 0);
-        }
-        commit(lead, s_full + 8 * g);
+        for (int k = 0; k < DP / 64; k++)
+          mma_ss4(tmem + 128 * g, qd + k * (KT * 128 / 16), kd + k * (KT * 128 / 16), C::IDESC_S, k > 0);
+        commit(s_full + 8 * g);
       };
       while (ok) {
         const Segment *sg = seg_at(segs, 51);
@@ -523,7 +538,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
         fence_after();
         issue_s(0, slot);
         issue_s(1, slot);
-        commit(lead, kv_empty(slot));
+        commit(kv_empty(slot));
         step();
         for (int j = 0; j < n && ok; j++) {
           const bool more = j + 1 < n;
@@ -537,20 +552,23 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
           step();
 #pragma unroll 1
           for (int g = 0; g < 2; g++) {
-            ok = ok && bar_wait(p_full + 8 * g, tiles & 1, s_failed, 6 + g);
+            ok = ok && bar_wait(p_half + 8 * g, tiles & 1, s_failed, 6 + g);
             ok = __all_sync(~0u, ok);
             if (!ok) break;
             fence_after();
             const uint64_t vd = desc_mn(kv_a + vs * C::TILE, KT * 128);
-#pragma unroll
-            for (int k = 0; k < KT / 16; k++)
-              mma_ts(lead, tmem + 256 + DP * g, tmem + 128 * g + 8 * k, vd + k * (2048 / 16), C::IDESC_O, j > 0 || k > 0);
-            commit(lead, pv_done + 8 * g);
+            mma_ts4(tmem + 256 + DP * g, tmem + 128 * g, vd, C::IDESC_O, j > 0);
+            ok = bar_wait(p_full + 8 * g, tiles & 1, s_failed, 8 + g);
+            ok = __all_sync(~0u, ok);
+            if (!ok) break;
+            fence_after();
+            mma_ts4(tmem + 256 + DP * g, tmem + 128 * g + 32, vd + 512, C::IDESC_O, 1);
+            commit(pv_done + 8 * g);
             if (more) issue_s(g, ks);
           }
           if (!ok) break;
-          commit(lead, kv_empty(vs));
-          if (more) commit(lead, kv_empty(ks));
+          commit(kv_empty(vs));
+          if (more) commit(kv_empty(ks));
           tiles++;
         }
         segs++;
@@ -839,6 +857,11 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
             pk[i] = pack2<C::MF16>(e.x, e.y);
           }
           tst16(t_s + 16 * c4, pk);
+          if (c4 == 1) {                                   // the second product can begin with half of the keys
+            tst_wait();
+            fence_before();
+            bar_arrive(p_half + 8 * g);
+          }
         }
         tst_wait();
         fence_before();
