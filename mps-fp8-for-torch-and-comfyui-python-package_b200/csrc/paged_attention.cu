@@ -104,55 +104,89 @@ __device__ __forceinline__ long long units_of(const AttnParams &p, int r, int &t
   return row_tiles * p.hk * tiles;
 }
 
+// a / b and the rest, in 32 bits where they fit (a 64-bit division is a call of
+// some hundred cycles, and these stand in front of the first load).
+__device__ __forceinline__ long long quotient(long long a, long long b, long long &rest) {
+  if (((a | b) >> 32) == 0) {
+    const uint32_t q = (uint32_t)a / (uint32_t)b;
+    rest = (uint32_t)a - q * (uint32_t)b;
+    return q;
+  }
+  const long long q = a / b;
+  rest = a - q * b;
+  return q;
+}
+
 // A block's share [u, u_end) of the line of units, found by all its threads:
-// the request that u falls into and the units before that request. At least
-// MIN_UNITS a block: below that the join costs more than the share saves.
+// the request that u falls into and the units before that request. The first
+// `extra` blocks have `each` + 1 units, the others `each`; at least MIN_UNITS a
+// block, below that the join costs more than the share saves.
 constexpr int MIN_UNITS = 2;
 struct Share {
-  long long u, u_end, before, total, blocks;
+  long long u, u_end, before, each, extra;
   int r;  // -1: nothing for this block
+  // the block that has unit x
+  __device__ __forceinline__ int block_of(long long x) const {
+    long long rest;
+    const long long front = extra * (each + 1);
+    return (int)(x < front ? quotient(x, each + 1, rest) : extra + quotient(x - front, each, rest));
+  }
 };
 template <int MR>
 __device__ __forceinline__ Share find_share(const AttnParams &p, long long *s_scan) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Share sh;
   int tiles;
-  const long long first = tid < p.requests ? units_of<MR>(p, tid, tiles) : 0;
-  long long sum = first;
-  for (int r = tid + THREADS; r < p.requests; r += THREADS) sum += units_of<MR>(p, r, tiles);
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-  if (lane == 0) s_scan[warp] = sum;
-  __syncthreads();
-  sh.total = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
-  sh.blocks = min((long long)gridDim.x, (sh.total + MIN_UNITS - 1) / MIN_UNITS);
-  sh.r = -1;
-  sh.u = sh.u_end = sh.before = 0;
-  const long long c = blockIdx.x;
-  if (tid == 0) p.desc[c].rows = 0;
-  if (c >= sh.blocks) return sh;
-  sh.u = c * sh.total / sh.blocks;
-  sh.u_end = (c + 1) * sh.total / sh.blocks;
-  long long before = 0;
-  for (int r0 = 0; r0 < p.requests; r0 += THREADS) {
-    const int r = r0 + tid;
-    const long long mine = r0 == 0 ? first : r < p.requests ? units_of<MR>(p, r, tiles) : 0;
+  // inclusive scan over up to THREADS requests; with more, their sum first
+  auto scan = [&](long long mine, long long &total) {
     long long inc = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const long long a = __shfl_up_sync(~0u, inc, d);
       if (lane >= d) inc += a;
     }
-    __syncthreads();
     if (lane == 31) s_scan[warp] = inc;
     __syncthreads();
-    long long base = before;
-    for (int w = 0; w < warp; w++) base += s_scan[w];
-    before += s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
-    if (base + inc > sh.u && base + inc - mine <= sh.u) {
-      s_scan[4] = r;
-      s_scan[5] = base + inc - mine;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      if (w < warp) inc += s_scan[w];
+      total += s_scan[w];
     }
+    return inc;
+  };
+  const long long first = tid < p.requests ? units_of<MR>(p, tid, tiles) : 0;
+  long long total, inc = scan(first, total);
+  if (p.requests > THREADS) {
+    long long more = 0, sum;
+    for (int r = tid + THREADS; r < p.requests; r += THREADS) more += units_of<MR>(p, r, tiles);
+    __syncthreads();
+    scan(more, sum);
+    total += sum;
+  }
+  const long long c = blockIdx.x;
+  if (tid == 0) p.desc[c].rows = 0;
+  const long long blocks = min((long long)gridDim.x, (total + MIN_UNITS - 1) / MIN_UNITS);
+  sh.r = -1;
+  sh.u = sh.u_end = sh.before = sh.each = sh.extra = 0;
+  if (c >= blocks) return sh;
+  sh.each = quotient(total, blocks, sh.extra);
+  sh.u = c * sh.each + min(c, sh.extra);
+  sh.u_end = sh.u + sh.each + (c < sh.extra);
+  long long before = 0, mine = first;
+  for (int r0 = 0; r0 < p.requests; r0 += THREADS) {
+    const int r = r0 + tid;
+    long long all = total;
+    if (p.requests > THREADS) {
+      mine = r < p.requests ? units_of<MR>(p, r, tiles) : 0;
+      __syncthreads();
+      inc = scan(mine, all);
+    }
+    if (before + inc > sh.u && before + inc - mine <= sh.u) {
+      s_scan[4] = r;
+      s_scan[5] = before + inc - mine;
+    }
+    before += all;
     if (before > sh.u) break;
   }
   __syncthreads();
@@ -233,12 +267,10 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Share sh = find_share<C::MR>(p, s_scan);
-  if (p.zero_rest) zero_rest(p, blockIdx.x, gridDim.x);
-  if (sh.r < 0) return;
   const long long c = blockIdx.x;
   long long u = sh.u, before = sh.before;
   int r = sh.r;
-  while (u < sh.u_end) {
+  while (r >= 0 && u < sh.u_end) {
     // ---- the segment that unit u belongs to
     const Request rq = load_request(p, r);
     int tiles_n;
@@ -248,10 +280,9 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged
       r++;
       continue;
     }
-    const int local = (int)(u - before) % tiles_n;
-    const long long seg = (u - before) / tiles_n;
-    const int t_begin = local, t_end = (int)min((long long)tiles_n, t_begin + (sh.u_end - u));
-    const int h = (int)(seg % p.hk), qt = (int)(seg / p.hk);
+    long long in_tiles, in_heads;
+    const int qt = (int)quotient(quotient(u - before, tiles_n, in_tiles), p.hk, in_heads), h = (int)in_heads;
+    const int t_begin = (int)in_tiles, t_end = (int)min((long long)tiles_n, t_begin + (sh.u_end - u));
     const long long seg_start = u - t_begin;
     u += t_end - t_begin;
     const Tiles<BN> tl = visible_tiles<BN>(p, rq.first, rq.first + rq.n - 1);
@@ -302,20 +333,25 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged
     long long off[C::ST];
 #pragma unroll
     for (int k = 0; k < C::ST; k++) off[k] = find(t_begin + k);  // all table reads in flight at once
-    for (int i = tid; i < C::MR * (DP / 8); i += THREADS) {
-      const int row = i / (DP / 8), cu = i % (DP / 8);
-      uint4 v = make_uint4(0, 0, 0, 0);
+    constexpr int QN = C::MR * (DP / 8) / THREADS;           // 16-byte units of the queries a thread loads
+    uint4 qv[QN];
+#pragma unroll
+    for (int k = 0; k < QN; k++) {
+      const int row = (tid + k * THREADS) / (DP / 8), cu = (tid + k * THREADS) % (DP / 8);
+      qv[k] = make_uint4(0, 0, 0, 0);
       if (row < rows && cu * 8 < p.d) {
-        const int qr = row0 + row, tok = rq.start + qr / p.group, head = h * p.group + qr % p.group;
-        v = __ldg(reinterpret_cast<const uint4 *>(p.q + (int64_t)tok * p.q_tok + (int64_t)head * p.q_head + cu * 8));
+        const int qr = row0 + row, tok = qr / p.group, head = h * p.group + qr - tok * p.group;
+        qv[k] = __ldg(reinterpret_cast<const uint4 *>(p.q + (int64_t)(rq.start + tok) * p.q_tok + (int64_t)head * p.q_head + cu * 8));
       }
-      *reinterpret_cast<uint4 *>(s_q + row * C::QROW + cu * 16) = v;
     }
 #pragma unroll
     for (int k = 0; k < C::ST - 1; k++) {
       issue(k, off[k]);
       cp_commit();
     }
+#pragma unroll
+    for (int k = 0; k < QN; k++)
+      *reinterpret_cast<uint4 *>(s_q + (tid + k * THREADS) / (DP / 8) * C::QROW + (tid + k * THREADS) % (DP / 8) * 16) = qv[k];
     long long ahead = off[C::ST - 1];                       // offsets of the next tile to load
     __syncthreads();
     if ((C::FP8 && !F16) || scale < 0.0f) {
@@ -533,7 +569,7 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged
     const float vs = C::FP8 && p.vs ? __ldg(p.vs + p.vs_step * h) : 1.0f;
     float *part = p.part + (c * 2 + (begins ? 1 : 0)) * (int64_t)(C::MR * (DP + 2));
     if (tid == 0 && begins && !ends)
-      p.desc[c] = PartDesc{rows, row0, h, (int)(((seg_start + tiles_n) * sh.blocks - 1) / sh.total), rq.start};
+      p.desc[c] = PartDesc{rows, row0, h, sh.block_of(seg_start + tiles_n - 1), rq.start};
     float *s_o = reinterpret_cast<float *>(smem);           // [4 warps][16 rows][DP]
 #pragma unroll
     for (int mg = 0; mg < MG; mg++) {
@@ -607,6 +643,7 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged
       }
     }
   }
+  if (p.zero_rest) zero_rest(p, blockIdx.x, gridDim.x);
 }
 
 // ------------------------------------------------------------------ more rows
@@ -661,7 +698,7 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
   const Share sh = find_share<C::MR>(p, s_scan);
   if (p.zero_rest) zero_rest(p, blockIdx.x, gridDim.x);
   if (sh.r < 0) return;
-  const long long c = blockIdx.x, u_end = sh.u_end, blocks = sh.blocks, total = sh.total;
+  const long long c = blockIdx.x, u_end = sh.u_end;
   long long u = sh.u, before = sh.before;
   int r = sh.r;
   while (u < u_end) {
@@ -1037,7 +1074,7 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
     const float vs = C::FP8 && p.vs ? __ldg(p.vs + p.vs_step * h) : 1.0f;
     float *part = p.part + (c * 2 + (begins ? 1 : 0)) * (int64_t)(C::MR * (DP + 2));
     if (tid == 0 && begins && !ends)
-      p.desc[c] = PartDesc{rows, row0, h, (int)(((seg_start + tiles_n) * blocks - 1) / total), rq.start};
+      p.desc[c] = PartDesc{rows, row0, h, sh.block_of(seg_start + tiles_n - 1), rq.start};
     for (int i = tid; i < rows * (DP / 4); i += THREADS) {
       const int row = i / (DP / 4), d4 = (i % (DP / 4)) * 4;
       const int at = (row >> 4) * C::KW * 16 + (row & 15);
@@ -1214,7 +1251,8 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
   if (int rc = launch_attributes((const void *)v.main, v.smem)) return rc;
   const int grid = current_sm_count() * v.per_sm;
   launch_dependent(v.main, dim3((unsigned)grid), THREADS, v.smem, (cudaStream_t)stream, p);
-  launch_dependent(v.merge, dim3((unsigned)grid, 4), MERGE_THREADS, 0, (cudaStream_t)stream, p);
+  p.blocks = grid;
+  launch_dependent(v.merge, dim3((unsigned)current_sm_count(), (unsigned)(v.rows / 16)), MERGE_THREADS, 0, (cudaStream_t)stream, p);
   count_launch(2);
   return check_launch("paged_attention");
 }

@@ -43,6 +43,7 @@ struct AttnParams {
   // split segments: partial results and which block continues what
   float *part;
   PartDesc *desc;
+  int blocks;                 // for the merge: how many descriptors there are
 };
 
 // The new tokens of request r: rows [start, start + n) of q, the last at
@@ -220,15 +221,12 @@ __device__ __noinline__ void careful_row(const AttnParams &p, int r, int tok, in
 // in block c of the attention kernel (its second part), with the first parts
 // of the blocks after it, in their order. A warp a row: its lanes fetch the
 // parts' bases and sums together, then the rows' values, whose loads do not
-// wait for one another. MR: rows a part has room for.
-constexpr int MERGE_THREADS = 128;
+// wait for one another. MR: rows a part has room for. A block an SM (times
+// the row groups) goes through the descriptors: so few fit beside the
+// attention kernel's blocks and are there when it ends.
+constexpr int MERGE_THREADS = 256;
 template <bool F16, int DP, int MR>
-__global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnParams p) {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int64_t c = blockIdx.x;
-  const PartDesc d = p.desc[c];
-  if (d.rows == 0) return;
+__device__ __forceinline__ void merge_segment(const AttnParams &p, int64_t c, const PartDesc &d) {
   const int lane = threadIdx.x & 31;
   const int n = d.last - (int)c + 1;                        // parts
   constexpr int64_t SLOT = MR * (DP + 2);
@@ -238,34 +236,45 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnPa
   constexpr int V = DP / 4;                                 // float4 a row
   constexpr int SPLIT = V < 32 ? 32 / V : 1, PASS = V > 32 ? V / 32 : 1;  // parts side by side, float4 a lane
   for (int row = blockIdx.y * (MERGE_THREADS / 32) + (threadIdx.x >> 5); row < d.rows; row += gridDim.y * (MERGE_THREADS / 32)) {
-    float base = -INFINITY;
-    for (int k = lane; k < n; k += 32) base = fmaxf(base, part_at(k)[MR * DP + row]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) base = fmaxf(base, __shfl_xor_sync(~0u, base, x));
-    const float ref = base == -INFINITY ? 0.0f : base;
-    float l = 0.0f;
+    // AT parts at a time: their values, bases and sums in flight together
+    constexpr int AT = 16 / PASS, N = AT / SPLIT;
+    float base = -INFINITY, l = 0.0f;
     float4 acc[PASS];
 #pragma unroll
     for (int q = 0; q < PASS; q++) acc[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int k0 = 0; k0 < n; k0 += 32) {
-      float w = 0.0f;
-      if (k0 + lane < n) {
-        const float *part = part_at(k0 + lane);
-        w = ex2(part[MR * DP + row] - ref);
-        l += w * part[MR * DP + MR + row];
-      }
-#pragma unroll 4
-      for (int j = 0; j < 32; j += SPLIT) {
-        if (k0 + j >= n) break;
-        const int mine = j + (SPLIT > 1 ? lane / V : 0);
-        const float wj = __shfl_sync(~0u, w, mine);
-        if (k0 + mine < n) {
+#pragma unroll 1
+    for (int k0 = 0; k0 < n; k0 += AT) {
+      float4 v[N][PASS];
+      const int side = SPLIT > 1 ? lane / V : 0;
 #pragma unroll
-          for (int q = 0; q < PASS; q++) {
-            const float4 v = *reinterpret_cast<const float4 *>(part_at(k0 + mine) + row * DP + ((SPLIT > 1 ? lane % V : lane) + 32 * q) * 4);
-            acc[q].x += wj * v.x, acc[q].y += wj * v.y, acc[q].z += wj * v.z, acc[q].w += wj * v.w;
-          }
+      for (int j = 0; j < N; j++)
+#pragma unroll
+        for (int q = 0; q < PASS; q++) {
+          v[j][q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (k0 + j * SPLIT + side < n)
+            v[j][q] = *reinterpret_cast<const float4 *>(part_at(k0 + j * SPLIT + side) + row * DP + ((SPLIT > 1 ? lane % V : lane) + 32 * q) * 4);
         }
+      float b = -INFINITY, bl = 0.0f;
+      if (lane < AT && k0 + lane < n) {
+        const float *part = part_at(k0 + lane) + MR * DP + row;
+        b = part[0];
+        bl = part[MR];
+      }
+      float nb = fmaxf(base, b);
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) nb = fmaxf(nb, __shfl_xor_sync(~0u, nb, x));
+      const float ref = nb == -INFINITY ? 0.0f : nb, f = ex2(base - ref), w = ex2(b - ref);
+      base = nb;
+      l = l * f + w * bl;
+#pragma unroll
+      for (int q = 0; q < PASS; q++) acc[q].x *= f, acc[q].y *= f, acc[q].z *= f, acc[q].w *= f;
+#pragma unroll
+      for (int j = 0; j < N; j++) {
+        const float wj = __shfl_sync(~0u, w, j * SPLIT + side);
+        if (k0 + j * SPLIT + side < n)
+#pragma unroll
+          for (int q = 0; q < PASS; q++)
+            acc[q].x += wj * v[j][q].x, acc[q].y += wj * v[j][q].y, acc[q].z += wj * v[j][q].z, acc[q].w += wj * v[j][q].w;
       }
     }
 #pragma unroll
@@ -290,6 +299,16 @@ __global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnPa
             make_uint2(pack2<F16>(acc[q].x * inv, acc[q].y * inv), pack2<F16>(acc[q].z * inv, acc[q].w * inv));
       }
     }
+  }
+}
+
+template <bool F16, int DP, int MR>
+__global__ void __launch_bounds__(MERGE_THREADS) paged_merge_kernel(const AttnParams p) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int c = blockIdx.x; c < p.blocks; c += gridDim.x) {
+    const PartDesc d = p.desc[c];
+    if (d.rows) merge_segment<F16, DP, MR>(p, c, d);
   }
 }
 

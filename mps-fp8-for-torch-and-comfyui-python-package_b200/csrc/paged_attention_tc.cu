@@ -1049,6 +1049,7 @@ int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int s
   AttnParams p = params;
   p.desc = (PartDesc *)workspace;
   p.part = (float *)(workspace + (int64_t)sms * sizeof(PartDesc));
+  p.blocks = sms;
   const bool fp8 = cache_dtype == FP8B200_E4M3 || cache_dtype == FP8B200_E5M2;
   TcVariant v;
   if (cache_dtype == FP8B200_E4M3) v = f16 ? pick_tc<true, FP8B200_E4M3>(dp) : pick_tc<false, FP8B200_E4M3>(dp);
@@ -1074,7 +1075,7 @@ int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int s
   }
   if (int rc = launch_attributes((const void *)v.main, v.smem)) return rc;
   launch_dependent(v.main, dim3((unsigned)sms), v.threads, v.smem, st, p, maps, box_log);
-  launch_dependent(v.merge, dim3((unsigned)sms, 16), MERGE_THREADS, 0, st, p);
+  launch_dependent(v.merge, dim3((unsigned)sms, 8), MERGE_THREADS, 0, st, p);
   count_launch(2);
   return check_launch("paged_attention");
 }

@@ -102,7 +102,7 @@ def _launch(dev: torch.device, fn, what: str, *args) -> None:
 
 def slots_outputs(requests: int, num_tokens: int, dev: torch.device) -> PagedStep:
     """The tensors of a step, the int32 ones in one allocation."""
-    cu, kv, pos, head = torch.empty(2 * requests + 2 + num_tokens, dtype=torch.int32, device=dev).split(
+    cu, kv, pos, head = torch.empty(2 * requests + 2 + num_tokens, dtype=torch.int32, device=dev).split_with_sizes(
         [requests + 1, requests, num_tokens, 1])
     return PagedStep(cu, kv, pos, torch.empty(num_tokens, dtype=torch.int64, device=dev), head)
 
