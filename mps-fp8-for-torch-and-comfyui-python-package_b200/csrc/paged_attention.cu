@@ -222,14 +222,19 @@ __device__ __forceinline__ void normalise_rows(uint8_t *s_q, int qrow, int rows,
 
 // ------------------------------------------------------------------ few rows
 //
-// Up to 16 * MG query rows a request (decoding, a few drafted tokens). The
-// four warps of a block share nothing but the queries: each takes 16 of a
+// Up to 8 * NG query rows a request (decoding, a few drafted tokens). The
+// products are turned around: S^T = K Q^T and O^T = V^T P^T, so that keys and
+// dims fill the MMA's 16 rows and the query rows its 8 columns: half the MMAs
+// and exponentials of 16-row tiles where a decode has 8 rows or fewer (the
+// warp-level MMAs bound the 64 ragged decodes then, not the cache's bytes). P^T
+// becomes the second product's operand by an 8 x 8 transpose (movmatrix).
+// The four warps of a block share nothing but the queries: each takes 16 of a
 // tile's 64 keys, brings them into a ring of its own and multiplies them with
 // all rows, so there is no block barrier between a segment's ends, a key's
 // codes are converted once whatever the number of rows, and the SM's warps
 // drift apart and cover one another's latencies. O is rescaled only when a
 // row's maximum has grown by more than 2^8 (see paged_attention_tc.cu).
-template <bool F16, int KV, int DP, int MG>
+template <bool F16, int KV, int DP, int NG>
 struct Few {
   static constexpr bool FP8 = is_fp8<KV>;
   static constexpr bool MF16 = F16 || FP8;
@@ -238,22 +243,26 @@ struct Few {
   static constexpr int HALF = WK * ROWB;                  // K or V of them
   static constexpr int ST = DP == 256 && !FP8 ? 2 : DP == 64 ? 4 : 3;
   static constexpr int RING = ST * 2 * HALF;              // a warp's
-  static constexpr int MR = 16 * MG;
+  static constexpr int MR = 8 * NG;
   static constexpr int QROW = DP * 2 + 16;
+  static constexpr int SO = DP + 4;                       // floats a row of the warps' outputs (padded: no bank conflicts)
   static constexpr int OFF_Q = 4 * RING;
   static constexpr int OFF_SCALE = OFF_Q + MR * QROW;     // [MR] query scales, [4][MR] bases, [4][MR] sums
   static constexpr int OFF_SCAN = OFF_SCALE + 9 * MR * 4;
   static constexpr int SMEM = OFF_SCAN + 64;
   static constexpr float SHIFT = MF16 ? 7.0f : 0.0f;
-  static constexpr bool QREG = MG == 1 && DP <= 128;      // query fragments stay in registers
-  static constexpr int PER_SM = DP == 256 ? (FP8 ? 2 : 1) : (DP == 128 && (!FP8 || MG > 1)) ? 2 : MG > 2 ? 2 : DP == 64 && MG == 1 && FP8 ? 4 : 3;
-  static_assert(4 * 16 * DP * 4 <= 4 * RING, "the warps' outputs of one row group fit the drained rings");
+  static constexpr bool QREG = NG * DP <= 128;            // query fragments stay in registers
+  // blocks an SM: what the registers (outputs: NG * DP / 4 a thread) and the rings leave
+  static constexpr int PER_SM = DP == 256 ? (FP8 ? 2 : 1)
+                                : DP == 128 ? (FP8 ? (NG == 1 ? 4 : NG == 2 ? 3 : 2) : 2)
+                                            : (NG <= 2 ? (FP8 ? 4 : 3) : NG == 4 ? 3 : 2);
+  static_assert(4 * 16 * SO * 4 <= 4 * RING, "the warps' outputs of 16 rows fit the drained rings");
   static_assert(PER_SM * (SMEM + 1024) <= 233472, "blocks an SM");
 };
 
-template <bool F16, int KV, int DP, int MG>
-__global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged_few_kernel(const AttnParams p) {
-  using C = Few<F16, KV, DP, MG>;
+template <bool F16, int KV, int DP, int NG>
+__global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, NG>::PER_SM)) paged_few_kernel(const AttnParams p) {
+  using C = Few<F16, KV, DP, NG>;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t *s_q = smem + C::OFF_Q;
   float *s_qscale = reinterpret_cast<float *>(smem + C::OFF_SCALE), *s_base = s_qscale + C::MR, *s_sum = s_base + 4 * C::MR;
@@ -333,7 +342,7 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged
     long long off[C::ST];
 #pragma unroll
     for (int k = 0; k < C::ST; k++) off[k] = find(t_begin + k);  // all table reads in flight at once
-    constexpr int QN = C::MR * (DP / 8) / THREADS;           // 16-byte units of the queries a thread loads
+    constexpr int QU = C::MR * (DP / 8), QN = (QU + THREADS - 1) / THREADS;  // 16-byte units of the queries, a thread's
     uint4 qv[QN];
 #pragma unroll
     for (int k = 0; k < QN; k++) {
@@ -351,50 +360,52 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged
     }
 #pragma unroll
     for (int k = 0; k < QN; k++)
-      *reinterpret_cast<uint4 *>(s_q + (tid + k * THREADS) / (DP / 8) * C::QROW + (tid + k * THREADS) % (DP / 8) * 16) = qv[k];
+      if (tid + k * THREADS < QU)
+        *reinterpret_cast<uint4 *>(s_q + (tid + k * THREADS) / (DP / 8) * C::QROW + (tid + k * THREADS) % (DP / 8) * 16) = qv[k];
     long long ahead = off[C::ST - 1];                       // offsets of the next tile to load
     __syncthreads();
     if ((C::FP8 && !F16) || scale < 0.0f) {
       normalise_rows<C::FP8 && !F16, DP>(s_q, C::QROW, C::MR, s_qscale, scale < 0.0f ? 0x80008000u : 0u);
       __syncthreads();
     }
-    auto load_q = [&](int mg, int ks, uint32_t (&a)[4]) {
-      const uint8_t *q0 = s_q + (mg * 16 + g) * C::QROW, *q1 = q0 + 8 * C::QROW;
+    // the queries as the first product's B: row ng * 8 + g, values of K step ks
+    auto load_q = [&](int ng, int ks, uint32_t (&q)[2]) {
+      const uint8_t *q0 = s_q + (ng * 8 + g) * C::QROW;
       if constexpr (C::FP8) {                               // k order of a 64-value block: lane tg holds values 16 tg .. 16 tg + 15
-        const int at = ((ks >> 2) * 64 + tg * 16 + (ks & 3) * 4) * 2;
-        const uint2 x = *reinterpret_cast<const uint2 *>(q0 + at), y = *reinterpret_cast<const uint2 *>(q1 + at);
-        a[0] = x.x, a[1] = y.x, a[2] = x.y, a[3] = y.y;
+        const uint2 x = *reinterpret_cast<const uint2 *>(q0 + ((ks >> 2) * 64 + tg * 16 + (ks & 3) * 4) * 2);
+        q[0] = x.x, q[1] = x.y;
       } else {
         const int at = (ks * 16 + tg * 2) * 2;
-        a[0] = *reinterpret_cast<const uint32_t *>(q0 + at);
-        a[1] = *reinterpret_cast<const uint32_t *>(q1 + at);
-        a[2] = *reinterpret_cast<const uint32_t *>(q0 + at + 16);
-        a[3] = *reinterpret_cast<const uint32_t *>(q1 + at + 16);
+        q[0] = *reinterpret_cast<const uint32_t *>(q0 + at);
+        q[1] = *reinterpret_cast<const uint32_t *>(q0 + at + 16);
       }
     };
-    uint32_t qf[C::QREG ? DP / 16 : 1][4];
+    uint32_t qf[C::QREG ? NG : 1][C::QREG ? DP / 16 : 1][2];
     if constexpr (C::QREG) {
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ks++) load_q(0, ks, qf[ks]);
-    }
-    float sc[MG][2];                                        // of rows g and g + 8 of each group; above 0, see paged_attention_tc.cu
-    int pos[MG][2];
+      for (int ng = 0; ng < NG; ng++)
 #pragma unroll
-    for (int mg = 0; mg < MG; mg++)
+        for (int ks = 0; ks < DP / 16; ks++) load_q(ng, ks, qf[ng][ks]);
+    }
+    // a thread's rows: ng * 8 + 2 tg and the next; its keys of a tile: g and g + 8
+    float sc[NG][2];                                        // above 0, see paged_attention_tc.cu
+    int pos[NG][2];
+#pragma unroll
+    for (int ng = 0; ng < NG; ng++)
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const int row = mg * 16 + g + 8 * e;
-        sc[mg][e] = fabsf(scale) * ((C::FP8 && !F16) ? s_qscale[row] : 1.0f);
-        if (sc[mg][e] == 0.0f) sc[mg][e] = 1e-30f;
-        pos[mg][e] = rq.first + min(row0 + row, row0 + rows - 1) / p.group;
+        const int row = ng * 8 + 2 * tg + e;
+        sc[ng][e] = fabsf(scale) * ((C::FP8 && !F16) ? s_qscale[row] : 1.0f);
+        if (sc[ng][e] == 0.0f) sc[ng][e] = 1e-30f;
+        pos[ng][e] = rq.first + min(row0 + row, row0 + rows - 1) / p.group;
       }
-    float o[MG][DP / 8][4], base[MG][2], sum[MG][2];
+    float o[NG][DP / 16][4], base[NG][2], sum[NG][2];
 #pragma unroll
-    for (int mg = 0; mg < MG; mg++) {
+    for (int ng = 0; ng < NG; ng++) {
 #pragma unroll
-      for (int i = 0; i < DP / 8; i++) o[mg][i][0] = o[mg][i][1] = o[mg][i][2] = o[mg][i][3] = 0.0f;
-      base[mg][0] = base[mg][1] = -INFINITY;
-      sum[mg][0] = sum[mg][1] = 0.0f;
+      for (int i = 0; i < DP / 16; i++) o[ng][i][0] = o[ng][i][1] = o[ng][i][2] = o[ng][i][3] = 0.0f;
+      base[ng][0] = base[ng][1] = -INFINITY;
+      sum[ng][0] = sum[ng][1] = 0.0f;
     }
 
     int stage = 0;
@@ -411,136 +422,123 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged
       }
       const uint32_t kt = ring_a + stage * 2 * C::HALF, vt = kt + C::HALF;
       if (++stage == C::ST) stage = 0;
-      float s[MG][2][4];
+      float s[NG][4];                                       // [keys g, g + 8][rows 2 tg, 2 tg + 1]
 #pragma unroll
-      for (int mg = 0; mg < MG; mg++)
+      for (int ng = 0; ng < NG; ng++) s[ng][0] = s[ng][1] = s[ng][2] = s[ng][3] = 0.0f;
+      auto first_product = [&](int ks, const uint32_t (&a)[4]) {
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++) s[mg][nt][0] = s[mg][nt][1] = s[mg][nt][2] = s[mg][nt][3] = 0.0f;
+        for (int ng = 0; ng < NG; ng++) {
+          if constexpr (C::QREG) {
+            mma<C::MF16>(s[ng], a, qf[ng][ks][0], qf[ng][ks][1]);
+          } else {
+            uint32_t q[2];
+            load_q(ng, ks, q);
+            mma<C::MF16>(s[ng], a, q[0], q[1]);
+          }
+        }
+      };
       if constexpr (C::FP8) {
 #pragma unroll
         for (int b = 0; b < DP / 64; b++) {
-          uint32_t w[2][4];
+          uint32_t w[2][4];                                 // 16 codes of keys g and g + 8
 #pragma unroll
-          for (int nt = 0; nt < 2; nt++)
+          for (int e = 0; e < 2; e++)
             asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(w[nt][0]), "=r"(w[nt][1]), "=r"(w[nt][2]), "=r"(w[nt][3])
-                         : "r"(kt + unit_at<C::ROWB, true>(nt * 8 + g, b * 4 + tg)));
+                         : "=r"(w[e][0]), "=r"(w[e][1]), "=r"(w[e][2]), "=r"(w[e][3])
+                         : "r"(kt + unit_at<C::ROWB, true>(e * 8 + g, b * 4 + tg)));
 #pragma unroll
           for (int ks = 0; ks < 4; ks++) {
-            uint32_t a[MG][4];
-#pragma unroll
-            for (int mg = 0; mg < MG; mg++) {
-              if constexpr (C::QREG) a[mg][0] = qf[b * 4 + ks][0], a[mg][1] = qf[b * 4 + ks][1], a[mg][2] = qf[b * 4 + ks][2], a[mg][3] = qf[b * 4 + ks][3];
-              else load_q(mg, b * 4 + ks, a[mg]);
-            }
-#pragma unroll
-            for (int nt = 0; nt < 2; nt++) {
-              const uint32_t b0 = fp8x2_to_f16x2<KV>(w[nt][ks] & 0xFFFFu), b1 = fp8x2_to_f16x2<KV>(w[nt][ks] >> 16);
-#pragma unroll
-              for (int mg = 0; mg < MG; mg++) mma<true>(s[mg][nt], a[mg], b0, b1);
-            }
+            const uint32_t a[4] = {fp8x2_to_f16x2<KV>(w[0][ks] & 0xFFFFu), fp8x2_to_f16x2<KV>(w[1][ks] & 0xFFFFu),
+                                   fp8x2_to_f16x2<KV>(w[0][ks] >> 16), fp8x2_to_f16x2<KV>(w[1][ks] >> 16)};
+            first_product(b * 4 + ks, a);
           }
         }
       } else {
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ks++) {
-          uint32_t b[4];
-          ldsm4(kt + unit_at<C::ROWB, false>(((lane >> 4) << 3) + (lane & 7), ks * 2 + ((lane >> 3) & 1)), b);
-#pragma unroll
-          for (int mg = 0; mg < MG; mg++) {
-            uint32_t a[4];
-            if constexpr (C::QREG) a[0] = qf[ks][0], a[1] = qf[ks][1], a[2] = qf[ks][2], a[3] = qf[ks][3];
-            else load_q(mg, ks, a);
-            mma<C::MF16>(s[mg][0], a, b[0], b[1]);
-            mma<C::MF16>(s[mg][1], a, b[2], b[3]);
-          }
+          uint32_t a[4];
+          ldsm4(kt + unit_at<C::ROWB, false>((((lane >> 3) & 1) << 3) + (lane & 7), ks * 2 + (lane >> 4)), a);
+          first_product(ks, a);
         }
       }
       const int k0 = tl.at(i) * BN + warp * C::WK;
       const uint32_t hide = (uint32_t)(hidden >> (16 * (C::ST - 1))) & 0xFFFFu;
       if (k0 + C::WK - 1 > pos_lo || hide || (p.window > 0 && pos_hi - k0 >= p.window && k0 + C::WK - 1 >= p.sinks)) {
 #pragma unroll
-        for (int mg = 0; mg < MG; mg++)
+        for (int e = 0; e < 2; e++) {
+          const int kk = g + 8 * e;
+          const bool gone = (hide >> kk) & 1u;
 #pragma unroll
-          for (int nt = 0; nt < 2; nt++)
+          for (int ng = 0; ng < NG; ng++)
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-              const int kk = nt * 8 + tg * 2 + x;
-              const bool gone = (hide >> kk) & 1u;
-              if (gone || !visible(p, k0 + kk, pos[mg][0])) s[mg][nt][x] = -INFINITY;
-              if (gone || !visible(p, k0 + kk, pos[mg][1])) s[mg][nt][2 + x] = -INFINITY;
-            }
+            for (int x = 0; x < 2; x++)
+              if (gone || !visible(p, k0 + kk, pos[ng][x])) s[ng][2 * e + x] = -INFINITY;
+        }
       }
-      float top[MG][2];
+      float top[NG][2];
       bool grow = false;
 #pragma unroll
-      for (int mg = 0; mg < MG; mg++)
+      for (int ng = 0; ng < NG; ng++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          float m = fmaxf(fmaxf(s[mg][0][2 * e], s[mg][0][2 * e + 1]), fmaxf(s[mg][1][2 * e], s[mg][1][2 * e + 1]));
-          m = fmaxf(m, __shfl_xor_sync(~0u, m, 1));
-          m = fmaxf(m, __shfl_xor_sync(~0u, m, 2));
-          top[mg][e] = m * sc[mg][e];
-          grow |= top[mg][e] > base[mg][e] + 8.0f;          // also a row's first key
+        for (int x = 0; x < 2; x++) {
+          float m = fmaxf(s[ng][x], s[ng][2 + x]);
+          m = fmaxf(m, __shfl_xor_sync(~0u, m, 4));
+          m = fmaxf(m, __shfl_xor_sync(~0u, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(~0u, m, 16));
+          top[ng][x] = m * sc[ng][x];
+          grow |= top[ng][x] > base[ng][x] + 8.0f;          // also a row's first key
         }
       if (__any_sync(~0u, grow)) {
 #pragma unroll
-        for (int mg = 0; mg < MG; mg++)
+        for (int ng = 0; ng < NG; ng++)
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const float nb = fmaxf(base[mg][e], top[mg][e]);
-            const float f = base[mg][e] == -INFINITY ? 0.0f : ex2(base[mg][e] - nb);
-            base[mg][e] = nb;
-            sum[mg][e] *= f;
+          for (int x = 0; x < 2; x++) {
+            const float nb = fmaxf(base[ng][x], top[ng][x]);
+            const float f = base[ng][x] == -INFINITY ? 0.0f : ex2(base[ng][x] - nb);
+            base[ng][x] = nb;
+            sum[ng][x] *= f;
 #pragma unroll
-            for (int j = 0; j < DP / 8; j++) o[mg][j][2 * e] *= f, o[mg][j][2 * e + 1] *= f;
+            for (int j = 0; j < DP / 16; j++) o[ng][j][x] *= f, o[ng][j][2 + x] *= f;
           }
       }
-      uint32_t a[MG][4];
+      uint32_t pb[NG][2];                                   // the weights as the second product's B
 #pragma unroll
-      for (int mg = 0; mg < MG; mg++) {
-        const float o0 = C::SHIFT - (base[mg][0] == -INFINITY ? 0.0f : base[mg][0]);
-        const float o1 = C::SHIFT - (base[mg][1] == -INFINITY ? 0.0f : base[mg][1]);
+      for (int ng = 0; ng < NG; ng++) {
+        const float o0 = C::SHIFT - (base[ng][0] == -INFINITY ? 0.0f : base[ng][0]);
+        const float o1 = C::SHIFT - (base[ng][1] == -INFINITY ? 0.0f : base[ng][1]);
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++) {
-          const float e0 = ex2(fmaf(s[mg][nt][0], sc[mg][0], o0)), e1 = ex2(fmaf(s[mg][nt][1], sc[mg][0], o0));
-          const float e2 = ex2(fmaf(s[mg][nt][2], sc[mg][1], o1)), e3 = ex2(fmaf(s[mg][nt][3], sc[mg][1], o1));
-          sum[mg][0] += e0 + e1;
-          sum[mg][1] += e2 + e3;
-          a[mg][2 * nt] = pack2<C::MF16>(e0, e1);
-          a[mg][2 * nt + 1] = pack2<C::MF16>(e2, e3);
+        for (int e = 0; e < 2; e++) {
+          const float e0 = ex2(fmaf(s[ng][2 * e], sc[ng][0], o0)), e1 = ex2(fmaf(s[ng][2 * e + 1], sc[ng][1], o1));
+          sum[ng][0] += e0;
+          sum[ng][1] += e1;
+          const uint32_t w = pack2<C::MF16>(e0, e1);
+          asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(pb[ng][e]) : "r"(w));
         }
       }
-      const int key = (((lane >> 3) & 1) << 3) + (lane & 7);
       if constexpr (C::FP8) {
+        const int key = (((lane >> 3) & 1) << 3) + (lane & 7);
 #pragma unroll
         for (int cp = 0; cp < DP / 32; cp++) {
           uint32_t w[4];
           ldsm4t(vt + unit_at<C::ROWB, false>(key, cp * 2 + (lane >> 4)), w);
 #pragma unroll
-          for (int e = 0; e < 2; e++) {                     // unit cp * 2 + e: its even dims, then its odd dims
+          for (int e = 0; e < 2; e++) {                     // unit cp * 2 + e: rows g its even dims, rows g + 8 its odd dims
             uint32_t x, y;
             asm("prmt.b32 %0, %1, 0, 0x3120;" : "=r"(x) : "r"(w[2 * e]));
             asm("prmt.b32 %0, %1, 0, 0x3120;" : "=r"(y) : "r"(w[2 * e + 1]));
-            const uint32_t x0 = fp8x2_to_f16x2<KV>(x & 0xFFFFu), y0 = fp8x2_to_f16x2<KV>(y & 0xFFFFu);
-            const uint32_t x1 = fp8x2_to_f16x2<KV>(x >> 16), y1 = fp8x2_to_f16x2<KV>(y >> 16);
+            const uint32_t a[4] = {fp8x2_to_f16x2<KV>(x & 0xFFFFu), fp8x2_to_f16x2<KV>(x >> 16), fp8x2_to_f16x2<KV>(y & 0xFFFFu),
+                                   fp8x2_to_f16x2<KV>(y >> 16)};
 #pragma unroll
-            for (int mg = 0; mg < MG; mg++) {
-              mma<true>(o[mg][cp * 4 + e * 2], a[mg], x0, y0);
-              mma<true>(o[mg][cp * 4 + e * 2 + 1], a[mg], x1, y1);
-            }
+            for (int ng = 0; ng < NG; ng++) mma<true>(o[ng][cp * 2 + e], a, pb[ng][0], pb[ng][1]);
           }
         }
       } else {
 #pragma unroll
         for (int dp = 0; dp < DP / 16; dp++) {
-          uint32_t b[4];
-          ldsm4t(vt + unit_at<C::ROWB, false>(key, dp * 2 + (lane >> 4)), b);
+          uint32_t a[4];
+          ldsm4t(vt + unit_at<C::ROWB, false>(((lane >> 4) << 3) + (lane & 7), dp * 2 + ((lane >> 3) & 1)), a);
 #pragma unroll
-          for (int mg = 0; mg < MG; mg++) {
-            mma<C::MF16>(o[mg][2 * dp], a[mg], b[0], b[1]);
-            mma<C::MF16>(o[mg][2 * dp + 1], a[mg], b[2], b[3]);
-          }
+          for (int ng = 0; ng < NG; ng++) mma<C::MF16>(o[ng][dp], a, pb[ng][0], pb[ng][1]);
         }
       }
     }
@@ -549,18 +547,18 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged
     // ---- the segment's end: the warps' results, a row group at a time, through the drained rings
     bool odd = false;                                       // infinities or NaN: see careful_row
 #pragma unroll
-    for (int mg = 0; mg < MG; mg++) {
+    for (int ng = 0; ng < NG; ng++) {
 #pragma unroll
-      for (int j = 0; j < DP / 8; j++)
+      for (int j = 0; j < DP / 16; j++)
 #pragma unroll
-        for (int x = 0; x < 4; x++) odd |= !(fabsf(o[mg][j][x]) < INFINITY);
+        for (int x = 0; x < 4; x++) odd |= !(fabsf(o[ng][j][x]) < INFINITY);
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
-        sum[mg][e] += __shfl_xor_sync(~0u, sum[mg][e], 1);
-        sum[mg][e] += __shfl_xor_sync(~0u, sum[mg][e], 2);
-        if (tg == 0) {
-          s_base[warp * C::MR + mg * 16 + g + 8 * e] = base[mg][e] - C::SHIFT;
-          s_sum[warp * C::MR + mg * 16 + g + 8 * e] = sum[mg][e];
+      for (int x = 0; x < 2; x++) {
+#pragma unroll
+        for (int d = 4; d <= 16; d <<= 1) sum[ng][x] += __shfl_xor_sync(~0u, sum[ng][x], d);
+        if (g == 0) {
+          s_base[warp * C::MR + ng * 8 + 2 * tg + x] = base[ng][x] - C::SHIFT;
+          s_sum[warp * C::MR + ng * 8 + 2 * tg + x] = sum[ng][x];
         }
       }
     }
@@ -570,29 +568,31 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged
     float *part = p.part + (c * 2 + (begins ? 1 : 0)) * (int64_t)(C::MR * (DP + 2));
     if (tid == 0 && begins && !ends)
       p.desc[c] = PartDesc{rows, row0, h, sh.block_of(seg_start + tiles_n - 1), rq.start};
-    float *s_o = reinterpret_cast<float *>(smem);           // [4 warps][16 rows][DP]
+    float *s_o = reinterpret_cast<float *>(smem);           // [4 warps][16 rows][SO]
 #pragma unroll
-    for (int mg = 0; mg < MG; mg++) {
+    for (int mg = 0; mg < (NG + 1) / 2; mg++) {
       if (mg * 16 < rows) {
         if (mg) __syncthreads();
         if (!careful) {
-          float *x0 = s_o + (warp * 16 + g) * DP, *x1 = x0 + 8 * DP;
-          if constexpr (C::FP8) {
 #pragma unroll
-            for (int k = 0; k < DP / 16; k++) {
-              const float(&e)[4] = o[mg][2 * k], (&f)[4] = o[mg][2 * k + 1];
-              *reinterpret_cast<float4 *>(x0 + k * 16 + tg * 4) = make_float4(e[0], f[0], e[1], f[1]);
-              *reinterpret_cast<float4 *>(x1 + k * 16 + tg * 4) = make_float4(e[2], f[2], e[3], f[3]);
-            }
-          } else {
+          for (int half = 0; half < (NG > 1 ? 2 : 1); half++) {
+            const int ng = mg * 2 + half;
+            if (ng >= NG) continue;
+            float *x0 = s_o + (warp * 16 + half * 8 + 2 * tg) * C::SO, *x1 = x0 + C::SO;
 #pragma unroll
-            for (int j = 0; j < DP / 8; j++) {
-              *reinterpret_cast<float2 *>(x0 + j * 8 + tg * 2) = make_float2(o[mg][j][0], o[mg][j][1]);
-              *reinterpret_cast<float2 *>(x1 + j * 8 + tg * 2) = make_float2(o[mg][j][2], o[mg][j][3]);
+            for (int j = 0; j < DP / 16; j++) {
+              const float(&v)[4] = o[ng][j];
+              if constexpr (C::FP8) {
+                *reinterpret_cast<float2 *>(x0 + j * 16 + 2 * g) = make_float2(v[0], v[2]);
+                *reinterpret_cast<float2 *>(x1 + j * 16 + 2 * g) = make_float2(v[1], v[3]);
+              } else {
+                x0[j * 16 + g] = v[0], x0[j * 16 + g + 8] = v[2];
+                x1[j * 16 + g] = v[1], x1[j * 16 + g + 8] = v[3];
+              }
             }
           }
         } else {
-          for (int row = warp; row < 16; row += 4) {
+          for (int row = warp; row < min(16, C::MR); row += 4) {
             const bool there = mg * 16 + row < rows;
             float m = -INFINITY, l = 0.0f, ov[DP / 32];
 #pragma unroll
@@ -603,7 +603,7 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged
             }
             for (int w = 0; w < 4; w++) {
 #pragma unroll
-              for (int k = 0; k < DP / 32; k++) s_o[(w * 16 + row) * DP + lane + 32 * k] = w == 0 ? ov[k] : 0.0f;
+              for (int k = 0; k < DP / 32; k++) s_o[(w * 16 + row) * C::SO + lane + 32 * k] = w == 0 ? ov[k] : 0.0f;
               if (lane == 0) {
                 s_base[w * C::MR + mg * 16 + row] = w == 0 ? m : -INFINITY;
                 s_sum[w * C::MR + mg * 16 + row] = w == 0 ? l : 0.0f;
@@ -621,7 +621,7 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, MG>::PER_SM)) paged
 #pragma unroll
           for (int w = 0; w < 4; w++) {
             const float f = ex2(s_base[w * C::MR + at] - ref);
-            const float4 v = *reinterpret_cast<const float4 *>(s_o + (w * 16 + row) * DP + d4);
+            const float4 v = *reinterpret_cast<const float4 *>(s_o + (w * 16 + row) * C::SO + d4);
             l += f * s_sum[w * C::MR + at];
             x[0] += f * v.x, x[1] += f * v.y, x[2] += f * v.z, x[3] += f * v.w;
           }
@@ -1113,10 +1113,10 @@ struct Variant {
   void (*merge)(AttnParams);
   int smem, per_sm, rows;
 };
-template <bool F16, int KV, int DP, int MG>
+template <bool F16, int KV, int DP, int NG>
 Variant few() {
-  using C = Few<F16, KV, DP, MG>;
-  return {paged_few_kernel<F16, KV, DP, MG>, paged_merge_kernel<F16, DP, C::MR>, C::SMEM, C::PER_SM, C::MR};
+  using C = Few<F16, KV, DP, NG>;
+  return {paged_few_kernel<F16, KV, DP, NG>, paged_merge_kernel<F16, DP, C::MR>, C::SMEM, C::PER_SM, C::MR};
 }
 template <bool F16, int KV, int DP>
 Variant many() {
@@ -1125,9 +1125,19 @@ Variant many() {
 // `rows`: query rows of the longest request (a request with more is served in several row tiles).
 template <bool F16, int KV>
 Variant pick(int dp, int64_t rows) {
-  if (dp == 64) return rows <= 16 ? few<F16, KV, 64, 1>() : rows <= 32 ? few<F16, KV, 64, 2>() : rows <= 64 ? few<F16, KV, 64, 4>() : many<F16, KV, 64>();
-  if (dp == 128) return rows <= 16 ? few<F16, KV, 128, 1>() : rows <= 32 ? few<F16, KV, 128, 2>() : many<F16, KV, 128>();
-  return rows <= 16 ? few<F16, KV, 256, 1>() : many<F16, KV, 256>();
+  if (dp == 64)
+    return rows <= 8    ? few<F16, KV, 64, 1>()
+           : rows <= 16 ? few<F16, KV, 64, 2>()
+           : rows <= 32 ? few<F16, KV, 64, 4>()
+           : rows <= 48 ? few<F16, KV, 64, 6>()
+           : rows <= 64 ? few<F16, KV, 64, 8>()
+                        : many<F16, KV, 64>();
+  if (dp == 128)
+    return rows <= 8    ? few<F16, KV, 128, 1>()
+           : rows <= 16 ? few<F16, KV, 128, 2>()
+           : rows <= 32 ? few<F16, KV, 128, 4>()
+                        : many<F16, KV, 128>();
+  return rows <= 8 ? few<F16, KV, 256, 1>() : rows <= 16 ? few<F16, KV, 256, 2>() : many<F16, KV, 256>();
 }
 Variant variant_for(bool f16, int cache_dtype, int dp, int64_t rows) {
   if (cache_dtype == FP8B200_E4M3) return f16 ? pick<true, FP8B200_E4M3>(dp, rows) : pick<false, FP8B200_E4M3>(dp, rows);
@@ -1252,7 +1262,7 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
   const int grid = current_sm_count() * v.per_sm;
   launch_dependent(v.main, dim3((unsigned)grid), THREADS, v.smem, (cudaStream_t)stream, p);
   p.blocks = grid;
-  launch_dependent(v.merge, dim3((unsigned)current_sm_count(), (unsigned)(v.rows / 16)), MERGE_THREADS, 0, (cudaStream_t)stream, p);
+  launch_dependent(v.merge, dim3((unsigned)current_sm_count(), (unsigned)std::max(1, v.rows / 16)), MERGE_THREADS, 0, (cudaStream_t)stream, p);
   count_launch(2);
   return check_launch("paged_attention");
 }
