@@ -1259,6 +1259,7 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
   }
   const Variant v = variant_for(f16, cache_dtype, dp, std::min<int64_t>(most, p.rows_upto));
   if (int rc = launch_attributes((const void *)v.main, v.smem)) return rc;
+  if (int rc = launch_attributes((const void *)v.merge, 0)) return rc;
   const int grid = current_sm_count() * v.per_sm;
   launch_dependent(v.main, dim3((unsigned)grid), THREADS, v.smem, (cudaStream_t)stream, p);
   p.blocks = grid;

@@ -1074,6 +1074,7 @@ int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int s
     if (r != CUDA_SUCCESS) return set_error(FP8B200_ELAUNCH, "paged_attention: tensor map encode failed (%d)", (int)r);
   }
   if (int rc = launch_attributes((const void *)v.main, v.smem)) return rc;
+  if (int rc = launch_attributes((const void *)v.merge, 0)) return rc;
   launch_dependent(v.main, dim3((unsigned)sms), v.threads, v.smem, st, p, maps, box_log);
   launch_dependent(v.merge, dim3((unsigned)sms, 8), MERGE_THREADS, 0, st, p);
   count_launch(2);
