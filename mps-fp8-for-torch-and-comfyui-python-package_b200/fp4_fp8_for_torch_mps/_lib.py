@@ -124,3 +124,13 @@ def gemm_status(reset: bool = False) -> int:
     if rc not in (0, ETIMEOUT):
         check(rc, "gemm status")
     return int(v.value)
+
+
+def paged_status(reset: bool = False) -> int:
+    """Device status word of the paged attention kernels' bounded waits on the
+    current device (0 = ok). Synchronises the device."""
+    v = ctypes.c_uint32(0)
+    rc = lib().fp8b200_paged_status(ctypes.byref(v), 1 if reset else 0)
+    if rc not in (0, ETIMEOUT):
+        check(rc, "paged status")
+    return int(v.value)

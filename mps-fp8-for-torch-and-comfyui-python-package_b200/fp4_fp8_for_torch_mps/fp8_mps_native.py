@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib as L
-from .paged import PagedStep, paged_attention, paged_slots, rope_write_paged  # noqa: F401
+from .paged import PagedKVCache, PagedStep, paged_attention, paged_slots, rope_write_paged  # noqa: F401
 
 _FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
 _FLOAT = (torch.float32, torch.bfloat16, torch.float16)

@@ -265,3 +265,57 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             ks, ks_step, vs, vs_step, window, sinks, max_new or 0, out.data_ptr(), o_tok, o_head, 1 if new_out else 0,
             ws.data_ptr(), size)
     return out
+
+
+class PagedKVCache:
+    """The pool of pages of a model's layers and the bookkeeping of a batch of
+    requests over it, all on the device.
+
+        cache = PagedKVCache(layers, pages, page_size, kv_heads, head_dim, requests, max_len, dtype, device)
+        step = cache.step(new_lens, num_tokens)          # once a step
+        k, v = cache.k[layer], cache.v[layer]            # for rope_write_paged and paged_attention
+
+    `dtype`: the activations' type or a float8 type; k_scale, v_scale: float8
+    caches' scales, one value or one per head (None: 1). All layers share the
+    pages' numbering. Slots hold nothing until they are written; the operators
+    never read such a slot. `step` only launches kernels, so it can be part of
+    a captured step."""
+
+    def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, requests: int, max_len: int,
+                 dtype: torch.dtype, device, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None):
+        if dtype not in _FP8 + _16BIT:
+            raise RuntimeError(f"PagedKVCache: dtype must be bfloat16, float16 or a float8 type, got {dtype}")
+        if min(layers, pages, page_size, kv_heads, head_dim, requests, max_len) < 1 or requests > MAX_REQUESTS:
+            raise RuntimeError(f"PagedKVCache: sizes must be positive, and at most {MAX_REQUESTS} requests")
+        self.page_size = page_size
+        pool = torch.empty(layers, 2, pages, page_size, kv_heads, head_dim, dtype=dtype, device=device)
+        self.k = [pool[i, 0] for i in range(layers)]
+        self.v = [pool[i, 1] for i in range(layers)]
+        self.k_scale, self.v_scale = k_scale, v_scale
+        self.block_table = torch.full((requests, -(-max_len // page_size)), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(requests, dtype=torch.int32, device=device)
+        self.free_pages = torch.arange(pages, dtype=torch.int32, device=device)
+        self.free_head = torch.zeros(1, dtype=torch.int32, device=device)
+
+    def step(self, new_lens: torch.Tensor, num_tokens: int) -> PagedStep:
+        """Pages and slots for new_lens (requests,) int32 more tokens; the lengths
+        move on. See paged_slots, also for a pool that runs short."""
+        s = paged_slots(self.lens, new_lens, self.block_table, self.free_pages, self.page_size, num_tokens, self.free_head)
+        self.lens.copy_(s.kv_lens)
+        self.free_head.copy_(s.free_head)
+        return s
+
+    def release(self, request: int) -> None:
+        """Ends a request: its pages are free again, its row starts anew. Waits
+        for the device."""
+        total = self.free_pages.numel()
+        head = min(int(self.free_head), total)
+        row = self.block_table[request]
+        ids = row[row >= 0]
+        n = ids.numel()
+        if n > head:
+            raise RuntimeError(f"PagedKVCache: request {request} holds {n} pages, {head} are taken")
+        self.free_pages[head - n:] = torch.cat([self.free_pages[head:], ids])
+        self.free_head.fill_(head - n)
+        row.fill_(-1)
+        self.lens[request] = 0

@@ -118,7 +118,8 @@ def fp4_gemm_operands(m: int, n: int, k: int, seed: int = 0):
 # scale, broadcast per output column) and per-token e4m3 activations; the
 # MLP's SiLU(g) * u is fused with its per-token quantisation and the rotary
 # embedding is one kernel (both bit-identical to the PyTorch expressions);
-# norms and attention (SDPA) stay in bf16 PyTorch.
+# norms and attention (SDPA) stay in bf16 PyTorch. `forward_paged` is the serving
+# form: prompts and decoded tokens of a batch of requests over a paged cache.
 
 LLAMA = dict(hidden=4096, intermediate=14336, heads=32, kv_heads=8, head_dim=128, layers=32,
              rope_theta=500000.0, eps=1e-5)
@@ -188,7 +189,27 @@ class Fp8LlamaLayer:
             q, k = _rope(q.view(batch, seq, nh, hd), cos, sin), _rope(k.view(batch, seq, nkv, hd), cos, sin)
         a = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2),
                                            is_causal=True, enable_gqa=True)
-        a = a.transpose(1, 2).reshape(t, h)
+        return self.after_attention(x, a.transpose(1, 2).reshape(t, h))
+
+    def forward_paged(self, x, cos, sin, step, cache, index, max_new=None, window=0, sinks=0):
+        """The layer over a paged cache: x holds the rows of a step of
+        `cache` (PagedKVCache.step), this layer is the cache's layer `index`;
+        cos, sin: float32 tables (paged_rope_tables). Attention and rotary
+        embedding are the package's operators."""
+        import torch.nn.functional as F
+        c = self.cfg
+        r = F.rms_norm(x, (c["hidden"],), self.n1, c["eps"])
+        qkv = self.linear(r, self.w_qkv, self.s_qkv)
+        k, v = cache.k[index], cache.v[index]
+        q = self.nat.rope_write_paged(qkv, cos, sin, step.positions, step.slots, k, v, c["heads"], cache.k_scale, cache.v_scale)
+        a = self.nat.paged_attention(q, k, v, cache.block_table, step.cu_new, step.kv_lens, window=window, sinks=sinks,
+                                     k_scale=cache.k_scale, v_scale=cache.v_scale, max_new=max_new)
+        return self.after_attention(x, a.view(x.shape[0], -1))
+
+    def after_attention(self, x, a):
+        import torch.nn.functional as F
+        c = self.cfg
+        h = c["hidden"]
         x = x + self.linear(a, self.w_o, self.s_o)
         r = F.rms_norm(x, (h,), self.n2, c["eps"])
         gu = self.linear(r, self.w_gu, self.s_gu)
@@ -220,6 +241,15 @@ def rope_tables(seq: int, device, cfg=LLAMA):
     return cos, sin
 
 
+def paged_rope_tables(positions: int, device, cfg=LLAMA):
+    """(positions, head_dim / 2) float32 cos and sin; the angles in float64, so
+    that far positions keep theirs."""
+    hd = cfg["head_dim"]
+    inv = cfg["rope_theta"] ** (-torch.arange(0, hd, 2, device=device, dtype=torch.float64) / hd)
+    ang = torch.arange(positions, device=device, dtype=torch.float64)[:, None] * inv[None, :]
+    return ang.cos().float(), ang.sin().float()
+
+
 class Fp8LlamaStack:
     """`layers` decoder layers over a batch of `batch` x `seq` tokens."""
 
@@ -232,6 +262,24 @@ class Fp8LlamaStack:
         cos, sin = rope_tables(seq, x.device)
         for layer in self.layers:
             x = layer.forward(x, cos, sin, batch, seq)
+        return x
+
+    def paged_cache(self, requests: int, max_len: int, pages: int, page_size: int = 64, dtype=torch.float8_e4m3fn,
+                    k_scale=None, v_scale=None):
+        """A paged cache for this stack's layers."""
+        from .paged import PagedKVCache
+        c = self.layers[0].cfg
+        return PagedKVCache(len(self.layers), pages, page_size, c["kv_heads"], c["head_dim"], requests, max_len, dtype,
+                            self.device, k_scale, v_scale)
+
+    def forward_paged(self, x, cache, new_lens, cos, sin, max_new=None, window=0, sinks=0):
+        """One step of a batch of requests: x (tokens, hidden) holds new_lens[r]
+        rows of each request r in order (rows behind them are padding), prompts
+        and decoded tokens alike. Only kernels are launched: a step can be
+        captured and replayed."""
+        step = cache.step(new_lens, x.shape[0])
+        for i, layer in enumerate(self.layers):
+            x = layer.forward_paged(x, cos, sin, step, cache, i, max_new, window, sinks)
         return x
 
     def gemm_flops(self, tokens: int) -> float:

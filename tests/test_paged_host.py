@@ -194,3 +194,26 @@ def test_fakes():
     q = torch.ops.fp8_mps.rope_write_paged(**m(write_args()))
     assert q.shape == (3, 4, 64) and q.dtype == BF16
     assert torch.ops.fp8_mps.paged_attention(**m(attention_args())).shape == (3, 4, 64)
+
+
+def test_cache_release_on_the_host():
+    """Which pages are free after requests end, in any order, and the refusals."""
+    from fp4_fp8_for_torch_mps import paged
+    c = paged.PagedKVCache(2, 6, 4, 1, 16, 3, 16, E4M3, "cpu")
+    assert len(c.k) == 2 and c.k[0].shape == (6, 4, 1, 16) and c.k[1].stride() == c.v[1].stride()
+    c.block_table[0, :2], c.block_table[2, :3] = i32(0, 1), i32(2, 3, 4)     # as two prompts would leave it
+    c.free_head.fill_(5)
+    c.lens.copy_(i32(7, 0, 12))
+    c.release(0)
+    assert c.free_pages[3:].tolist() == [5, 0, 1] and int(c.free_head) == 3 and c.lens.tolist() == [0, 0, 12]
+    c.release(1)                                                             # holds nothing
+    c.release(2)
+    assert sorted(c.free_pages.tolist()) == list(range(6)) and int(c.free_head) == 0
+    assert int((c.block_table >= 0).sum()) == 0
+    c.block_table[1, 0] = 3
+    with pytest.raises(RuntimeError, match="0 are taken"):
+        c.release(1)
+    for bad in (dict(layers=0), dict(requests=16385), dict(dtype=torch.float32)):
+        a = dict(layers=1, pages=2, page_size=4, kv_heads=1, head_dim=16, requests=1, max_len=4, dtype=BF16, device="cpu")
+        with pytest.raises(RuntimeError, match="PagedKVCache"):
+            paged.PagedKVCache(**{**a, **bad})
