@@ -157,9 +157,14 @@ __global__ void __launch_bounds__(SL_THREADS) slots_kernel(const SlotsParams p) 
 // saturates at the format's largest finite value, so one outlier cannot put
 // a NaN where every later query reads it. NaN stays NaN.
 // A thread takes 8 + 8 values (a 16-byte unit of each half) of up to HG heads
-// of one token, so the units' cos / sin are read once for HG heads. HBM bound.
-constexpr int RW_THREADS = 256;
-constexpr int HG = 4;
+// of one token, so the units' cos / sin are read once for HG heads. HBM bound:
+// 16384 tokens of 32 / 8 / 8 heads of 128, 16-bit cache, in 66.6 us (6.06 TB/s)
+// with HG = 4 and 69.2 us with 2. With few tokens the loads' latency counts,
+// and more threads hide it: 16 tokens into e4m3 in 3.0 us with HG = 2 and 4.7
+// with 4, 5001 tokens of 16 / 2 / 2 heads of 64 into e5m2 in 8.7 and 10.8 us (in
+// a graph). So HG = 4 where that fills the GPU (RW_FULL blocks an SM) and else 2.
+constexpr int RW_THREADS = 128;
+constexpr int RW_FULL = 16;
 
 struct WriteParams {
   const uint16_t *qkv;
@@ -238,8 +243,8 @@ __device__ __forceinline__ void store8(void *cache, int64_t off, float (&f)[8], 
 }
 
 // CACHE: E4M3, E5M2, or anything else for qkv's own type.
-template <bool F16, int CACHE>
-__global__ void __launch_bounds__(RW_THREADS) rope_write_kernel(const WriteParams p) {
+template <bool F16, int CACHE, int HG>
+__global__ void __launch_bounds__(RW_THREADS, HG == 4 ? 5 : 6) rope_write_kernel(const WriteParams p) {
   launch_dependents();
   wait_prior();
   const int half = p.hd / 2, units = half / 8;
@@ -312,6 +317,11 @@ __global__ void __launch_bounds__(RW_THREADS) rope_write_kernel(const WriteParam
       }
     }
   }
+}
+
+template <bool F16, int CACHE>
+auto rope_write(bool full) {
+  return full ? rope_write_kernel<F16, CACHE, 4> : rope_write_kernel<F16, CACHE, 2>;
 }
 
 template <typename P>
@@ -411,16 +421,14 @@ extern "C" int fp8b200_rope_write_paged(const void *qkv, int dtype, int64_t toke
                 positions, slots, (uint16_t *)q_out, k_cache, v_cache, pages, stride_page, stride_slot, stride_head,
                 (int)page_size, fp8 ? k_scale : nullptr, fp8 ? v_scale : nullptr, k_scale_step, v_scale_step};
   const int64_t heads = (int64_t)n_q_heads + 2 * n_kv_heads;
-  const int64_t work = tokens * ((heads + HG - 1) / HG) * (head_dim / 16);
-  const int grid = grid_for(work, RW_THREADS, 8);
-  void (*kernel)(WriteParams);
+  const int64_t work4 = tokens * ((heads + 3) / 4) * (head_dim / 16), work2 = tokens * ((heads + 1) / 2) * (head_dim / 16);
+  const bool full = work4 >= (int64_t)RW_THREADS * RW_FULL * current_sm_count();
+  const int grid = grid_for(full ? work4 : work2, RW_THREADS, RW_FULL);
   const bool f16 = dtype == FP8B200_F16;
-  if (cache_dtype == FP8B200_E4M3)
-    kernel = f16 ? rope_write_kernel<true, FP8B200_E4M3> : rope_write_kernel<false, FP8B200_E4M3>;
-  else if (cache_dtype == FP8B200_E5M2)
-    kernel = f16 ? rope_write_kernel<true, FP8B200_E5M2> : rope_write_kernel<false, FP8B200_E5M2>;
-  else
-    kernel = f16 ? rope_write_kernel<true, FP8B200_F16> : rope_write_kernel<false, FP8B200_BF16>;
+  void (*kernel)(WriteParams);
+  if (cache_dtype == FP8B200_E4M3) kernel = f16 ? rope_write<true, FP8B200_E4M3>(full) : rope_write<false, FP8B200_E4M3>(full);
+  else if (cache_dtype == FP8B200_E5M2) kernel = f16 ? rope_write<true, FP8B200_E5M2>(full) : rope_write<false, FP8B200_E5M2>(full);
+  else kernel = f16 ? rope_write<true, FP8B200_F16>(full) : rope_write<false, FP8B200_BF16>(full);
   launch_pdl(kernel, grid, RW_THREADS, 0, (cudaStream_t)stream, p);
   count_launch();
   return check_launch("rope_write_paged");

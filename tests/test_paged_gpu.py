@@ -176,7 +176,7 @@ def make_write(t, hq, hk, d, x, cache, page, seed, scales):
 
 @pytest.mark.parametrize("x,cache", [(BF16, BF16), (F16, F16), (BF16, E4M3), (F16, E4M3), (BF16, E5M2), (F16, E5M2)])
 @pytest.mark.parametrize("t,hq,hk,d,page,scales", [(1, 1, 1, 16, 1, 0), (7, 4, 2, 64, 16, 1), (33, 7, 1, 128, 24, 2),
-                                                   (129, 12, 12, 80, 64, 2), (5, 0, 3, 256, 16, 2), (1000, 32, 8, 128, 16, 2)])
+                                                   (129, 12, 12, 80, 64, 2), (5, 0, 3, 256, 16, 2), (1000, 32, 8, 128, 16, 2), (4100, 32, 8, 128, 64, 2)])
 def test_write(nat, x, cache, t, hq, hk, d, page, scales):
     """Every value of q and of both caches, the slots no token has included."""
     qkv, cos, sin, pos, slots, k, v, ks, vs = make_write(t, hq, hk, d, x, cache, page, t + d, scales)
