@@ -40,6 +40,9 @@ class PagedStep(NamedTuple):
 _workspace_bytes: dict[tuple[int, int, int], int] = {}
 
 
+# A call's arguments are looked over in one expression (every attribute of a
+# tensor costs 0.1 us and a call of a helper more: a small step is bound by
+# them); only what does not pass goes through the checks that say why.
 def _check(t: torch.Tensor, name: str, what: str, dtype: torch.dtype, dim: int, dev: torch.device) -> None:
     if t.dtype != dtype or t.dim() != dim:
         raise RuntimeError(f"{what}: {name} must be a {dim}-D {dtype} tensor, got {t.dim()}-D {t.dtype}")
@@ -88,16 +91,17 @@ def _check_scale(s: torch.Tensor | None, name: str, what: str, cache: torch.Tens
 
 def _launch(dev: torch.device, fn, what: str, *args) -> None:
     """fn(*args, current stream) on `dev`. The stream's handle comes without a
-    torch.cuda.Stream object, which takes 2 us: a fifth of a small call."""
+    torch.cuda.Stream object, which takes 2 us."""
+    index = dev.index
     if dev.type != "cuda":
         raise RuntimeError(f"{what}: tensors must be on a CUDA device, got {dev}")
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
         if rc:
             L.check(rc, what)
     else:
         with torch.cuda.device(dev):
-            L.check(fn(*args, torch._C._cuda_getCurrentRawStream(dev.index)), what)
+            L.check(fn(*args, torch._C._cuda_getCurrentRawStream(index)), what)
 
 
 def slots_outputs(requests: int, num_tokens: int, dev: torch.device) -> PagedStep:
@@ -105,6 +109,24 @@ def slots_outputs(requests: int, num_tokens: int, dev: torch.device) -> PagedSte
     cu, kv, pos, head = torch.empty(2 * requests + 2 + num_tokens, dtype=torch.int32, device=dev).split_with_sizes(
         [requests + 1, requests, num_tokens, 1])
     return PagedStep(cu, kv, pos, torch.empty(num_tokens, dtype=torch.int64, device=dev), head)
+
+
+def _check_slots(cached_lens, new_lens, block_table, free_pages, page_size, num_tokens, free_head) -> None:
+    what = "paged_slots"
+    dev = cached_lens.device
+    _check(cached_lens, "cached_lens", what, torch.int32, 1, dev)
+    _check(new_lens, "new_lens", what, torch.int32, 1, dev)
+    _check(free_pages, "free_pages", what, torch.int32, 1, dev)
+    _check_table(block_table, what, dev)
+    n = cached_lens.numel()
+    if new_lens.numel() != n or block_table.shape[0] != n:
+        raise RuntimeError(f"{what}: {n} cached_lens, {new_lens.numel()} new_lens and {block_table.shape[0]} block_table rows")
+    if n > MAX_REQUESTS:
+        raise RuntimeError(f"{what}: {n} requests, at most {MAX_REQUESTS}")
+    if page_size < 1 or num_tokens < 0:
+        raise RuntimeError(f"{what}: page_size={page_size} must be positive and num_tokens={num_tokens} not negative")
+    if free_head is not None and (free_head.dtype != torch.int32 or free_head.numel() != 1 or free_head.device != dev):
+        raise RuntimeError(f"{what}: free_head must be one int32 value on {dev}")
 
 
 def paged_slots(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
@@ -127,27 +149,46 @@ def paged_slots(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: 
     them); the returned free_head is then beyond free_pages.numel(). A token
     beyond the table's columns also gets slot -1. Lengths below zero count as
     zero; sums of lengths stay below 2^31."""
-    what = "paged_slots"
     dev = cached_lens.device
-    _check(cached_lens, "cached_lens", what, torch.int32, 1, dev)
-    _check(new_lens, "new_lens", what, torch.int32, 1, dev)
-    _check(free_pages, "free_pages", what, torch.int32, 1, dev)
-    ld = _check_table(block_table, what, dev)
     n = cached_lens.numel()
-    if new_lens.numel() != n or block_table.shape[0] != n:
-        raise RuntimeError(f"{what}: {n} cached_lens, {new_lens.numel()} new_lens and {block_table.shape[0]} block_table rows")
-    if n > MAX_REQUESTS:
-        raise RuntimeError(f"{what}: {n} requests, at most {MAX_REQUESTS}")
-    if page_size < 1 or num_tokens < 0:
-        raise RuntimeError(f"{what}: page_size={page_size} must be positive and num_tokens={num_tokens} not negative")
-    if free_head is not None and (free_head.dtype != torch.int32 or free_head.numel() != 1 or free_head.device != dev):
-        raise RuntimeError(f"{what}: free_head must be one int32 value on {dev}")
+    rows, cols = block_table.shape if block_table.dim() == 2 else (-1, 0)
+    ld = block_table.stride(0) if n > 1 and rows == n else cols
+    if not (cached_lens.dtype is new_lens.dtype is block_table.dtype is free_pages.dtype is torch.int32
+            and cached_lens.dim() == new_lens.dim() == free_pages.dim() == 1 and new_lens.numel() == n == rows
+            and cached_lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous()
+            and (cols <= 1 or block_table.stride(1) == 1) and ld >= cols and n <= MAX_REQUESTS
+            and new_lens.device == block_table.device == free_pages.device == dev and page_size >= 1 and num_tokens >= 0
+            and (free_head is None
+                 or (free_head.dtype is torch.int32 and free_head.numel() == 1 and free_head.device == dev))):
+        _check_slots(cached_lens, new_lens, block_table, free_pages, page_size, num_tokens, free_head)
     step = outputs(n, num_tokens, dev)
-    _launch(dev, L.lib().fp8b200_paged_slots, what, cached_lens.data_ptr(), new_lens.data_ptr(), n,
+    _launch(dev, L.lib().fp8b200_paged_slots, "paged_slots", cached_lens.data_ptr(), new_lens.data_ptr(), n,
             block_table.data_ptr(), ld, block_table.shape[1], free_pages.data_ptr(), free_pages.numel(),
             None if free_head is None else free_head.data_ptr(), page_size, num_tokens, step.cu_new.data_ptr(),
             step.kv_lens.data_ptr(), step.positions.data_ptr(), step.slots.data_ptr(), step.free_head.data_ptr())
     return step
+
+
+def _check_write(qkv, cos, sin, positions, slots, k_cache, v_cache, n_q_heads) -> None:
+    what = "rope_write_paged"
+    dev = qkv.device
+    _, _, hk, d = _check_caches(k_cache, v_cache, qkv, what)
+    width = (n_q_heads + 2 * hk) * d
+    if qkv.dim() != 2 or n_q_heads < 0 or qkv.shape[1] < width:
+        raise RuntimeError(f"{what}: qkv must be (tokens, at least {width}), got {tuple(qkv.shape)}")
+    t = qkv.shape[0]
+    ld = qkv.stride(0) if t > 1 else width
+    if (t and qkv.stride(1) != 1) or ld < width:
+        raise RuntimeError(f"{what}: qkv rows must be contiguous and not overlap, got strides {qkv.stride()}")
+    _check(cos, "cos", what, torch.float32, 2, dev)
+    _check(sin, "sin", what, torch.float32, 2, dev)
+    if cos.shape != sin.shape or cos.shape[1] * 2 != d or not cos.is_contiguous() or not sin.is_contiguous():
+        raise RuntimeError(f"{what}: cos and sin must be contiguous (positions, {d // 2}) tables, got {tuple(cos.shape)} and "
+                           f"{tuple(sin.shape)}")
+    _check(positions, "positions", what, torch.int32, 1, dev)
+    _check(slots, "slots", what, torch.int64, 1, dev)
+    if positions.numel() != t or slots.numel() != t:
+        raise RuntimeError(f"{what}: {t} rows, {positions.numel()} positions and {slots.numel()} slots")
 
 
 def rope_write_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
@@ -168,34 +209,49 @@ def rope_write_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, po
     value / scale (k_scale, v_scale: one float32 value or one per head; None:
     1), saturated at the format's largest finite value; NaN stays NaN.
     Returns q, (tokens, n_q_heads, head_dim)."""
-    what = "rope_write_paged"
-    dev = qkv.device
-    pages, page, hk, d = _check_caches(k_cache, v_cache, qkv, what)
+    dev, dt, cdt = qkv.device, qkv.dtype, k_cache.dtype
+    shape, strides, t = k_cache.shape, k_cache.stride(), positions.numel()
+    pages, page, hk, d = shape if len(shape) == 4 else (0, 0, 0, 0)
     width = (n_q_heads + 2 * hk) * d
-    if qkv.dim() != 2 or n_q_heads < 0 or qkv.shape[1] < width:
-        raise RuntimeError(f"{what}: qkv must be (tokens, at least {width}), got {tuple(qkv.shape)}")
-    t = qkv.shape[0]
-    ld = qkv.stride(0) if t > 1 else width
-    if (t and qkv.stride(1) != 1) or ld < width:
-        raise RuntimeError(f"{what}: qkv rows must be contiguous and not overlap, got strides {qkv.stride()}")
-    _check(cos, "cos", what, torch.float32, 2, dev)
-    _check(sin, "sin", what, torch.float32, 2, dev)
-    if cos.shape != sin.shape or cos.shape[1] * 2 != d or not cos.is_contiguous() or not sin.is_contiguous():
-        raise RuntimeError(f"{what}: cos and sin must be contiguous (positions, {d // 2}) tables, got {tuple(cos.shape)} and "
-                           f"{tuple(sin.shape)}")
-    _check(positions, "positions", what, torch.int32, 1, dev)
-    _check(slots, "slots", what, torch.int64, 1, dev)
-    if positions.numel() != t or slots.numel() != t:
-        raise RuntimeError(f"{what}: {t} rows, {positions.numel()} positions and {slots.numel()} slots")
-    ks, ks_step = _check_scale(k_scale, "k_scale", what, k_cache)
-    vs, vs_step = _check_scale(v_scale, "v_scale", what, v_cache)
-    q = torch.empty((t, n_q_heads, d), dtype=qkv.dtype, device=dev)
-    sp, ss, sh, _ = k_cache.stride()
-    _launch(dev, L.lib().fp8b200_rope_write_paged, what, qkv.data_ptr(), L.dtype_code(qkv.dtype), t, ld, n_q_heads, hk, d,
+    ld = qkv.stride(0) if t > 1 and qkv.dim() == 2 else width
+    if not (dt in _16BIT and (cdt is dt or cdt in _FP8) and v_cache.dtype is cdt and v_cache.shape == shape and len(shape) == 4
+            and v_cache.stride() == strides and strides[3] == 1 and qkv.shape == (t, qkv.shape[-1]) and qkv.shape[1] >= width
+            and ld >= width and n_q_heads >= 0 and (t == 0 or qkv.stride(1) == 1)
+            and cos.dtype is sin.dtype is torch.float32 and cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] * 2 == d
+            and cos.is_contiguous() and sin.is_contiguous() and positions.dtype is torch.int32 and positions.dim() == 1
+            and positions.is_contiguous() and slots.dtype is torch.int64 and slots.shape == (t,) and slots.is_contiguous()
+            and k_cache.device == v_cache.device == cos.device == sin.device == positions.device == slots.device == dev):
+        _check_write(qkv, cos, sin, positions, slots, k_cache, v_cache, n_q_heads)
+    ks, ks_step = (None, 0) if k_scale is None else _check_scale(k_scale, "k_scale", "rope_write_paged", k_cache)
+    vs, vs_step = (None, 0) if v_scale is None else _check_scale(v_scale, "v_scale", "rope_write_paged", v_cache)
+    q = qkv.new_empty((t, n_q_heads, d))
+    sp, ss, sh, _ = strides
+    _launch(dev, L.lib().fp8b200_rope_write_paged, "rope_write_paged", qkv.data_ptr(), L.dtype_code(dt), t, ld, n_q_heads, hk, d,
             cos.data_ptr(), sin.data_ptr(), cos.shape[0], positions.data_ptr(), slots.data_ptr(), q.data_ptr(),
-            k_cache.data_ptr(), v_cache.data_ptr(), L.dtype_code(k_cache.dtype), pages, page, sp, ss, sh, ks, ks_step, vs,
-            vs_step)
+            k_cache.data_ptr(), v_cache.data_ptr(), L.dtype_code(cdt), pages, page, sp, ss, sh, ks, ks_step, vs, vs_step)
     return q
+
+
+def _check_attention(q, k_cache, v_cache, block_table, cu_new, kv_lens, window, sinks, max_new) -> None:
+    what = "paged_attention"
+    dev = q.device
+    _, _, hk, d = _check_caches(k_cache, v_cache, q, what)
+    if q.dim() != 3 or q.shape[2] != d or (q.numel() and q.stride(2) != 1):
+        raise RuntimeError(f"{what}: q must be (tokens, q_heads, {d}) with contiguous heads, got {tuple(q.shape)}")
+    hq = q.shape[1]
+    if hq < 1 or hk < 1 or hq % hk:
+        raise RuntimeError(f"{what}: {hq} query heads over {hk} key/value heads")
+    _check_table(block_table, what, dev)
+    _check(cu_new, "cu_new", what, torch.int32, 1, dev)
+    _check(kv_lens, "kv_lens", what, torch.int32, 1, dev)
+    n = block_table.shape[0]
+    if cu_new.numel() != n + 1 or kv_lens.numel() != n:
+        raise RuntimeError(f"{what}: {n} block_table rows need {n + 1} cu_new and {n} kv_lens, got {cu_new.numel()} and "
+                           f"{kv_lens.numel()}")
+    if window < 0 or sinks < 0:
+        raise RuntimeError(f"{what}: window={window} and sinks={sinks} must not be negative")
+    if max_new is not None and max_new < 1:
+        raise RuntimeError(f"{what}: max_new={max_new} must be positive")
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -222,29 +278,25 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     were in a given `out` (of q's shape and type, any 16-byte aligned rows)
     and 0 in a new one."""
     what = "paged_attention"
-    dev = q.device
-    pages, page, hk, d = _check_caches(k_cache, v_cache, q, what)
-    if q.dim() != 3 or q.shape[2] != d or (q.numel() and q.stride(2) != 1):
-        raise RuntimeError(f"{what}: q must be (tokens, q_heads, {d}) with contiguous heads, got {tuple(q.shape)}")
-    t, hq, _ = q.shape
-    if hq < 1 or hk < 1 or hq % hk:
-        raise RuntimeError(f"{what}: {hq} query heads over {hk} key/value heads")
-    ld = _check_table(block_table, what, dev)
-    _check(cu_new, "cu_new", what, torch.int32, 1, dev)
-    _check(kv_lens, "kv_lens", what, torch.int32, 1, dev)
-    n, cols = block_table.shape
-    if cu_new.numel() != n + 1 or kv_lens.numel() != n:
-        raise RuntimeError(f"{what}: {n} block_table rows need {n + 1} cu_new and {n} kv_lens, got {cu_new.numel()} and "
-                           f"{kv_lens.numel()}")
-    if window < 0 or sinks < 0:
-        raise RuntimeError(f"{what}: window={window} and sinks={sinks} must not be negative")
-    if max_new is not None and max_new < 1:
-        raise RuntimeError(f"{what}: max_new={max_new} must be positive")
-    ks, ks_step = _check_scale(k_scale, "k_scale", what, k_cache)
-    vs, vs_step = _check_scale(v_scale, "v_scale", what, v_cache)
+    dev, dt, cdt = q.device, q.dtype, k_cache.dtype
+    shape, strides, qshape = k_cache.shape, k_cache.stride(), q.shape
+    pages, page, hk, d = shape if len(shape) == 4 else (0, 0, 0, 0)
+    t, hq, qd = qshape if len(qshape) == 3 else (0, 0, 0)
+    n, cols = block_table.shape if block_table.dim() == 2 else (0, 0)
+    ld = block_table.stride(0) if n > 1 else cols
+    if not (dt in _16BIT and (cdt is dt or cdt in _FP8) and v_cache.dtype is cdt and v_cache.shape == shape and len(shape) == 4
+            and v_cache.stride() == strides and strides[3] == 1 and len(qshape) == 3 and qd == d and q.stride(2) == 1
+            and hk >= 1 and hq >= 1 and hq % hk == 0 and block_table.dtype is cu_new.dtype is kv_lens.dtype is torch.int32
+            and block_table.dim() == 2 and (cols <= 1 or block_table.stride(1) == 1) and ld >= cols
+            and cu_new.shape == (n + 1,) and kv_lens.shape == (n,) and cu_new.is_contiguous() and kv_lens.is_contiguous()
+            and window >= 0 and sinks >= 0 and (max_new is None or max_new >= 1)
+            and k_cache.device == v_cache.device == block_table.device == cu_new.device == kv_lens.device == dev):
+        _check_attention(q, k_cache, v_cache, block_table, cu_new, kv_lens, window, sinks, max_new)
+    ks, ks_step = (None, 0) if k_scale is None else _check_scale(k_scale, "k_scale", what, k_cache)
+    vs, vs_step = (None, 0) if v_scale is None else _check_scale(v_scale, "v_scale", what, v_cache)
     new_out = out is None
     if new_out:
-        out = torch.empty((t, hq, d), dtype=q.dtype, device=dev)
+        out = q.new_empty(qshape)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or (out.numel() and out.stride(2) != 1):
         raise RuntimeError(f"{what}: `out` must be a {q.dtype} tensor of q's shape on {dev} with contiguous heads")
     max_rows = min(t if max_new is None else max_new, t) * (hq // hk)
@@ -256,7 +308,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             L.check(size, what)
         _workspace_bytes[dev.index, d, max_rows] = size
     ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    sp, ss, sh, _ = k_cache.stride()
+    sp, ss, sh, _ = strides
     q_tok, q_head, _ = q.stride()
     o_tok, o_head, _ = out.stride()
     _launch(dev, L.lib().fp8b200_paged_attention, what, q.data_ptr(), L.dtype_code(q.dtype), q_tok, q_head, t, hq, hk, d,
