@@ -1257,7 +1257,9 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
     if (alike) return FP8B200_OK;
     p.zero_rest = 0;
   }
-  const Variant v = variant_for(f16, cache_dtype, dp, std::min<int64_t>(most, p.rows_upto));
+  // beside chunks nearly all short requests decode one token: their rows are the group
+  const int64_t rows = p.rows_upto == TC_OVER ? std::min<int64_t>(p.group <= 8 ? 8 : 16, TC_OVER) : most;
+  const Variant v = variant_for(f16, cache_dtype, dp, rows);
   if (int rc = launch_attributes((const void *)v.main, v.smem)) return rc;
   if (int rc = launch_attributes((const void *)v.merge, 0)) return rc;
   const int grid = current_sm_count() * v.per_sm;
