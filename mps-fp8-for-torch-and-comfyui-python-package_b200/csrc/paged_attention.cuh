@@ -236,8 +236,9 @@ __device__ __forceinline__ void merge_segment(const AttnParams &p, int64_t c, co
   constexpr int V = DP / 4;                                 // float4 a row
   constexpr int SPLIT = V < 32 ? 32 / V : 1, PASS = V > 32 ? V / 32 : 1;  // parts side by side, float4 a lane
   for (int row = blockIdx.y * (MERGE_THREADS / 32) + (threadIdx.x >> 5); row < d.rows; row += gridDim.y * (MERGE_THREADS / 32)) {
-    // AT parts at a time: their values, bases and sums in flight together
-    constexpr int AT = 16 / PASS, N = AT / SPLIT;
+    // AT parts at a time: their values, bases and sums in flight together. A
+    // few rows' segment has many parts, a block of 256 rows two or three.
+    constexpr int AT = MR >= 128 ? 4 : 16 / PASS, N = AT / SPLIT;
     float base = -INFINITY, l = 0.0f;
     float4 acc[PASS];
 #pragma unroll
