@@ -91,8 +91,8 @@ __device__ __forceinline__ uint32_t unit_at(int r, int c) {
   return (uint32_t)(r * ROWB + ((c ^ x) << 4));
 }
 
-// Units (key tiles x row tiles x heads) of request r; 0 if this launch leaves
-// it to another. A request whose mask leaves nothing still has one, which
+// Units (key tiles x row tiles, x heads unless each head has blocks of its own)
+// of request r; 0 if this launch leaves it to another. A request whose mask leaves nothing still has one, which
 // writes its zeros.
 template <int MR>
 __device__ __forceinline__ long long units_of(const AttnParams &p, int r, int &tiles) {
@@ -101,7 +101,7 @@ __device__ __forceinline__ long long units_of(const AttnParams &p, int r, int &t
   if (q.n == 0 || !takes(p, q.n)) return 0;
   tiles = max(1, visible_tiles<BN>(p, q.first, q.first + q.n - 1).count());
   const long long row_tiles = ((long long)q.n * p.group + MR - 1) / MR;
-  return row_tiles * p.hk * tiles;
+  return row_tiles * p.line_heads * tiles;
 }
 
 // a / b and the rest, in 32 bits where they fit (a 64-bit division is a call of
@@ -133,7 +133,7 @@ struct Share {
   }
 };
 template <int MR>
-__device__ __forceinline__ Share find_share(const AttnParams &p, long long *s_scan) {
+__device__ __forceinline__ Share find_share(const AttnParams &p, long long *s_scan, long long c, long long most) {  // block c of at most `most`
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Share sh;
   int tiles;
@@ -164,9 +164,8 @@ __device__ __forceinline__ Share find_share(const AttnParams &p, long long *s_sc
     scan(more, sum);
     total += sum;
   }
-  const long long c = blockIdx.x;
-  if (tid == 0) p.desc[c].rows = 0;
-  const long long blocks = min((long long)gridDim.x, (total + MIN_UNITS - 1) / MIN_UNITS);
+  if (tid == 0) p.desc[blockIdx.x].rows = 0;
+  const long long blocks = min(most, (total + MIN_UNITS - 1) / MIN_UNITS);
   sh.r = -1;
   sh.u = sh.u_end = sh.before = sh.each = sh.extra = 0;
   if (c >= blocks) return sh;
@@ -275,8 +274,11 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, NG>::PER_SM)) paged
   const int used = (p.d * (C::FP8 ? 1 : 2)) / 16;          // 16-byte units of a key's row that hold values
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const Share sh = find_share<C::MR>(p, s_scan);
+  // line_heads 1: as many lines as heads, their blocks side by side, so that the
+  // heads of a key (neighbours in memory) are read at about the same time
   const long long c = blockIdx.x;
+  const int lines = p.line_heads == 1 ? p.hk : 1, line = (int)(c % lines);
+  const Share sh = find_share<C::MR>(p, s_scan, c / lines, gridDim.x / lines);
   long long u = sh.u, before = sh.before;
   int r = sh.r;
   while (r >= 0 && u < sh.u_end) {
@@ -290,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, NG>::PER_SM)) paged
       continue;
     }
     long long in_tiles, in_heads;
-    const int qt = (int)quotient(quotient(u - before, tiles_n, in_tiles), p.hk, in_heads), h = (int)in_heads;
+    const int qt = (int)quotient(quotient(u - before, tiles_n, in_tiles), p.line_heads, in_heads), h = line + (int)in_heads;
     const int t_begin = (int)in_tiles, t_end = (int)min((long long)tiles_n, t_begin + (sh.u_end - u));
     const long long seg_start = u - t_begin;
     u += t_end - t_begin;
@@ -567,7 +569,7 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, NG>::PER_SM)) paged
     const float vs = C::FP8 && p.vs ? __ldg(p.vs + p.vs_step * h) : 1.0f;
     float *part = p.part + (c * 2 + (begins ? 1 : 0)) * (int64_t)(C::MR * (DP + 2));
     if (tid == 0 && begins && !ends)
-      p.desc[c] = PartDesc{rows, row0, h, sh.block_of(seg_start + tiles_n - 1), rq.start};
+      p.desc[c] = PartDesc{rows, row0, h, rq.start, sh.block_of(seg_start + tiles_n - 1) - (int)(c / lines) + 1, lines};
     float *s_o = reinterpret_cast<float *>(smem);           // [4 warps][16 rows][SO]
 #pragma unroll
     for (int mg = 0; mg < (NG + 1) / 2; mg++) {
@@ -695,7 +697,7 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ---- this block's share of the line of units
-  const Share sh = find_share<C::MR>(p, s_scan);
+  const Share sh = find_share<C::MR>(p, s_scan, blockIdx.x, gridDim.x);
   if (p.zero_rest) zero_rest(p, blockIdx.x, gridDim.x);
   if (sh.r < 0) return;
   const long long c = blockIdx.x, u_end = sh.u_end;
@@ -1074,7 +1076,7 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
     const float vs = C::FP8 && p.vs ? __ldg(p.vs + p.vs_step * h) : 1.0f;
     float *part = p.part + (c * 2 + (begins ? 1 : 0)) * (int64_t)(C::MR * (DP + 2));
     if (tid == 0 && begins && !ends)
-      p.desc[c] = PartDesc{rows, row0, h, sh.block_of(seg_start + tiles_n - 1), rq.start};
+      p.desc[c] = PartDesc{rows, row0, h, rq.start, sh.block_of(seg_start + tiles_n - 1) - (int)c + 1, 1};
     for (int i = tid; i < rows * (DP / 4); i += THREADS) {
       const int row = i / (DP / 4), d4 = (i % (DP / 4)) * 4;
       const int at = (row >> 4) * C::KW * 16 + (row & 15);
@@ -1112,15 +1114,16 @@ struct Variant {
   void (*main)(AttnParams);
   void (*merge)(AttnParams);
   int smem, per_sm, rows;
+  bool few;
 };
 template <bool F16, int KV, int DP, int NG>
 Variant few() {
   using C = Few<F16, KV, DP, NG>;
-  return {paged_few_kernel<F16, KV, DP, NG>, paged_merge_kernel<F16, DP, C::MR>, C::SMEM, C::PER_SM, C::MR};
+  return {paged_few_kernel<F16, KV, DP, NG>, paged_merge_kernel<F16, DP, C::MR>, C::SMEM, C::PER_SM, C::MR, true};
 }
 template <bool F16, int KV, int DP>
 Variant many() {
-  return {paged_attention_kernel<F16, KV, DP, 4>, paged_merge_kernel<F16, DP, 64>, Cfg<F16, KV, DP, 4>::SMEM, DP == 256 ? 1 : 2, 64};
+  return {paged_attention_kernel<F16, KV, DP, 4>, paged_merge_kernel<F16, DP, 64>, Cfg<F16, KV, DP, 4>::SMEM, DP == 256 ? 1 : 2, 64, false};
 }
 // `rows`: query rows of the longest request (a request with more is served in several row tiles).
 template <bool F16, int KV>
@@ -1263,6 +1266,7 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
   if (int rc = launch_attributes((const void *)v.main, v.smem)) return rc;
   if (int rc = launch_attributes((const void *)v.merge, 0)) return rc;
   const int grid = current_sm_count() * v.per_sm;
+  p.line_heads = v.few && n_kv_heads <= grid / 4 ? 1 : n_kv_heads;
   launch_dependent(v.main, dim3((unsigned)grid), THREADS, v.smem, (cudaStream_t)stream, p);
   p.blocks = grid;
   launch_dependent(v.merge, dim3((unsigned)current_sm_count(), (unsigned)std::max(1, v.rows / 16)), MERGE_THREADS, 0, (cudaStream_t)stream, p);

@@ -12,8 +12,9 @@ namespace paged {
 // A segment that was cut, for the merge: written by the block that begins it.
 struct alignas(16) PartDesc {
   int rows;                   // of the row tile; 0: this block began no such segment
-  int row0, h, last;          // the tile's first row in its request, the key/value head, the block that ends the segment
+  int row0, h;                // the tile's first row in its request, the key/value head
   int start;                  // the request's first row of q
+  int parts, step;            // the parts: the second of this block, the first of the blocks step, 2 * step, ... behind it
 };
 static_assert(sizeof(PartDesc) == 32, "two 16-byte words");
 
@@ -44,6 +45,7 @@ struct AttnParams {
   float *part;
   PartDesc *desc;
   int blocks;                 // for the merge: how many descriptors there are
+  int line_heads;             // key/value heads that a line of units holds: all, or one (a line a head)
 };
 
 // The new tokens of request r: rows [start, start + n) of q, the last at
@@ -159,7 +161,7 @@ __device__ __forceinline__ float cache_value(const uint8_t *base, int64_t elem) 
 }
 
 // The kernel for many query rows (paged_attention_tc.cu): head sizes up to
-// 128, caches that a tensor map can describe (tc_takes).
+// 128, caches that a tensor map can describe, at most 16384 requests (tc_takes).
 bool tc_takes(const AttnParams &p);
 int64_t tc_workspace(int dp, int sms);
 int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int sms, uint8_t *workspace, cudaStream_t st);
@@ -219,7 +221,7 @@ __device__ __noinline__ void careful_row(const AttnParams &p, int r, int tok, in
 
 // Joins the parts of the segments that were cut: block c the one that began
 // in block c of the attention kernel (its second part), with the first parts
-// of the blocks after it, in their order. A warp a row: its lanes fetch the
+// of the blocks that went on with it, in their order. A warp a row: its lanes fetch the
 // parts' bases and sums together, then the rows' values, whose loads do not
 // wait for one another. MR: rows a part has room for. A block an SM (times
 // the row groups) goes through the descriptors: so few fit beside the
@@ -228,10 +230,10 @@ constexpr int MERGE_THREADS = 256;
 template <bool F16, int DP, int MR>
 __device__ __forceinline__ void merge_segment(const AttnParams &p, int64_t c, const PartDesc &d) {
   const int lane = threadIdx.x & 31;
-  const int n = d.last - (int)c + 1;                        // parts
+  const int n = d.parts;
   constexpr int64_t SLOT = MR * (DP + 2);
-  const float *parts = p.part + (c * 2 + 1) * SLOT;         // the first; part k > 0 is the first of block c + k
-  auto part_at = [&](int k) { return parts + (k == 0 ? 0 : (2 * (int64_t)k - 1) * SLOT); };
+  const float *parts = p.part + (c * 2 + 1) * SLOT;         // the first; part k > 0 is the first of block c + k * step
+  auto part_at = [&](int k) { return parts + (k == 0 ? 0 : (2 * (int64_t)k * d.step - 1) * SLOT); };
   const float vs = p.vs ? __ldg(p.vs + p.vs_step * d.h) : 1.0f;
   constexpr int V = DP / 4;                                 // float4 a row
   constexpr int SPLIT = V < 32 ? 32 / V : 1, PASS = V > 32 ? V / 32 : 1;  // parts side by side, float4 a lane

@@ -53,9 +53,12 @@ constexpr int KT = 128;          // keys a tile
 constexpr int QT = 128;          // rows a tile
 constexpr int QB = 2 * QT;       // rows a block
 constexpr int SEG_COST = 3;       // what a segment's start and end cost, in key tiles
+constexpr int MAX_REQUESTS = 16384;  // their first rows pass through shared memory
 constexpr int SEGS = 4;           // segments in the ring
 constexpr int HIDE_RING = 8;     // tiles whose page masks are kept: more than the producers run ahead of the softmax
-constexpr unsigned long long WAIT_NS = 2000000000ull;
+// Long: a group that recomputes rows value by value (careful_row) over a long
+// segment keeps the other roles waiting for a second or more.
+constexpr unsigned long long WAIT_NS = 10000000000ull;
 
 __device__ uint32_t g_paged_status;  // 0, or the site of a wait that ran out
 
@@ -92,7 +95,7 @@ struct Tc {
   static constexpr uint32_t IDESC_S = (1u << 4) | (FMT << 7) | (FMT << 10) | ((uint32_t)(KT >> 3) << 17) | ((128u >> 4) << 24);
   static constexpr uint32_t IDESC_O =
       (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((128u >> 4) << 24);
-  static_assert(OFF_PLAN >= (16384 + 1) * 4, "the requests' first rows fit in front of it");
+  static_assert(OFF_PLAN >= (MAX_REQUESTS + 1) * 4, "the requests' first rows fit in front of it");
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
 
@@ -885,7 +888,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
       fence_after();
       const bool begins = t_begin == 0, whole = begins && t_end == sg->units;
       if (tid == 0 && begins && !whole)
-        p.desc[c] = PartDesc{min(QB, all_rows - sg->qt * QB), sg->qt * QB, h, sg->last, sg->start};
+        p.desc[c] = PartDesc{min(QB, all_rows - sg->qt * QB), sg->qt * QB, h, sg->start, sg->last - (int)c + 1, 1};
       const float vs = C::FP8 && p.vs ? __ldg(p.vs + p.vs_step * h) : 1.0f;
       const float inv = sum == 0.0f ? 0.0f : vs / sum;
       const float mine_base = base - C::SHIFT;
@@ -1038,11 +1041,12 @@ int launch_attributes(const void *kernel, int smem) {
 
 int64_t tc_workspace(int dp, int sms) { return (int64_t)sms * (2 * QB * (int64_t)(dp + 2) * 4 + (int64_t)sizeof(PartDesc)); }
 
-// What a tensor map can describe: strides above 0 (below 2^40 bytes), extents below 2^31.
+// What a tensor map can describe: strides above 0 (below 2^40 bytes), extents
+// below 2^31; and as many requests as the plan holds.
 bool tc_takes(const AttnParams &p) {
   const int64_t most = (int64_t)1 << 38;
   auto fits = [&](int64_t n, int64_t stride) { return n == 1 || (stride > 0 && stride < most); };
-  return p.pages > 0 && p.pages < INT32_MAX && fits(p.hk, p.s_head) && fits(p.page, p.s_slot) && fits(p.pages, p.s_page);
+  return p.requests <= MAX_REQUESTS && p.pages > 0 && p.pages < INT32_MAX && fits(p.hk, p.s_head) && fits(p.page, p.s_slot) && fits(p.pages, p.s_page);
 }
 
 int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int sms, uint8_t *workspace, cudaStream_t st) {

@@ -26,6 +26,7 @@ from . import _lib as L
 _FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
 _16BIT = (torch.bfloat16, torch.float16)
 MAX_REQUESTS = 16384
+_INT_MAX = 2 ** 31 - 1
 
 
 class PagedStep(NamedTuple):
@@ -215,7 +216,7 @@ def rope_write_paged(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, po
     width = (n_q_heads + 2 * hk) * d
     ld = qkv.stride(0) if t > 1 and qkv.dim() == 2 else width
     if not (dt in _16BIT and (cdt is dt or cdt in _FP8) and v_cache.dtype is cdt and v_cache.shape == shape and len(shape) == 4
-            and v_cache.stride() == strides and strides[3] == 1 and qkv.shape == (t, qkv.shape[-1]) and qkv.shape[1] >= width
+            and v_cache.stride() == strides and strides[3] == 1 and qkv.dim() == 2 and qkv.shape[0] == t and qkv.shape[1] >= width
             and ld >= width and n_q_heads >= 0 and (t == 0 or qkv.stride(1) == 1)
             and cos.dtype is sin.dtype is torch.float32 and cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] * 2 == d
             and cos.is_contiguous() and sin.is_contiguous() and positions.dtype is torch.int32 and positions.dim() == 1
@@ -248,8 +249,8 @@ def _check_attention(q, k_cache, v_cache, block_table, cu_new, kv_lens, window, 
     if cu_new.numel() != n + 1 or kv_lens.numel() != n:
         raise RuntimeError(f"{what}: {n} block_table rows need {n + 1} cu_new and {n} kv_lens, got {cu_new.numel()} and "
                            f"{kv_lens.numel()}")
-    if window < 0 or sinks < 0:
-        raise RuntimeError(f"{what}: window={window} and sinks={sinks} must not be negative")
+    if not (0 <= window <= _INT_MAX and 0 <= sinks <= _INT_MAX):
+        raise RuntimeError(f"{what}: window={window} and sinks={sinks} must not be negative or 2^31 and more")
     if max_new is not None and max_new < 1:
         raise RuntimeError(f"{what}: max_new={max_new} must be positive")
 
@@ -275,8 +276,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     see the kernels for the weights' type. A query that sees no key gives 0; a
     table entry outside the pool hides its keys; hidden keys' values, NaN
     included, have no effect. Rows that belong to no request are left as they
-    were in a given `out` (of q's shape and type, any 16-byte aligned rows)
-    and 0 in a new one."""
+    were in a given `out` (of q's shape and type, any 16-byte aligned rows, no
+    overlap with q) and 0 in a new one."""
     what = "paged_attention"
     dev, dt, cdt = q.device, q.dtype, k_cache.dtype
     shape, strides, qshape = k_cache.shape, k_cache.stride(), q.shape
@@ -289,7 +290,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             and hk >= 1 and hq >= 1 and hq % hk == 0 and block_table.dtype is cu_new.dtype is kv_lens.dtype is torch.int32
             and block_table.dim() == 2 and (cols <= 1 or block_table.stride(1) == 1) and ld >= cols
             and cu_new.shape == (n + 1,) and kv_lens.shape == (n,) and cu_new.is_contiguous() and kv_lens.is_contiguous()
-            and window >= 0 and sinks >= 0 and (max_new is None or max_new >= 1)
+            and 0 <= window <= _INT_MAX and 0 <= sinks <= _INT_MAX and (max_new is None or max_new >= 1)
             and k_cache.device == v_cache.device == block_table.device == cu_new.device == kv_lens.device == dev):
         _check_attention(q, k_cache, v_cache, block_table, cu_new, kv_lens, window, sinks, max_new)
     ks, ks_step = (None, 0) if k_scale is None else _check_scale(k_scale, "k_scale", what, k_cache)
@@ -299,6 +300,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         out = q.new_empty(qshape)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or (out.numel() and out.stride(2) != 1):
         raise RuntimeError(f"{what}: `out` must be a {q.dtype} tensor of q's shape on {dev} with contiguous heads")
+    elif out.data_ptr() == q.data_ptr() and t:
+        raise RuntimeError(f"{what}: `out` must not overlap q")
     max_rows = min(t if max_new is None else max_new, t) * (hq // hk)
     size = _workspace_bytes.get((dev.index, d, max_rows), 0)
     if size == 0 and dev.type == "cuda":

@@ -521,6 +521,13 @@ def test_attention_many_requests(nat):
     check(nat, build(new, kv, 2, 1, 64, 16, BF16, BF16, seed=15))
     new = [0] * 400 + [50] + [0] * 300
     check(nat, build(new, [50] * 701, 2, 1, 64, 16, BF16, BF16, seed=16))
+    new = [0] * 20000                                     # more than the kernel for chunks plans for
+    new[3], new[19999] = 130, 1
+    kv = [0] * 20000
+    kv[3], kv[19999] = 140, 70
+    check(nat, build(new, kv, 2, 1, 64, 16, BF16, E4M3, seed=19))
+    new = [0] * 400 + [50] + [0] * 300
+    check(nat, build(new, [50] * 701, 2, 1, 64, 16, BF16, BF16, seed=16))
 
 
 def test_two_streams_and_two_graphs(nat):

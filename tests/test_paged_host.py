@@ -55,6 +55,7 @@ SLOTS = [
 ]
 WRITE = [
     (dict(qkv=torch.zeros(3, 512)), "bfloat16 or float16"),
+    (dict(qkv=torch.zeros((), dtype=BF16)), "qkv must be"),
     (dict(qkv=torch.zeros(3, 512, dtype=F16)), "the caches must both be"),
     (dict(v_cache=torch.zeros(4, 16, 2, 64, dtype=BF16).to(E4M3)), "the caches must both be"),
     (dict(v_cache=WIDE), "of one shape"),
@@ -77,6 +78,7 @@ WRITE = [
 FP8_CACHES = dict(k_cache=torch.zeros(4, 16, 2, 64).to(E4M3), v_cache=torch.zeros(4, 16, 2, 64).to(E4M3))
 WRITE += [(dict(FP8_CACHES, k_scale=s), "k_scale must be") for s in
           (torch.ones(3), torch.ones(2, dtype=BF16), torch.ones(4)[::2])] + [(FP8_CACHES, "CUDA device")]
+SAME = torch.zeros(3, 4, 64, dtype=BF16)
 ATTENTION = [
     (dict(q=torch.zeros(3, 4, 64)), "bfloat16 or float16"),
     (dict(q=torch.zeros(3, 4, 32, dtype=BF16)), "q must be"),
@@ -91,12 +93,15 @@ ATTENTION = [
     (dict(kv_lens=torch.zeros(2, dtype=torch.int64)), "kv_lens must be"),
     (dict(window=-1), "window=-1"),
     (dict(sinks=-1), "sinks=-1"),
+    (dict(window=2 ** 32), "2\\^31"),
+    (dict(sinks=2 ** 31), "2\\^31"),
     (dict(max_new=0), "max_new=0"),
     (dict(v_scale=torch.ones(1)), "float8 cache only"),
     (dict(FP8_CACHES, v_scale=torch.ones(3)), "v_scale must be"),
     (dict(out=torch.zeros(3, 4, 64)), "`out` must be"),
     (dict(out=torch.zeros(3, 4, 128, dtype=BF16)[..., ::2]), "`out` must be"),
     (dict(out=torch.zeros(2, 4, 64, dtype=BF16)), "`out` must be"),
+    (dict(q=SAME, out=SAME), "overlap"),
     ({}, "CUDA device"),
 ]
 
