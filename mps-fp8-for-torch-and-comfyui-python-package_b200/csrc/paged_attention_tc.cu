@@ -33,8 +33,17 @@
 // share of a segment's edge moves there, so with many segments none is split,
 // and with few all SMs still work.
 //
-// Bound by the tensor core and the exponentials alike: 256 x 128 scores cost
-// 2048 cycles of MMA at head size 128 and 2048 cycles of ex2 (16 a cycle).
+// Bound by the chain S -> weights -> P V -> next S of a row tile, against the
+// other's: 256 x 128 scores cost 2048 cycles of MMA at head size 128 and 2048
+// cycles of ex2 (16 a cycle), and take about 3600. Measured, 32 / 8 heads of
+// 128: 2048 tokens over 14001 cached in e4m3 524 us (960 TFLOP/s), prompts of 8
+// x 2048 in bf16 397 us (690 TFLOP/s), 1500 tokens with a window of 4096 and 4
+// sinks 142 us. Tried and slower: two score buffers of 64 keys a row tile (570
+// us on the first: N = 64 MMAs read A again for half the work), two threads a
+// row (the registers spill), part of the exponentials as a polynomial on the
+// multiply-add pipes (596 us; issue slots are as short as ex2), K and V through
+// cp.async (a proxy fence waits for all of a thread's copies) or four-row
+// gathers.
 //
 // No counterpart in the reference.
 #include "paged_attention.cuh"
