@@ -73,8 +73,10 @@ __device__ uint32_t g_paged_status;  // 0, or the site of a wait that ran out
 
 // Tensor maps of the caches, 4-D (head_dim, heads, slots of a page, pages):
 // boxes of 2^box_log slots, and of one.
+// And of q (head_dim, heads, tokens), boxes of 128 rows of the group's heads.
 struct TcMaps {
   CUtensorMap box[2], one[2];  // K, V
+  CUtensorMap q;
 };
 
 template <bool F16, int KV, int DP>
@@ -95,8 +97,8 @@ struct Tc {
   static constexpr int OFF_PLAN = OFF_RAW + RAWS * RAW;   // the plan's scratch
   static constexpr int OFF_HIDE = OFF_PLAN + 256;         // page masks, 128 bits a tile
   static constexpr int OFF_BARS = OFF_HIDE + HIDE_RING * 16;
-  static constexpr int BARS = 2 * SLOTS + 2 * RAWS + 10 + 2 * SEGS;
-  static constexpr int OFF_SEGS = OFF_BARS + BARS * 8;
+  static constexpr int BARS = 2 * SLOTS + 2 * RAWS + 11 + 2 * SEGS;
+  static constexpr int OFF_SEGS = (OFF_BARS + BARS * 8 + 15) / 16 * 16;
   static constexpr int SMEM = OFF_SEGS + SEGS * 48 + 16;
   static constexpr float SHIFT = MF16 ? 7.0f : 0.0f;      // weights are scaled by 2^SHIFT and stay below 2^(SHIFT + 8)
   static constexpr uint32_t FMT = MF16 ? 0u : 1u;
@@ -105,6 +107,9 @@ struct Tc {
   static constexpr uint32_t IDESC_O =
       (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((128u >> 4) << 24);
   static_assert(OFF_PLAN >= (MAX_REQUESTS + 1) * 4, "the requests' first rows fit in front of it");
+  static_assert(OFF_KV % 1024 == 0 && TILE % 1024 == 0 && OFF_RAW % 1024 == 0 && OFF_PLAN % 16 == 0 && OFF_HIDE % 16 == 0 &&
+                    OFF_BARS % 8 == 0 && OFF_SEGS % 16 == 0,
+                "swizzled tiles, vector accesses and barriers are aligned");
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
 
@@ -261,6 +266,13 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, i
       "l"(map), "r"(x), "r"(h), "r"(off), "r"(page), "r"(bar)
       : "memory");
 }
+// Columns x .. of the group's heads from h on, of the tokens from tok on.
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap *map, int x, int h, int tok, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(h), "r"(tok), "r"(bar)
+      : "memory");
+}
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void sts16(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
@@ -336,7 +348,8 @@ static_assert(sizeof(Segment) == 48, "SEGS * 48 bytes");
 
 template <bool F16, int KV, int DP>
 __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
-    paged_attention_tc_kernel(const AttnParams p, const __grid_constant__ TcMaps maps, const int box_log) {
+    paged_attention_tc_kernel(const AttnParams p, const __grid_constant__ TcMaps maps, const int box_log,
+                              const int q_boxes) {
   using C = Tc<F16, KV, DP>;
   constexpr int TC_THREADS = C::THREADS;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -352,7 +365,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
   auto raw_full = [&](int s) { return bars + 8u * (2 * C::SLOTS + s); };
   auto raw_empty = [&](int s) { return bars + 8u * (2 * C::SLOTS + C::RAWS + s); };
   const uint32_t q_full = bars + 8u * (2 * C::SLOTS + 2 * C::RAWS), s_full = q_full + 16, p_full = q_full + 32, pv_done = q_full + 48;
-  const uint32_t p_half = q_full + 64, seg_full = q_full + 80, seg_empty = seg_full + 8 * SEGS;
+  const uint32_t p_half = q_full + 64, q_free = q_full + 80, seg_full = q_full + 88, seg_empty = seg_full + 8 * SEGS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
 
   if (base_a & 1023u) {  // the swizzled tiles need it; the same for every CTA
@@ -369,12 +382,13 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
       bar_init(raw_empty(s), 128);
     }
     for (int g = 0; g < 2; g++) {
-      bar_init(q_full + 8 * g, QT);
+      bar_init(q_full + 8 * g, q_boxes ? 1 : QT);
       bar_init(s_full + 8 * g, 1);
       bar_init(p_half + 8 * g, QT);
       bar_init(p_full + 8 * g, QT);
       bar_init(pv_done + 8 * g, 1);
     }
+    bar_init(q_free, 1);
     for (int i = 0; i < SEGS; i++) {
       bar_init(seg_full + 8 * i, 1);
       bar_init(seg_empty + 8 * i, C::FP8 ? 15 : 11);  // the warps that read it: softmax, converting, MMA, TMA
@@ -517,6 +531,15 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
           if (n >= SEGS && !bar_wait(seg_empty + 8 * (n % SEGS), ((n / SEGS) & 1) ^ 1, s_failed, 50)) break;
           s_seg[n % SEGS] = sg;
           bar_arrive(seg_full + 8 * (n % SEGS));
+          if (!C::FP8 && q_boxes && sg.r >= 0) {           // its rows of Q, once the last S of the segment before has read those
+            if (n > 0 && !bar_wait(q_free, (n - 1) & 1, s_failed, 56)) break;
+            for (int g = 0; g < 2; g++) {
+              const int tok = sg.start + (sg.qt * QB + g * QT) / p.group;
+              bar_expect(q_full + 8 * g, C::TILE);
+              for (int b = 0; b < DP / 64; b++)
+                load_rows(base_a + g * C::TILE + b * (QT * 128), &maps.q, b * 64, sg.h * p.group, tok, q_full + 8 * g);
+            }
+          }
           more = sg.r >= 0;
           n++;
         }
@@ -551,6 +574,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
         issue_s(0, slot);
         issue_s(1, slot);
         commit(kv_empty(slot));
+        if (n == 1) commit(q_free);
         step();
         for (int j = 0; j < n && ok; j++) {
           const bool more = j + 1 < n;
@@ -581,6 +605,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
           if (!ok) break;
           commit(kv_empty(vs));
           if (more) commit(kv_empty(ks));
+          if (j + 2 == n) commit(q_free);                  // the segment's last S is issued
           tiles++;
         }
         segs++;
@@ -709,7 +734,8 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
     const uint32_t q_a = base_a + g * C::TILE;
     uint32_t tiles = 0;
     bool ok = true;
-    // The group's rows of Q for a segment. A row takes DP / 8 lanes, so that a
+    // The group's rows of Q for a segment, where they do not come by boxes
+    // (float8 caches, groups that do not divide 128, negative scales). A row takes DP / 8 lanes, so that a
     // warp reads whole rows; the owner of row r gets its scale from them.
     float qscale = 1.0f;
     auto load_q = [&](const Segment *sg) {
@@ -767,7 +793,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
     };
     const Segment *sg = seg_at(0, 53);
     if (!__all_sync(~0u, sg != nullptr)) ok = false;
-    if (ok && sg->r >= 0) load_q(sg);
+    if (ok && sg->r >= 0 && !q_boxes) load_q(sg);
     for (uint32_t segs = 0; ok && sg->r >= 0; segs++) {
       const int h = sg->h, first = sg->first, t_begin = sg->t_begin, t_end = sg->t_end;
       const int all_rows = sg->n * p.group;                // below 2^31: tokens x query heads are
@@ -786,7 +812,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
         ok = false;
         break;
       }
-      if (next->r >= 0) prefetch_q(next);
+      if (next->r >= 0 && !q_boxes) prefetch_q(next);
       float base = -INFINITY, sum = 0.0f;                  // of this row: weights are 2^(score - base + SHIFT)
       for (int t = t_begin; t < t_end; t++) {
         const int k0 = sg->tile(t) * KT;
@@ -887,7 +913,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
         break;
       }
       // ---- the next segment's rows of Q: the last S, for which all have waited, was the last reader of these
-      if (next->r >= 0) load_q(next);
+      if (next->r >= 0 && !q_boxes) load_q(next);
       // ---- the segment's end
       ok = bar_wait(pv_done + 8 * g, (tiles - 1) & 1, s_failed, 40 + g);
       if (!__all_sync(~0u, ok)) {
@@ -995,7 +1021,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
   if (warp == C::CTRL) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 
-using TcKernel = void (*)(AttnParams, TcMaps, int);
+using TcKernel = void (*)(AttnParams, TcMaps, int, int);
 struct TcVariant {
   TcKernel main;
   void (*merge)(AttnParams);
@@ -1086,9 +1112,20 @@ int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int s
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(FP8B200_ELAUNCH, "paged_attention: tensor map encode failed (%d)", (int)r);
   }
+  const auto above0 = [](int64_t n, int64_t stride) { return n == 1 || (stride > 0 && stride < (int64_t)1 << 38); };
+  int q_boxes = !fp8 && QT % p.group == 0 && !(p.scale_log2 < 0.0f) && above0(p.hq, p.q_head) && above0(p.tokens, p.q_tok);
+  maps.q = maps.box[0];
+  if (q_boxes) {
+    const cuuint64_t dims[3] = {(cuuint64_t)p.d, (cuuint64_t)p.hq, (cuuint64_t)p.tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)(p.hq > 1 ? p.q_head : p.d) * 2, (cuuint64_t)(p.tokens > 1 ? p.q_tok : p.d) * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)(QT / p.group)}, step[3] = {1, 1, 1};
+    q_boxes = encode(&maps.q, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<uint16_t *>(p.q), dims, strides, box, step,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  }
   if (int rc = launch_attributes((const void *)v.main, v.smem)) return rc;
   if (int rc = launch_attributes((const void *)v.merge, 0)) return rc;
-  launch_dependent(v.main, dim3((unsigned)sms), v.threads, v.smem, st, p, maps, box_log);
+  launch_dependent(v.main, dim3((unsigned)sms), v.threads, v.smem, st, p, maps, box_log, q_boxes);
   launch_dependent(v.merge, dim3((unsigned)sms, 8), MERGE_THREADS, 0, st, p);
   count_launch(2);
   return check_launch("paged_attention");
