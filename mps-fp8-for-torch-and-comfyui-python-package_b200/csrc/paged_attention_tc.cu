@@ -61,7 +61,7 @@ namespace {
 constexpr int KT = 128;          // keys a tile
 constexpr int QT = 128;          // rows a tile
 constexpr int QB = 2 * QT;       // rows a block
-constexpr int SEG_COST = 3;       // what a segment's start and end cost, in key tiles
+constexpr int SEG_COST = 2;       // what a segment's start and end cost, in key tiles
 constexpr int MAX_REQUESTS = 16384;  // their first rows pass through shared memory
 constexpr int SEGS = 4;           // segments in the ring
 constexpr int HIDE_RING = 8;     // tiles whose page masks are kept: more than the producers run ahead of the softmax
@@ -746,7 +746,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
       const int64_t own_at = (int64_t)(sg->start + own_tok) * p.q_tok + (int64_t)(sg->h * p.group + own - own_tok * p.group) * p.q_head;
       // its sign takes that of the scale, so that the maximum of the products is the maximum of the scores
       const uint32_t flip = p.scale_log2 * (C::FP8 && p.ks ? __ldg(p.ks + p.ks_step * sg->h) : 1.0f) < 0.0f ? 0x80008000u : 0u;
-      constexpr int BATCH = C::FP8 || DP == 64 ? 8 : 16;   // loads in flight
+      constexpr int BATCH = C::FP8 ? 4 : DP == 64 ? 8 : 16;  // loads in flight
 #pragma unroll 1
       for (int i0 = 0; i0 < 32 / RPI; i0 += BATCH) {
         uint4 v[BATCH];
