@@ -11,7 +11,9 @@
 // and a warpgroup for control:
 //   MMA      issues S = Q K^T and O += P V (a uniform warp, one lane's
 //            instructions: the descriptors stay in uniform registers)
-//   segments walks the CTA's share of the work and hands its segments on
+//   segments walks the CTA's share of the work and hands its segments on; with a
+//            16-bit cache and a group that divides 128 it also brings their rows
+//            of Q by TMA boxes (397 -> 364 us at 8 x 2048), else the groups do
 //   2 x TMA  in turn bring K and V tiles in, boxes of as many slots as divide
 //            both the page and the tile (16 for pages of 16 or 48 slots); boxes
 //            without a key are out of the map's bounds and arrive as zeros, a
@@ -35,15 +37,17 @@
 //
 // Bound by the chain S -> weights -> P V -> next S of a row tile, against the
 // other's: 256 x 128 scores cost 2048 cycles of MMA at head size 128 and 2048
-// cycles of ex2 (16 a cycle), and take about 3600. Measured, 32 / 8 heads of
-// 128: 2048 tokens over 14001 cached in e4m3 524 us (960 TFLOP/s), prompts of 8
-// x 2048 in bf16 397 us (690 TFLOP/s), 1500 tokens with a window of 4096 and 4
-// sinks 142 us. Tried and slower: two score buffers of 64 keys a row tile (570
-// us on the first: N = 64 MMAs read A again for half the work), two threads a
-// row (the registers spill), part of the exponentials as a polynomial on the
-// multiply-add pipes (596 us; issue slots are as short as ex2), K and V through
-// cp.async (a proxy fence waits for all of a thread's copies) or four-row
-// gathers.
+// cycles of ex2 (16 a cycle), and take about 4100 (tensor pipe busy 49 % of the
+// time at 2048 rows over 14001 keys). Measured, 32 / 8 heads of 128: 2048 tokens
+// over 14001 cached in e4m3 512 us (985 TFLOP/s), prompts of 8 x 2048 in bf16
+// 351 us (783 TFLOP/s; short segments, so their starts and ends count), 1500
+// tokens with a window of 4096 and 4 sinks 142 us. SEG_COST of 2 gave 351 us on
+// the prompts, 3 gave 364. Tried and slower: two score buffers of 64 keys a row
+// tile (570 us against 540 then: N = 64 MMAs read A again for half the work),
+// two threads a row (the registers spill), part of the exponentials as a
+// polynomial on the multiply-add pipes (596 us against 540; issue slots are as
+// short as ex2), K and V through cp.async (a proxy fence waits for all of a
+// thread's copies) or four-row gathers.
 //
 // No counterpart in the reference.
 #include "paged_attention.cuh"
