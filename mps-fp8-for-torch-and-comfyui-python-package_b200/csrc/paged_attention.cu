@@ -119,9 +119,12 @@ __device__ __forceinline__ long long quotient(long long a, long long b, long lon
 
 // A block's share [u, u_end) of the line of units, found by all its threads:
 // the request that u falls into and the units before that request. The first
-// `extra` blocks have `each` + 1 units, the others `each`; at least MIN_UNITS a
-// block, below that the join costs more than the share saves.
-constexpr int MIN_UNITS = 2;
+// `extra` blocks have `each` + 1 units, the others `each`. With few units every
+// one has its block: with two a block as the least, blocks whose two units lie in
+// different segments went through two prologues and ends (12 rows of 3 requests
+// over 700 keys 20.9 us, now 18.4; 64 rows of 4 over 300 30.9, now 20.6), which
+// outweighs the join of segments of two units (16 decodes over 100 keys 12.5 us,
+// now 14.5; in graphs).
 struct Share {
   long long u, u_end, before, each, extra;
   int r;  // -1: nothing for this block
@@ -132,8 +135,9 @@ struct Share {
     return (int)(x < front ? quotient(x, each + 1, rest) : extra + quotient(x - front, each, rest));
   }
 };
-template <int MR>
+template <int MR, int NW = 4>  // NW: the block's warps
 __device__ __forceinline__ Share find_share(const AttnParams &p, long long *s_scan, long long c, long long most) {  // block c of at most `most`
+  constexpr int THREADS = NW * 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   Share sh;
   int tiles;
@@ -149,7 +153,7 @@ __device__ __forceinline__ Share find_share(const AttnParams &p, long long *s_sc
     __syncthreads();
     total = 0;
 #pragma unroll
-    for (int w = 0; w < 4; w++) {
+    for (int w = 0; w < NW; w++) {
       if (w < warp) inc += s_scan[w];
       total += s_scan[w];
     }
@@ -165,7 +169,7 @@ __device__ __forceinline__ Share find_share(const AttnParams &p, long long *s_sc
     total += sum;
   }
   if (tid == 0) p.desc[blockIdx.x].rows = 0;
-  const long long blocks = min(most, (total + MIN_UNITS - 1) / MIN_UNITS);
+  const long long blocks = min(most, total);
   sh.r = -1;
   sh.u = sh.u_end = sh.before = sh.each = sh.extra = 0;
   if (c >= blocks) return sh;
@@ -182,15 +186,15 @@ __device__ __forceinline__ Share find_share(const AttnParams &p, long long *s_sc
       inc = scan(mine, all);
     }
     if (before + inc > sh.u && before + inc - mine <= sh.u) {
-      s_scan[4] = r;
-      s_scan[5] = before + inc - mine;
+      s_scan[NW] = r;
+      s_scan[NW + 1] = before + inc - mine;
     }
     before += all;
     if (before > sh.u) break;
   }
   __syncthreads();
-  sh.r = (int)s_scan[4];
-  sh.before = s_scan[5];
+  sh.r = (int)s_scan[NW];
+  sh.before = s_scan[NW + 1];
   return sh;
 }
 
@@ -659,41 +663,49 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, NG>::PER_SM)) paged
 // ------------------------------------------------------------------ more rows
 //
 // Where the tensor-memory kernel does not serve (head sizes above 128, caches
-// that no tensor map describes, a few dozen rows): the block's four warps take
-// 16 rows each and share the tile's keys.
-template <bool F16, int KV, int DP, int RW>
+// that no tensor map describes, a few dozen rows): each of the block's NW warps
+// takes 16 rows; with fewer than 16 NW rows NW / RW warps share the tile's keys.
+// Head sizes up to 128: four warps, two blocks an SM. Above, where one block
+// fills the SM: eight warps, since four, one a scheduler, wait on each
+// instruction: 1073 rows of 8 heads over up to 2408 keys 182 -> 138 us in e4m3,
+// 111 us in bf16; 88 rows a request, 10 over 19531 keys in f16 183 -> 142 us. A
+// tile of 128 rows by 64 keys takes 5 to 6 us: 2 us of warp-level MMA, as much
+// of shared-memory reads (each warp reads all of K and V), little overlapped.
+template <bool F16, int KV, int DP, int RW, int NW>
 struct Cfg {
+  static constexpr int THREADS = NW * 32;
   static constexpr bool FP8 = is_fp8<KV>;
   static constexpr bool MF16 = F16 || FP8;              // operand type of the matrix instructions
   static constexpr int ROWB = DP * (FP8 ? 1 : 2);       // bytes of a key's row in shared memory
   static constexpr int CPR = ROWB / 16;                 // 16-byte units of it
   static constexpr int TILE = BN * ROWB;                // K or V
   // two blocks an SM (head size 256: one), the more bytes in flight the better
-  static constexpr int STAGES = FP8 ? (DP == 64 ? 8 : DP == 128 ? (RW == 4 ? 5 : 6) : 3)
+  static constexpr int STAGES = FP8 ? (DP == 64 ? 8 : DP == 128 ? (RW == 4 ? 5 : 6) : 4)
                                     : (DP == 64 ? 6 : DP == 128 ? (RW == 4 ? 2 : 3) : 2);
   static constexpr int MR = 16 * RW;                    // rows a block
-  static constexpr int KW = 4 / RW;                     // warps that share a tile's keys
+  static constexpr int KW = NW / RW;                    // warps that share a tile's keys
   static constexpr int WN = BN / KW;                    // keys a warp
   static constexpr int QROW = DP * 2 + 16;              // bytes of a query row (padded: no bank conflicts)
   static constexpr int RING = STAGES * 2 * TILE;
   static constexpr int OFFS = STAGES + 1;               // slot offsets are found one tile further ahead
-  static constexpr int SMEM = RING + MR * QROW + OFFS * BN * 8 + OFFS * 2 * 4 + MR * 4 + 64 * 2 * 4 + 64;
+  static constexpr int SMEM = RING + MR * QROW + OFFS * BN * 8 + OFFS * 2 * 4 + MR * 4 + NW * 16 * 2 * 4 + NW * 8 + 32;
   static constexpr float SHIFT = MF16 ? 15.0f : 0.0f;   // weights are scaled by 2^SHIFT
-  static_assert(64 * DP * 4 <= RING, "the warps' outputs fit the drained ring");
+  static_assert(NW * 16 * DP * 4 <= RING, "the warps' outputs fit the drained ring");
 };
 
-template <bool F16, int KV, int DP, int RW>
-__global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_kernel(const AttnParams p) {
-  using C = Cfg<F16, KV, DP, RW>;
+template <bool F16, int KV, int DP, int RW, int NW>
+__global__ void __launch_bounds__(NW * 32, DP == 256 ? 1 : 2) paged_attention_kernel(const AttnParams p) {
+  using C = Cfg<F16, KV, DP, RW, NW>;
+  constexpr int THREADS = C::THREADS;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t *ring = smem;
   uint8_t *s_q = ring + C::RING;
   long long *s_off = reinterpret_cast<long long *>(s_q + C::MR * C::QROW);
   int *s_bad = reinterpret_cast<int *>(s_off + C::OFFS * BN);   // [OFFS][2]
   float *s_qscale = reinterpret_cast<float *>(s_bad + C::OFFS * 2);
-  float *s_base = s_qscale + C::MR;                             // [4 warps][16 rows]
-  float *s_sum = s_base + 64;
-  long long *s_scan = reinterpret_cast<long long *>(s_sum + 64);  // 4 warps' totals, then found request and its prefix
+  float *s_base = s_qscale + C::MR;                             // [NW warps][16 rows]
+  float *s_sum = s_base + NW * 16;
+  long long *s_scan = reinterpret_cast<long long *>(s_sum + NW * 16);  // NW warps' totals, then found request and its prefix
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, tg = lane & 3;
   const int rw = warp / C::KW, kw = warp % C::KW;
@@ -705,7 +717,7 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ---- this block's share of the line of units
-  const Share sh = find_share<C::MR>(p, s_scan, blockIdx.x, gridDim.x);
+  const Share sh = find_share<C::MR, NW>(p, s_scan, blockIdx.x, gridDim.x);
   if (p.zero_rest) zero_rest(p, blockIdx.x, gridDim.x);
   if (sh.r < 0) return;
   const long long c = blockIdx.x, u_end = sh.u_end;
@@ -807,15 +819,26 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
 #pragma unroll
       for (int s = 0; s < C::STAGES; s++) put_offset(s, offs[s], bads[s]);
     }
-    // query rows
-    for (int i = tid; i < C::MR * (DP / 8); i += THREADS) {
-      const int row = i / (DP / 8), cu = i % (DP / 8);
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (row < rows && cu * 8 < p.d) {
-        const int qr = row0 + row, tok = rq.start + qr / p.group, head = h * p.group + qr % p.group;
-        v = __ldg(reinterpret_cast<const uint4 *>(p.q + (int64_t)tok * p.q_tok + (int64_t)head * p.q_head + cu * 8));
+    // query rows, four units a thread in flight
+    constexpr int QU = C::MR * (DP / 8), QN = 4;
+    static_assert(QU % (THREADS * QN) == 0, "whole rounds");
+#pragma unroll 1
+    for (int i0 = tid; i0 < QU; i0 += THREADS * QN) {
+      uint4 v[QN];
+#pragma unroll
+      for (int k = 0; k < QN; k++) {
+        const int i = i0 + k * THREADS, row = i / (DP / 8), cu = i % (DP / 8);
+        v[k] = make_uint4(0, 0, 0, 0);
+        if (row < rows && cu * 8 < p.d) {
+          const int qr = row0 + row, tok = qr / p.group, head = h * p.group + qr - tok * p.group;
+          v[k] = __ldg(reinterpret_cast<const uint4 *>(p.q + (int64_t)(rq.start + tok) * p.q_tok + (int64_t)head * p.q_head + cu * 8));
+        }
       }
-      *reinterpret_cast<uint4 *>(s_q + row * C::QROW + cu * 16) = v;
+#pragma unroll
+      for (int k = 0; k < QN; k++) {
+        const int i = i0 + k * THREADS;
+        *reinterpret_cast<uint4 *>(s_q + i / (DP / 8) * C::QROW + i % (DP / 8) * 16) = v[k];
+      }
     }
     __syncthreads();
 #pragma unroll
@@ -824,7 +847,7 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
       cp_commit();
     }
     if constexpr (C::FP8 && !F16) {           // bf16 rows to f16, the largest value in [1, 2)
-      for (int row = warp; row < C::MR; row += 4) {
+      for (int row = warp; row < C::MR; row += NW) {
         uint32_t *w = reinterpret_cast<uint32_t *>(s_q + row * C::QROW);
         float a = 0.0f;
         for (int i = lane; i < DP / 2; i += 32)
@@ -1039,7 +1062,7 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
 #pragma unroll
       for (int x = 0; x < 4; x++) odd |= !(fabsf(o[i][x]) < INFINITY);
     const bool careful = __syncthreads_or(odd);
-    float *s_o = reinterpret_cast<float *>(ring);  // [4 warps][16 rows][DP]
+    float *s_o = reinterpret_cast<float *>(ring);  // [NW warps][16 rows][DP]
     if (!careful) {
       float *o0 = s_o + (warp * 16 + g) * DP, *o1 = o0 + 8 * DP;
       if constexpr (C::FP8) {
@@ -1062,7 +1085,7 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
         s_sum[warp * 16 + g + 8] = l1;
       }
     } else {
-      for (int row = warp; row < rows; row += 4) {
+      for (int row = warp; row < rows; row += NW) {
         const int qr = row0 + row, tok = qr / p.group;
         float m, l, ov[DP / 32];
         careful_row<F16, KV, DP, BN>(p, r, rq.start + tok, h * p.group + qr % p.group, rq.first + tok, tl, t_begin, t_end, m, l, ov);
@@ -1121,17 +1144,18 @@ __global__ void __launch_bounds__(THREADS, DP == 256 ? 1 : 2) paged_attention_ke
 struct Variant {
   void (*main)(AttnParams);
   void (*merge)(AttnParams);
-  int smem, per_sm, rows;
+  int threads, smem, per_sm, rows;
   bool few;
 };
 template <bool F16, int KV, int DP, int NG>
 Variant few() {
   using C = Few<F16, KV, DP, NG>;
-  return {paged_few_kernel<F16, KV, DP, NG>, paged_merge_kernel<F16, DP, C::MR>, C::SMEM, C::PER_SM, C::MR, true};
+  return {paged_few_kernel<F16, KV, DP, NG>, paged_merge_kernel<F16, DP, C::MR>, THREADS, C::SMEM, C::PER_SM, C::MR, true};
 }
-template <bool F16, int KV, int DP>
+template <bool F16, int KV, int DP, int RW = 4, int NW = 4>
 Variant many() {
-  return {paged_attention_kernel<F16, KV, DP, 4>, paged_merge_kernel<F16, DP, 64>, Cfg<F16, KV, DP, 4>::SMEM, DP == 256 ? 1 : 2, 64, false};
+  using C = Cfg<F16, KV, DP, RW, NW>;
+  return {paged_attention_kernel<F16, KV, DP, RW, NW>, paged_merge_kernel<F16, DP, C::MR>, C::THREADS, C::SMEM, DP == 256 ? 1 : 2, C::MR, false};
 }
 // `rows`: query rows of the longest request (a request with more is served in several row tiles).
 template <bool F16, int KV>
@@ -1148,7 +1172,11 @@ Variant pick(int dp, int64_t rows) {
            : rows <= 16 ? few<F16, KV, 128, 2>()
            : rows <= 32 ? few<F16, KV, 128, 4>()
                         : many<F16, KV, 128>();
-  return rows <= 8 ? few<F16, KV, 256, 1>() : rows <= 16 ? few<F16, KV, 256, 2>() : many<F16, KV, 256>();
+  return rows <= 8    ? few<F16, KV, 256, 1>()
+         : rows <= 16 ? few<F16, KV, 256, 2>()
+         : rows <= 32 ? many<F16, KV, 256, 2, 8>()
+         : rows <= 64 ? many<F16, KV, 256, 4, 8>()
+                      : many<F16, KV, 256, 8, 8>();
 }
 Variant variant_for(bool f16, int cache_dtype, int dp, int64_t rows) {
   if (cache_dtype == FP8B200_E4M3) return f16 ? pick<true, FP8B200_E4M3>(dp, rows) : pick<false, FP8B200_E4M3>(dp, rows);
@@ -1275,7 +1303,7 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
   if (int rc = launch_attributes((const void *)v.merge, 0)) return rc;
   const int grid = current_sm_count() * v.per_sm;
   p.line_heads = v.few && n_kv_heads <= grid / 4 ? 1 : n_kv_heads;
-  launch_dependent(v.main, dim3((unsigned)grid), THREADS, v.smem, (cudaStream_t)stream, p);
+  launch_dependent(v.main, dim3((unsigned)grid), v.threads, v.smem, (cudaStream_t)stream, p);
   p.blocks = grid;
   launch_dependent(v.merge, dim3((unsigned)current_sm_count(), (unsigned)std::max(1, v.rows / 16)), MERGE_THREADS, 0, (cudaStream_t)stream, p);
   count_launch(2);

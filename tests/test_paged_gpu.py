@@ -379,6 +379,22 @@ def test_attention_heads(nat, x, cache, kind, hq, hk, d, page):
     check(nat, build(new, kv, hq, hk, d, page, x, cache, seed=hq + d))
 
 
+@pytest.mark.parametrize("x,cache", TYPES)
+@pytest.mark.parametrize("new,window", [(2, 0), (3, 70), (4, 0), (5, 0), (8, 100), (9, 0), (16, 0), (17, 60), (33, 0)])
+def test_attention_wide_heads_by_rows(nat, x, cache, new, window):
+    """Head sizes above 128, eight heads a group: 16, 24, 32, 40, 64, 72, 128, 136 and 264 rows a request."""
+    s = build([new, 1, new], [new + 700, 65, new], 8, 1, 256, 24, x, cache, seed=new)
+    check(nat, s, window=window, sinks=3 if window else 0, max_new=new)
+
+
+@pytest.mark.parametrize("new", [3, 8, 17])
+def test_attention_wide_heads_many_requests(nat, new):
+    """More requests than the block that looks for its share has threads."""
+    n = 300
+    s = build([new] * n, [new + r % 70 for r in range(n)], 8, 1, 256, 16, BF16, E4M3, seed=new)
+    check(nat, s, max_new=new)
+
+
 @pytest.mark.parametrize("x,cache", [(BF16, BF16), (BF16, E4M3)])
 @pytest.mark.parametrize("kind", list(LENS))
 @pytest.mark.parametrize("window,sinks", [(1, 0), (5, 3), (64, 0), (100, 64), (100, 130), (63, 1), (1500, 4), (10 ** 9, 7), (300, 10 ** 9)])
