@@ -279,6 +279,8 @@ int fp8b200_gemm_16bit(const void *A, const void *B, int dtype, int64_t lda, int
  *     page * page_size + position % page_size, -1 where it has no page
  *   tokens from cu_new[requests] on: position 0, slot -1
  *   free_head_out[0] = free_head + sum of add (beyond n_free: the pool is short)
+ * add counts columns beyond table_cols and pages that only tokens behind
+ * `tokens` open, too; those are passed over in the list and no row holds them.
  * `tokens`: rows of positions / slots, at least the sum of new. free_head may
  * be NULL (0). Lengths below zero count as zero. At most 16384 requests; sums
  * of lengths below 2^31.
@@ -288,6 +290,23 @@ int fp8b200_paged_slots(const int32_t *cached_lens, const int32_t *new_lens, int
                         const int32_t *free_pages, int64_t n_free, const int32_t *free_head, int64_t page_size,
                         int64_t tokens, int32_t *cu_new, int32_t *kv_lens, int32_t *positions,
                         int64_t *slots, int32_t *free_head_out, void *stream);
+
+/*
+ * The same for a cache that keeps account of its pages from step to step: a
+ * page is taken only for a column that the table has and a token that is
+ * placed, and a column that has its page keeps it when lengths are taken back.
+ *   new_r  = what of the new tokens fits into `tokens` rows (the others are not
+ *            added: cu_new, kv_lens and the pages do not count them)
+ *   have_r = min(max(held[r], ceil(cached_r / page_size)), table_cols)
+ *   add_r  = max(min(ceil((cached_r + new_r) / page_size), table_cols) - have_r, 0)
+ *   held_out[r] = have_r + the columns of add_r that found a page
+ * held: the leading columns of each row that have had a page (0 at first).
+ */
+int fp8b200_paged_step(const int32_t *cached_lens, const int32_t *new_lens, const int32_t *held, int64_t requests,
+                       int32_t *block_table, int64_t table_ld, int64_t table_cols, const int32_t *free_pages,
+                       int64_t n_free, const int32_t *free_head, int64_t page_size, int64_t tokens, int32_t *cu_new,
+                       int32_t *kv_lens, int32_t *positions, int64_t *slots, int32_t *held_out,
+                       int32_t *free_head_out, void *stream);
 
 /*
  * Rotary embedding of a step's q and k and the write of its k and v into the

@@ -37,6 +37,17 @@ __device__ __forceinline__ void wait_prior() { asm volatile("griddepcontrol.wait
 // entries before have_r are only read, entries from have_r on only written.
 // Bound by latency: 2.4 us for one request, 4.8 us for 300 prompts with 124468
 // rows (in a graph), of which the scan over 300 lengths and the launch are most.
+//
+// HELD is the form for a cache that keeps account of its pages from step to
+// step (PagedKVCache): held_r is the number of leading columns of row r that
+// have had a page, and
+//   new_r  = what of the new tokens still fits into `tokens` rows
+//   have_r = min(max(held_r, ceil(cached_r / P)), columns)
+//   add_r  = max(min(ceil((cached_r + new_r) / P), columns) - have_r, 0)
+// so a page is only taken for a column that exists and a token that is placed,
+// and one that the row still holds (lengths were taken back) serves again. Every
+// new column then begins with a placed token, which writes its entry. new_r
+// needs the tokens' running sum, so the pages are summed in a second scan.
 constexpr int SL_THREADS = 512;
 constexpr int SL_MAX_REQUESTS = 16384;  // two int32 a request in shared memory
 
@@ -54,8 +65,27 @@ struct SlotsParams {
   int32_t *cu, *kv, *positions;
   int64_t *slots;
   int32_t *head_out;
+  const int32_t *held;                    // HELD
+  int32_t *held_out;
 };
 
+__device__ __forceinline__ int pages_for(int64_t n, int page) { return (int)((n + page - 1) / page); }
+
+// Inclusive sum over the block's threads; s has a place a warp.
+__device__ __forceinline__ int block_sum(int v, int *s) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int a = __shfl_up_sync(~0u, v, d);
+    if (lane >= d) v += a;
+  }
+  if (lane == 31) s[warp] = v;
+  __syncthreads();
+  for (int w = 0; w < warp; w++) v += s[w];
+  return v;
+}
+
+template <bool HELD>
 __global__ void __launch_bounds__(SL_THREADS) slots_kernel(const SlotsParams p) {
   extern __shared__ int s_mem[];
   int *s_cu = s_mem;                      // [requests + 1] first token of each request
@@ -63,53 +93,60 @@ __global__ void __launch_bounds__(SL_THREADS) slots_kernel(const SlotsParams p) 
   __shared__ int s_tok[SL_THREADS / 32], s_pg[SL_THREADS / 32];
   launch_dependents();
   wait_prior();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x;
   const int head = p.free_head ? *p.free_head : 0;
+  // columns of request r that have a page already, of c cached and n new tokens
+  auto columns = [&](int r, int c, int n, int &have) {
+    have = pages_for(c, p.page);
+    int need = pages_for((int64_t)c + n, p.page);
+    if constexpr (HELD) {
+      have = min(max(have, p.held[r]), p.table_cols);
+      need = max(min(need, p.table_cols), have);
+    }
+    return need - have;
+  };
   // each thread a contiguous run of requests; lengths below zero count as zero
   const int run = (p.requests + SL_THREADS - 1) / SL_THREADS;
   const int r0 = min(tid * run, p.requests), r1 = min(r0 + run, p.requests);
-  int tok = 0, pg = 0;
+  int tok = 0, pg = 0, have;
   for (int r = r0; r < r1; r++) {
     const int c = max(p.cached[r], 0), n = max(p.fresh[r], 0);
     tok += n;
-    pg += (int)(((int64_t)c + n + p.page - 1) / p.page - ((int64_t)c + p.page - 1) / p.page);
+    if constexpr (!HELD) pg += columns(r, c, n, have);
   }
-  int itok = tok, ipg = pg;               // inclusive scan over the warp, then over the warps
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int a = __shfl_up_sync(~0u, itok, d), b = __shfl_up_sync(~0u, ipg, d);
-    if (lane >= d) {
-      itok += a;
-      ipg += b;
+  int ctok = block_sum(tok, s_tok) - tok;
+  auto placed = [&](int n) { return HELD ? min(n, max(p.tokens - ctok, 0)) : n; };  // of n tokens from row ctok on
+  if constexpr (HELD) {
+    const int first = ctok;
+    for (int r = r0; r < r1; r++) {
+      const int c = max(p.cached[r], 0), n = max(p.fresh[r], 0);
+      pg += columns(r, c, placed(n), have);
+      ctok += n;
     }
+    ctok = first;
   }
-  if (lane == 31) {
-    s_tok[warp] = itok;
-    s_pg[warp] = ipg;
-  }
-  __syncthreads();
-  int btok = 0, bpg = 0;
-  for (int w = 0; w < warp; w++) {
-    btok += s_tok[w];
-    bpg += s_pg[w];
-  }
-  int ctok = btok + itok - tok, cpg = bpg + ipg - pg;
+  int cpg = block_sum(pg, s_pg) - pg;
+  auto offset = [&]() { return HELD ? min(ctok, p.tokens) : ctok; };
   const bool writer = blockIdx.x == 0;
   for (int r = r0; r < r1; r++) {
-    const int c = max(p.cached[r], 0), n = max(p.fresh[r], 0);
-    s_cu[r] = ctok;
+    const int c = max(p.cached[r], 0), n = max(p.fresh[r], 0), add = columns(r, c, placed(n), have);
+    s_cu[r] = offset();
     s_base[r] = cpg;
     if (writer) {
-      p.cu[r] = ctok;
-      p.kv[r] = c + n;
+      p.cu[r] = offset();
+      p.kv[r] = c + placed(n);
+      if constexpr (HELD) {               // once the list is used up, columns get no page
+        const int64_t left = p.n_free - ((int64_t)head + cpg);
+        p.held_out[r] = have + (int)min((int64_t)add, max(left, (int64_t)0));
+      }
     }
     ctok += n;
-    cpg += (int)(((int64_t)c + n + p.page - 1) / p.page - ((int64_t)c + p.page - 1) / p.page);
+    cpg += add;
   }
   if (tid == SL_THREADS - 1) {            // its run ends with the last request
-    s_cu[p.requests] = ctok;
+    s_cu[p.requests] = offset();
     if (writer) {
-      p.cu[p.requests] = ctok;
+      p.cu[p.requests] = offset();
       *p.head_out = head + cpg;
     }
   }
@@ -129,7 +166,8 @@ __global__ void __launch_bounds__(SL_THREADS) slots_kernel(const SlotsParams p) 
       const int c = max(p.cached[lo], 0);
       pos = c + (t - s_cu[lo]);
       const int col = pos / p.page, off = pos - col * p.page;
-      const int have = (int)(((int64_t)c + p.page - 1) / p.page);
+      int have;
+      columns(lo, c, 0, have);
       int page = -1;
       if (col >= 0 && col < p.table_cols) {
         int32_t *e = p.table + (int64_t)lo * p.table_ld + col;
@@ -345,41 +383,68 @@ cudaError_t launch_pdl(void (*kernel)(P), int grid, int threads, int smem, cudaS
 }  // namespace paged
 }  // namespace fp8b200
 
-extern "C" int fp8b200_paged_slots(const int32_t *cached_lens, const int32_t *new_lens, int64_t requests,
-                                   int32_t *block_table, int64_t table_ld, int64_t table_cols,
-                                   const int32_t *free_pages, int64_t n_free, const int32_t *free_head, int64_t page_size,
-                                   int64_t tokens, int32_t *cu_new, int32_t *kv_lens, int32_t *positions,
-                                   int64_t *slots, int32_t *free_head_out, void *stream) {
-  using namespace fp8b200;
-  using namespace fp8b200::paged;
-  if (requests < 0 || table_cols < 0 || n_free < 0 || tokens < 0)
-    return set_error(FP8B200_EINVAL, "paged_slots: negative size");
+namespace fp8b200 {
+namespace paged {
+namespace {
+
+// `what` names the entry in messages; HELD: with held and held_out.
+template <bool HELD>
+int launch_slots(const char *what, const int32_t *cached_lens, const int32_t *new_lens, const int32_t *held, int64_t requests,
+                 int32_t *block_table, int64_t table_ld, int64_t table_cols, const int32_t *free_pages, int64_t n_free,
+                 const int32_t *free_head, int64_t page_size, int64_t tokens, int32_t *cu_new, int32_t *kv_lens,
+                 int32_t *positions, int64_t *slots, int32_t *held_out, int32_t *free_head_out, void *stream) {
+  if (requests < 0 || table_cols < 0 || n_free < 0 || tokens < 0) return set_error(FP8B200_EINVAL, "%s: negative size", what);
   if (requests > SL_MAX_REQUESTS)
-    return set_error(FP8B200_EINVAL, "paged_slots: %lld requests, at most %d", (long long)requests, SL_MAX_REQUESTS);
-  if (page_size < 1 || page_size > (1 << 30)) return set_error(FP8B200_EINVAL, "paged_slots: page_size must be in 1 .. 2^30");
+    return set_error(FP8B200_EINVAL, "%s: %lld requests, at most %d", what, (long long)requests, SL_MAX_REQUESTS);
+  if (page_size < 1 || page_size > (1 << 30)) return set_error(FP8B200_EINVAL, "%s: page_size must be in 1 .. 2^30", what);
   if (tokens > INT32_MAX || table_cols > INT32_MAX)
-    return set_error(FP8B200_EINVAL, "paged_slots: more than 2^31 - 1 tokens or table columns");
-  if (table_ld < table_cols) return set_error(FP8B200_EINVAL, "paged_slots: block-table rows overlap");
+    return set_error(FP8B200_EINVAL, "%s: more than 2^31 - 1 tokens or table columns", what);
+  if (table_ld < table_cols) return set_error(FP8B200_EINVAL, "%s: block-table rows overlap", what);
   if (!cu_new || !free_head_out ||
-      (requests && (!cached_lens || !new_lens || !kv_lens || (table_cols && !block_table))) ||
+      (requests && (!cached_lens || !new_lens || !kv_lens || (table_cols && !block_table) || (HELD && (!held || !held_out)))) ||
       (tokens && (!positions || !slots)) || (n_free && !free_pages))
-    return set_error(FP8B200_EINVAL, "paged_slots: null pointer");
+    return set_error(FP8B200_EINVAL, "%s: null pointer", what);
   int dev;
   if (int rc = check_device(&dev)) return rc;
   const int smem = (int)(2 * requests + 1) * 4;
   static std::atomic<uint64_t> raised{0};
   if (smem > 47 * 1024 && !((raised.load() >> dev) & 1)) {
-    if (cudaFuncSetAttribute(slots_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * SL_MAX_REQUESTS + 1) * 4) !=
+    if (cudaFuncSetAttribute(slots_kernel<HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * SL_MAX_REQUESTS + 1) * 4) !=
         cudaSuccess)
-      return check_launch("paged_slots");
+      return check_launch(what);
     raised.fetch_or(1ull << dev);
   }
   SlotsParams p{cached_lens, new_lens, (int)requests, block_table, table_ld, (int)table_cols, free_pages, n_free,
-                free_head, (int)page_size, (int)tokens, cu_new, kv_lens, positions, slots, free_head_out};
+                free_head, (int)page_size, (int)tokens, cu_new, kv_lens, positions, slots, free_head_out, held, held_out};
   const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((tokens + SL_THREADS - 1) / SL_THREADS, current_sm_count()));
-  launch_pdl(slots_kernel, grid, SL_THREADS, smem, (cudaStream_t)stream, p);
+  launch_pdl(slots_kernel<HELD>, grid, SL_THREADS, smem, (cudaStream_t)stream, p);
   count_launch();
-  return check_launch("paged_slots");
+  return check_launch(what);
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace fp8b200
+
+extern "C" int fp8b200_paged_slots(const int32_t *cached_lens, const int32_t *new_lens, int64_t requests,
+                                   int32_t *block_table, int64_t table_ld, int64_t table_cols,
+                                   const int32_t *free_pages, int64_t n_free, const int32_t *free_head, int64_t page_size,
+                                   int64_t tokens, int32_t *cu_new, int32_t *kv_lens, int32_t *positions,
+                                   int64_t *slots, int32_t *free_head_out, void *stream) {
+  return fp8b200::paged::launch_slots<false>("paged_slots", cached_lens, new_lens, nullptr, requests, block_table, table_ld,
+                                             table_cols, free_pages, n_free, free_head, page_size, tokens, cu_new, kv_lens,
+                                             positions, slots, nullptr, free_head_out, stream);
+}
+
+extern "C" int fp8b200_paged_step(const int32_t *cached_lens, const int32_t *new_lens, const int32_t *held, int64_t requests,
+                                  int32_t *block_table, int64_t table_ld, int64_t table_cols, const int32_t *free_pages,
+                                  int64_t n_free, const int32_t *free_head, int64_t page_size, int64_t tokens, int32_t *cu_new,
+                                  int32_t *kv_lens, int32_t *positions, int64_t *slots, int32_t *held_out,
+                                  int32_t *free_head_out, void *stream) {
+  if (held && held == held_out) return fp8b200::set_error(FP8B200_EINVAL, "paged_step: held and held_out must not overlap");
+  return fp8b200::paged::launch_slots<true>("paged_step", cached_lens, new_lens, held, requests, block_table, table_ld,
+                                            table_cols, free_pages, n_free, free_head, page_size, tokens, cu_new, kv_lens,
+                                            positions, slots, held_out, free_head_out, stream);
 }
 
 extern "C" int fp8b200_rope_write_paged(const void *qkv, int dtype, int64_t tokens, int64_t ld, int n_q_heads,

@@ -63,6 +63,7 @@ def _declare(L):
         "fp8b200_linear_fp8w": [vp, i32, i64, vp, i32, i64, i64, i64, i64, vp, i32, vp, i32, vp, i32, i64, vp],
         "fp8b200_gemm_16bit": [vp, vp, i32, i64, i64, i64, i64, i64, vp, i32, vp, i32, vp, i32, i64, vp],
         "fp8b200_paged_slots": [vp, vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp],
+        "fp8b200_paged_step": [vp, vp, vp, i64, vp, i64, i64, vp, i64, vp, i64, i64, vp, vp, vp, vp, vp, vp, vp],
         "fp8b200_rope_write_paged": [vp, i32, i64, i64, i32, i32, i32, vp, vp, i64, vp, vp, vp, vp, vp, i32,
                                      i64, i64, i64, i64, i64, vp, i32, vp, i32, vp],
         "fp8b200_paged_attention": [vp, i32, i64, i64, i64, i32, i32, i32, vp, vp, i32, i64, i64, i64, i64, i64,

@@ -130,6 +130,22 @@ def _check_slots(cached_lens, new_lens, block_table, free_pages, page_size, num_
         raise RuntimeError(f"{what}: free_head must be one int32 value on {dev}")
 
 
+def _slots_table_ld(cached_lens, new_lens, block_table, free_pages, page_size, num_tokens, free_head) -> int:
+    """The row stride of the block table, once the arguments have passed."""
+    dev, n = cached_lens.device, cached_lens.numel()
+    rows, cols = block_table.shape if block_table.dim() == 2 else (-1, 0)
+    ld = block_table.stride(0) if n > 1 and rows == n else cols
+    if not (cached_lens.dtype is new_lens.dtype is block_table.dtype is free_pages.dtype is torch.int32
+            and cached_lens.dim() == new_lens.dim() == free_pages.dim() == 1 and new_lens.numel() == n == rows
+            and cached_lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous()
+            and (cols <= 1 or block_table.stride(1) == 1) and ld >= cols and n <= MAX_REQUESTS
+            and new_lens.device == block_table.device == free_pages.device == dev and page_size >= 1 and num_tokens >= 0
+            and (free_head is None
+                 or (free_head.dtype is torch.int32 and free_head.numel() == 1 and free_head.device == dev))):
+        _check_slots(cached_lens, new_lens, block_table, free_pages, page_size, num_tokens, free_head)
+    return ld
+
+
 def paged_slots(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_pages: torch.Tensor,
                 page_size: int, num_tokens: int, free_head: torch.Tensor | None = None,
                 outputs=slots_outputs) -> PagedStep:
@@ -148,26 +164,32 @@ def paged_slots(cached_lens: torch.Tensor, new_lens: torch.Tensor, block_table: 
     Returns a PagedStep. Once the list of free pages is used up, the requests
     after it get table entries of -1 and slots of -1 (`rope_write_paged` skips
     them); the returned free_head is then beyond free_pages.numel(). A token
-    beyond the table's columns also gets slot -1. Lengths below zero count as
-    zero; sums of lengths stay below 2^31."""
-    dev = cached_lens.device
-    n = cached_lens.numel()
-    rows, cols = block_table.shape if block_table.dim() == 2 else (-1, 0)
-    ld = block_table.stride(0) if n > 1 and rows == n else cols
-    if not (cached_lens.dtype is new_lens.dtype is block_table.dtype is free_pages.dtype is torch.int32
-            and cached_lens.dim() == new_lens.dim() == free_pages.dim() == 1 and new_lens.numel() == n == rows
-            and cached_lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous()
-            and (cols <= 1 or block_table.stride(1) == 1) and ld >= cols and n <= MAX_REQUESTS
-            and new_lens.device == block_table.device == free_pages.device == dev and page_size >= 1 and num_tokens >= 0
-            and (free_head is None
-                 or (free_head.dtype is torch.int32 and free_head.numel() == 1 and free_head.device == dev))):
-        _check_slots(cached_lens, new_lens, block_table, free_pages, page_size, num_tokens, free_head)
+    beyond the table's columns also gets slot -1. free_head counts every page
+    that the lengths ask for: those for columns that the table lacks and those
+    that only tokens without a row open are passed over, and no row holds them
+    (PagedKVCache.step takes neither). Lengths below zero count as zero; sums of
+    lengths stay below 2^31."""
+    dev, n = cached_lens.device, cached_lens.numel()
+    ld = _slots_table_ld(cached_lens, new_lens, block_table, free_pages, page_size, num_tokens, free_head)
     step = outputs(n, num_tokens, dev)
     _launch(dev, L.lib().fp8b200_paged_slots, "paged_slots", cached_lens.data_ptr(), new_lens.data_ptr(), n,
             block_table.data_ptr(), ld, block_table.shape[1], free_pages.data_ptr(), free_pages.numel(),
             None if free_head is None else free_head.data_ptr(), page_size, num_tokens, step.cu_new.data_ptr(),
             step.kv_lens.data_ptr(), step.positions.data_ptr(), step.slots.data_ptr(), step.free_head.data_ptr())
     return step
+
+
+def _step_slots(cache: PagedKVCache, new_lens: torch.Tensor, num_tokens: int) -> tuple[PagedStep, torch.Tensor]:
+    """(step, held) of a cache's step: paged_slots with its account of the pages."""
+    lens, table, free = cache.lens, cache.block_table, cache.free_pages
+    ld = _slots_table_ld(lens, new_lens, table, free, cache.page_size, num_tokens, cache.free_head)
+    n, dev = lens.numel(), lens.device
+    step, held = slots_outputs(n, num_tokens, dev), torch.empty_like(cache.held)
+    _launch(dev, L.lib().fp8b200_paged_step, "paged_slots", lens.data_ptr(), new_lens.data_ptr(), cache.held.data_ptr(), n,
+            table.data_ptr(), ld, table.shape[1], free.data_ptr(), free.numel(), cache.free_head.data_ptr(),
+            cache.page_size, num_tokens, step.cu_new.data_ptr(), step.kv_lens.data_ptr(), step.positions.data_ptr(),
+            step.slots.data_ptr(), held.data_ptr(), step.free_head.data_ptr())
+    return step, held
 
 
 def _check_write(qkv, cos, sin, positions, slots, k_cache, v_cache, n_q_heads) -> None:
@@ -334,7 +356,12 @@ class PagedKVCache:
     caches' scales, one value or one per head (None: 1). All layers share the
     pages' numbering. Slots hold nothing until they are written; the operators
     never read such a slot. `step` only launches kernels, so it can be part of
-    a captured step."""
+    a captured step.
+
+    lens may be lowered in place between steps (drafted tokens that were not
+    taken): the pages stay with their request and serve the tokens that come
+    instead. A request beyond max_len (rounded up to whole pages) takes no more
+    pages; its further tokens get slot -1."""
 
     def __init__(self, layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, requests: int, max_len: int,
                  dtype: torch.dtype, device, k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None):
@@ -349,15 +376,17 @@ class PagedKVCache:
         self.k_scale, self.v_scale = k_scale, v_scale
         self.block_table = torch.full((requests, -(-max_len // page_size)), -1, dtype=torch.int32, device=device)
         self.lens = torch.zeros(requests, dtype=torch.int32, device=device)
+        self.held = torch.zeros(requests, dtype=torch.int32, device=device)  # leading columns of each row that have had a page
         self.free_pages = torch.arange(pages, dtype=torch.int32, device=device)
         self.free_head = torch.zeros(1, dtype=torch.int32, device=device)
 
     def step(self, new_lens: torch.Tensor, num_tokens: int) -> PagedStep:
         """Pages and slots for new_lens (requests,) int32 more tokens; the lengths
-        move on. See paged_slots, also for a pool that runs short."""
-        s = paged_slots(self.lens, new_lens, self.block_table, self.free_pages, self.page_size, num_tokens, self.free_head)
-        self.lens.copy_(s.kv_lens)
-        self.free_head.copy_(s.free_head)
+        move on. Tokens that do not fit into num_tokens rows are not added. See
+        paged_slots, also for a pool that runs short: a token that found no
+        page is lost for good."""
+        s, held = _step_slots(self, new_lens, num_tokens)
+        torch._foreach_copy_([self.lens, self.held, self.free_head], [s.kv_lens, held, s.free_head])
         return s
 
     def release(self, request: int) -> None:
@@ -374,3 +403,4 @@ class PagedKVCache:
         self.free_head.fill_(head - n)
         row.fill_(-1)
         self.lens[request] = 0
+        self.held[request] = 0
