@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(NW * 32, DP == 256 ? 1 : 2) paged_attention_ke
     const int rows = (int)min((long long)C::MR, (long long)rq.n * p.group - row0);
     const int pos_lo = rq.first + row0 / p.group, pos_hi = rq.first + (row0 + rows - 1) / p.group;
     // of the request's tiles, those that this row tile sees
-    const int live_from = p.window > 0 ? max(0, pos_lo - p.window + 1) / BN : 0;
+    const int live_from = p.window > 0 ? (int)(max((long long)pos_lo - p.window + 1, 0ll) / BN) : 0;
     const int live_sinks = p.window > 0 ? (int)(((long long)p.sinks + BN - 1) / BN) : 0;
     auto live = [&](int i) {
       const int t = tl.at(i);
