@@ -411,7 +411,10 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
   int *s_start = reinterpret_cast<int *>(smem);  // [requests + 1]
   long long *s_sum = reinterpret_cast<long long *>(smem + C::OFF_PLAN);                 // [warps]
   long long(*s_found)[4] = reinterpret_cast<long long(*)[4]>(s_sum + TC_THREADS / 32);  // cut, place, units before it, request
-  for (int r = tid; r <= p.requests; r += TC_THREADS) s_start[r] = r < p.requests ? load_request(p, r).start : p.tokens;
+  for (int r = tid; r <= p.requests; r += TC_THREADS) {
+    s_start[r] = r < p.requests ? load_request(p, r).start : p.tokens;
+    fence_async();  // Q and K arrive over it through TMA
+  }
   if (tid < 2) s_found[tid][0] = -1;
   __syncthreads();
   const int places = p.requests == 0 ? 0 : place(p, min(max(__ldg(p.cu + p.requests), 0), p.tokens), p.requests);
@@ -655,12 +658,9 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
               if (filled >= RING) ok = bar_wait(C::FP8 ? raw_empty(at) : kv_empty(at), (turns & 1) ^ 1, s_failed, 10);
               ok = __all_sync(~0u, ok);
               if (!ok) break;
-              if (lane == 0) {
-                if (keys) {
+              if (lane == 0 && keys) {
 #pragma unroll
-                  for (int e = 1; e < 4; e++) s_hide[(number % HIDE_RING) * 4 + e] = 0;
-                }
-                bar_expect(bar, C::FP8 ? C::RAW : C::TILE);
+                for (int e = 1; e < 4; e++) s_hide[(number % HIDE_RING) * 4 + e] = 0;
               }
             }
             if (lane == 0 && keys) s_hide[(number % HIDE_RING) * 4 + (b0 >> 5)] = hide;  // bit b: box b
@@ -681,6 +681,9 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
             }
           }
           if (!ok) break;
+          // The bytes may arrive before they are expected; the mask's words all stand before this arrival, which the
+          // softmax's wait goes back to.
+          if (lane == 0) bar_expect(bar, C::FP8 ? C::RAW : C::TILE);
         }
         __syncwarp();
         if (lane == 0) bar_arrive(seg_empty + 8 * (segs % SEGS));

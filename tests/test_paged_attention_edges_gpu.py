@@ -17,3 +17,23 @@ def test_largest_window_with_rows_before_the_first_key(nat, x, cache, hq, hk, d,
     """More new tokens than the length says: the first rows lie before position 0, the others see all keys."""
     got = check(nat, build(new, kv, hq, hk, d, 16, x, cache, seed=d + new[0]), window=window, sinks=sinks, max_new=max(new))
     assert bool((got[new[0] - 1] != 0).any())
+
+
+@pytest.mark.parametrize("x,cache", [(BF16, BF16), (F16, F16), (BF16, E4M3), (F16, E5M2)])
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 64), (4, 1, 128)])
+@pytest.mark.parametrize("page", [1, 2, 6, 7, 16, 200])
+def test_page_masks_of_many_rows(nat, x, cache, hq, hk, d, page):  # noqa: F811
+    """Table entries outside the pool at every third page, and in runs: with pages of odd or twice odd slots a key
+    tile's mask has more than one word. More than 64 rows a request, tiles before, on and behind the diagonal."""
+    new, kv = [90, 300, 2], [700, 300, 40]
+    s = build(new, kv, hq, hk, d, page, x, cache, seed=page)
+    t = s["table"]
+    bad = torch.tensor([-1, s["k"].shape[0], 2 ** 31 - 1, -2 ** 31], dtype=torch.int32, device="cuda")
+    cols = torch.arange(t.shape[1], device="cuda")
+    hit = (cols % 3 == 1) | ((cols >= 40) & (cols < 75)) | (cols % 97 > 90)
+    t[:2, hit] = bad[cols[hit] % 4]
+    check(nat, s, max_new=300)
+    check(nat, s, window=100, sinks=9, max_new=300)
+    t[1] = -1
+    got = check(nat, s, max_new=300)
+    assert int((got[90:390] != 0).sum()) == 0
