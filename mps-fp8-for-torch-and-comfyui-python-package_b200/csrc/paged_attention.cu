@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, NG>::PER_SM)) paged
     cp_wait<0>();
 
     // ---- the segment's end: the warps' results, a row group at a time, through the drained rings
-    bool odd = false;                                       // infinities or NaN: see careful_row
+    bool odd = false;                                       // infinities or NaN: see odd_rows
 #pragma unroll
     for (int ng = 0; ng < NG; ng++) {
 #pragma unroll
@@ -587,41 +587,20 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, NG>::PER_SM)) paged
     for (int mg = 0; mg < (NG + 1) / 2; mg++) {
       if (mg * 16 < rows) {
         if (mg) __syncthreads();
-        if (!careful) {
 #pragma unroll
-          for (int half = 0; half < (NG > 1 ? 2 : 1); half++) {
-            const int ng = mg * 2 + half;
-            if (ng >= NG) continue;
-            float *x0 = s_o + (warp * 16 + half * 8 + 2 * tg) * C::SO, *x1 = x0 + C::SO;
+        for (int half = 0; half < (NG > 1 ? 2 : 1); half++) {
+          const int ng = mg * 2 + half;
+          if (ng >= NG) continue;
+          float *x0 = s_o + (warp * 16 + half * 8 + 2 * tg) * C::SO, *x1 = x0 + C::SO;
 #pragma unroll
-            for (int j = 0; j < DP / 16; j++) {
-              const float(&v)[4] = o[ng][j];
-              if constexpr (C::FP8) {
-                *reinterpret_cast<float2 *>(x0 + j * 16 + 2 * g) = make_float2(v[0], v[2]);
-                *reinterpret_cast<float2 *>(x1 + j * 16 + 2 * g) = make_float2(v[1], v[3]);
-              } else {
-                x0[j * 16 + g] = v[0], x0[j * 16 + g + 8] = v[2];
-                x1[j * 16 + g] = v[1], x1[j * 16 + g + 8] = v[3];
-              }
-            }
-          }
-        } else {
-          for (int row = warp; row < min(16, C::MR); row += 4) {
-            const bool there = mg * 16 + row < rows;
-            float m = -INFINITY, l = 0.0f, ov[DP / 32];
-#pragma unroll
-            for (int k = 0; k < DP / 32; k++) ov[k] = 0.0f;
-            if (there) {
-              const int qr = row0 + mg * 16 + row, tok = qr / p.group;
-              careful_row<F16, KV, DP, BN>(p, r, rq.start + tok, h * p.group + qr % p.group, rq.first + tok, tl, t_begin, t_end, m, l, ov);
-            }
-            for (int w = 0; w < 4; w++) {
-#pragma unroll
-              for (int k = 0; k < DP / 32; k++) s_o[(w * 16 + row) * C::SO + lane + 32 * k] = w == 0 ? ov[k] : 0.0f;
-              if (lane == 0) {
-                s_base[w * C::MR + mg * 16 + row] = w == 0 ? m : -INFINITY;
-                s_sum[w * C::MR + mg * 16 + row] = w == 0 ? l : 0.0f;
-              }
+          for (int j = 0; j < DP / 16; j++) {
+            const float(&v)[4] = o[ng][j];
+            if constexpr (C::FP8) {
+              *reinterpret_cast<float2 *>(x0 + j * 16 + 2 * g) = make_float2(v[0], v[2]);
+              *reinterpret_cast<float2 *>(x1 + j * 16 + 2 * g) = make_float2(v[1], v[3]);
+            } else {
+              x0[j * 16 + g] = v[0], x0[j * 16 + g + 8] = v[2];
+              x1[j * 16 + g] = v[1], x1[j * 16 + g + 8] = v[3];
             }
           }
         }
@@ -639,6 +618,7 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, NG>::PER_SM)) paged
             l += f * s_sum[w * C::MR + at];
             x[0] += f * v.x, x[1] += f * v.y, x[2] += f * v.z, x[3] += f * v.w;
           }
+          if (careful && d4 == 0) s_qscale[at] = l;
           if (begins && ends) {
             if (d4 < p.d) {
               const float inv = l == 0.0f ? 0.0f : vs / l;
@@ -655,6 +635,13 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, NG>::PER_SM)) paged
           }
         }
       }
+    }
+    if (careful) {                                          // each warp looks through its share of the rows
+      __syncthreads();
+      const int row = warp + 4 * lane;
+      const bool mine = lane < C::MR / 4 && row < rows;
+      const SegmentRows<BN> seg_rows{r, rq.start, rq.first, h, row0, tl, t_begin, t_end};
+      odd_rows<F16, KV, DP, BN>(p, seg_rows, row, mine, mine ? s_qscale[row] : 0.0f, begins && ends, part, C::MR, nullptr);
     }
   }
   if (p.zero_rest) zero_rest(p, blockIdx.x, gridDim.x);
@@ -690,6 +677,7 @@ struct Cfg {
   static constexpr int OFFS = STAGES + 1;               // slot offsets are found one tile further ahead
   static constexpr int SMEM = RING + MR * QROW + OFFS * BN * 8 + OFFS * 2 * 4 + MR * 4 + NW * 16 * 2 * 4 + NW * 8 + 32;
   static constexpr float SHIFT = MF16 ? 15.0f : 0.0f;   // weights are scaled by 2^SHIFT
+  static_assert(MR <= NW * 32, "a lane a row");
   static_assert(NW * 16 * DP * 4 <= RING, "the warps' outputs fit the drained ring");
 };
 
@@ -1056,51 +1044,32 @@ __global__ void __launch_bounds__(NW * 32, DP == 256 ? 1 : 2) paged_attention_ke
     l0 += __shfl_xor_sync(~0u, l0, 2);
     l1 += __shfl_xor_sync(~0u, l1, 1);
     l1 += __shfl_xor_sync(~0u, l1, 2);
-    bool odd = false;                         // infinities or NaN: see careful_row
+    bool odd = false;                         // infinities or NaN: see odd_rows
 #pragma unroll
     for (int i = 0; i < DP / 8; i++)
 #pragma unroll
       for (int x = 0; x < 4; x++) odd |= !(fabsf(o[i][x]) < INFINITY);
     const bool careful = __syncthreads_or(odd);
     float *s_o = reinterpret_cast<float *>(ring);  // [NW warps][16 rows][DP]
-    if (!careful) {
-      float *o0 = s_o + (warp * 16 + g) * DP, *o1 = o0 + 8 * DP;
-      if constexpr (C::FP8) {
+    float *o0 = s_o + (warp * 16 + g) * DP, *o1 = o0 + 8 * DP;
+    if constexpr (C::FP8) {
 #pragma unroll
-        for (int u2 = 0; u2 < DP / 16; u2++) {
-          *reinterpret_cast<float4 *>(o0 + u2 * 16 + tg * 4) = make_float4(o[2 * u2][0], o[2 * u2 + 1][0], o[2 * u2][1], o[2 * u2 + 1][1]);
-          *reinterpret_cast<float4 *>(o1 + u2 * 16 + tg * 4) = make_float4(o[2 * u2][2], o[2 * u2 + 1][2], o[2 * u2][3], o[2 * u2 + 1][3]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < DP / 8; j++) {
-          *reinterpret_cast<float2 *>(o0 + j * 8 + tg * 2) = make_float2(o[j][0], o[j][1]);
-          *reinterpret_cast<float2 *>(o1 + j * 8 + tg * 2) = make_float2(o[j][2], o[j][3]);
-        }
-      }
-      if (tg == 0) {
-        s_base[warp * 16 + g] = m0 - C::SHIFT;
-        s_base[warp * 16 + g + 8] = m1 - C::SHIFT;
-        s_sum[warp * 16 + g] = l0;
-        s_sum[warp * 16 + g + 8] = l1;
+      for (int u2 = 0; u2 < DP / 16; u2++) {
+        *reinterpret_cast<float4 *>(o0 + u2 * 16 + tg * 4) = make_float4(o[2 * u2][0], o[2 * u2 + 1][0], o[2 * u2][1], o[2 * u2 + 1][1]);
+        *reinterpret_cast<float4 *>(o1 + u2 * 16 + tg * 4) = make_float4(o[2 * u2][2], o[2 * u2 + 1][2], o[2 * u2][3], o[2 * u2 + 1][3]);
       }
     } else {
-      for (int row = warp; row < rows; row += NW) {
-        const int qr = row0 + row, tok = qr / p.group;
-        float m, l, ov[DP / 32];
-        careful_row<F16, KV, DP, BN>(p, r, rq.start + tok, h * p.group + qr % p.group, rq.first + tok, tl, t_begin, t_end, m, l, ov);
-        const int at = (row >> 4) * C::KW * 16 + (row & 15);  // the row's place in its first key warp
 #pragma unroll
-        for (int i = 0; i < DP / 32; i++) s_o[at * DP + lane + 32 * i] = ov[i];
-        if (lane == 0) {
-          for (int w = 0; w < C::KW; w++) {
-            s_base[at + w * 16] = w == 0 ? m : -INFINITY;
-            s_sum[at + w * 16] = w == 0 ? l : 0.0f;
-          }
-        }
-        for (int w = 1; w < C::KW; w++)
-          for (int i = lane; i < DP; i += 32) s_o[(at + w * 16) * DP + i] = 0.0f;
+      for (int j = 0; j < DP / 8; j++) {
+        *reinterpret_cast<float2 *>(o0 + j * 8 + tg * 2) = make_float2(o[j][0], o[j][1]);
+        *reinterpret_cast<float2 *>(o1 + j * 8 + tg * 2) = make_float2(o[j][2], o[j][3]);
       }
+    }
+    if (tg == 0) {
+      s_base[warp * 16 + g] = m0 - C::SHIFT;
+      s_base[warp * 16 + g + 8] = m1 - C::SHIFT;
+      s_sum[warp * 16 + g] = l0;
+      s_sum[warp * 16 + g + 8] = l1;
     }
     __syncthreads();
     const bool begins = t_begin == 0, ends = t_end == tiles_n;
@@ -1123,6 +1092,7 @@ __global__ void __launch_bounds__(NW * 32, DP == 256 ? 1 : 2) paged_attention_ke
         l += f * s_sum[at + w * 16];
         x[0] += f * v.x, x[1] += f * v.y, x[2] += f * v.z, x[3] += f * v.w;
       }
+      if (careful && d4 == 0) s_qscale[row] = l;
       if (begins && ends) {
         if (d4 < p.d) {
           const float inv = l == 0.0f ? 0.0f : vs / l;
@@ -1137,6 +1107,13 @@ __global__ void __launch_bounds__(NW * 32, DP == 256 ? 1 : 2) paged_attention_ke
           part[C::MR * DP + C::MR + row] = l;
         }
       }
+    }
+    if (careful) {                            // each warp looks through its share of the rows
+      __syncthreads();
+      const int row = warp + NW * lane;
+      const bool mine = lane < C::MR / NW && row < rows;
+      const SegmentRows<BN> seg_rows{r, rq.start, rq.first, h, row0, tl, t_begin, t_end};
+      odd_rows<F16, KV, DP, BN>(p, seg_rows, row, mine, mine ? s_qscale[row] : 0.0f, begins && ends, part, C::MR, nullptr);
     }
   }
 }

@@ -121,6 +121,12 @@ __device__ __forceinline__ int64_t slot_offset(const AttnParams &p, int r, int j
   return (int64_t)page * p.s_page + (int64_t)((uint32_t)j - col * (uint32_t)p.page) * p.s_slot;
 }
 
+constexpr uint64_t WAIT_NS = 10000000000ull;  // the tensor-memory kernel's waits run out that long after the last progress
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
 __device__ __forceinline__ uint32_t saddr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -166,57 +172,326 @@ bool tc_takes(const AttnParams &p);
 int64_t tc_workspace(int dp, int sms);
 int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int sms, uint8_t *workspace, cudaStream_t st);
 
-// One query row over the keys of tiles [t0, t1) of `tiles`, value by value:
-// the way out where a hidden key's infinity or NaN met a zero weight in a
-// matrix product (0 * inf). Hidden keys are not touched here. The warp's
-// lanes hold dims lane, lane + 32, ...; returns the running maximum (log2
-// units) and sum, and the unnormalised output in o.
-template <bool F16, int KV, int DMAX, int BN>
-__device__ __noinline__ void careful_row(const AttnParams &p, int r, int tok, int head, int pos, const Tiles<BN> tiles,
-                                         int t0, int t1, float &m_out, float &l_out, float (&o)[DMAX / 32]) {
-  const int lane = threadIdx.x & 31;
-  const int kh = head / p.group;
-  const uint16_t *q = p.q + (int64_t)tok * p.q_tok + (int64_t)head * p.q_head;
-  const float s2 = p.scale_log2 * (p.ks ? __ldg(p.ks + p.ks_step * kh) : 1.0f);
-  float qv[DMAX / 32];
+// ---- rows whose product came out not finite
+//
+// A hidden key's weight is 0, but 0 times its V's infinity or NaN is NaN and
+// takes a whole output with it. odd_rows puts such rows right at a segment's
+// end, a warp's rows at a time, in two steps:
+//   1. one pass over V alone finds the keys that hold infinities or NaN. What a
+//      row sees of them is its result in that dim, whatever the other keys add
+//      (weights of visible keys are above 0): NaN, or both infinities: NaN; else
+//      the infinity. Rows whose every odd dim is settled so need nothing more.
+//   2. the others (a hidden key's value in the way) are recomputed from their
+//      visible keys alone, CAREFUL rows at a time (careful_rows). Those are at
+//      most the rows whose tiles hold the key and that do not see it.
+// 2048 rows of 32 / 8 heads of 128 over 16049 keys in bf16 (0.50 ms): 1.7 ms with
+// a NaN that all rows of one head see, 2.9 ms with one in each head; 78 ms with
+// one in the last key, which the last 256 rows of a head are recomputed for.
+constexpr int CAREFUL = 4;
+
+// An infinity or NaN among the 16 bytes of cached values.
+template <bool F16, int KV>
+__device__ __forceinline__ bool odd16(const uint4 &v) {
+  constexpr bool BYTES = KV == FP8B200_E4M3 || KV == FP8B200_E5M2;
+  constexpr uint32_t ONES = KV == FP8B200_E4M3 ? 0x7F7F7F7Fu : KV == FP8B200_E5M2 ? 0x7C7C7C7Cu : F16 ? 0x7C007C00u : 0x7F807F80u;
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t hit = 0;
 #pragma unroll
-  for (int i = 0; i < DMAX / 32; i++) {
-    qv[i] = lane + 32 * i < p.d ? to_f32<F16>(__ldg(q + lane + 32 * i)) : 0.0f;
-    o[i] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  for (int t = t0; t < t1; t++) {
-    const int k0 = tiles.at(t) * BN;
-    for (int j = k0; j < k0 + BN; j++) {
-      if (!visible(p, j, pos)) continue;
-      const int64_t off = slot_offset(p, r, j);
-      if (off < 0) continue;
-      const int64_t e = off + (int64_t)kh * p.s_head;
-      float s = 0.0f;
+  for (int i = 0; i < 4; i++) hit |= BYTES ? __vcmpeq4(w[i] & ONES, ONES) : __vcmpeq2(w[i] & ONES, ONES);
+  return hit != 0;
+}
+// 16 values from element `elem` (at 16 bytes' alignment) as floats.
+template <bool F16, int KV>
+__device__ __forceinline__ void load16(const void *base, int64_t elem, float (&f)[16]) {
+  if constexpr (KV == FP8B200_E4M3 || KV == FP8B200_E5M2) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(base) + elem));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int i = 0; i < DMAX / 32; i++)
-        if (lane + 32 * i < p.d) s += qv[i] * cache_value<F16, KV>(p.k, e + lane + 32 * i);
+    for (int i = 0; i < 8; i++) {
+      const uint32_t h = fp8x2_to_f16x2<KV>((w[i / 2] >> (16 * (i & 1))) & 0xFFFFu);
+      f[2 * i] = to_f32<true>((uint16_t)h);
+      f[2 * i + 1] = to_f32<true>((uint16_t)(h >> 16));
+    }
+  } else {
+    const uint4 *at = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(base) + elem);
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-      s *= s2;
-      const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.0f : mn;
-      const float keep = exp2f(m - base), w = exp2f(s - base);
-      m = mn;
-      l = l * keep + w;
-      if (l != l) {            // a score is NaN, or +inf: so is every output
+    for (int k = 0; k < 2; k++) {
+      const uint4 v = __ldg(at + k);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int i = 0; i < DMAX / 32; i++) o[i] = l;
-        m_out = m;
-        l_out = l;
-        return;
+      for (int i = 0; i < 4; i++) {
+        f[8 * k + 2 * i] = to_f32<F16>((uint16_t)w[i]);
+        f[8 * k + 2 * i + 1] = to_f32<F16>((uint16_t)(w[i] >> 16));
       }
-#pragma unroll
-      for (int i = 0; i < DMAX / 32; i++)
-        if (lane + 32 * i < p.d) o[i] = o[i] * keep + w * cache_value<F16, KV>(p.v, e + lane + 32 * i);
     }
   }
-  m_out = m;
-  l_out = l;
+}
+
+// A segment: request r with rows from `start` of q and positions from `first`,
+// key/value head h, rows of the request from row0 on, key tiles [t0, t1).
+template <int BN>
+struct SegmentRows {
+  int r, start, first, h, row0;
+  Tiles<BN> tiles;
+  int t0, t1;
+};
+
+// Rows `row` of a segment (-1: none) over their visible keys, 32 keys at a
+// time: a lane has a key's scores, then dims lane, lane + 32, ... of the outputs.
+// Gives the maxima (log2 units), the sums, and the unnormalised outputs. The
+// `deadline` of the other roles' waits, if any, moves on at every tile.
+template <bool F16, int KV, int DMAX, int BN>
+__device__ __noinline__ void careful_rows(const AttnParams &params, const SegmentRows<BN> &segment, const int (&row)[CAREFUL],
+                                          volatile uint64_t *deadline, float (&m)[CAREFUL], float (&l)[CAREFUL],
+                                          float (&o)[CAREFUL][DMAX / 32]) {
+  const AttnParams p = params;                            // in registers
+  const SegmentRows<BN> sg = segment;
+  constexpr int N = DMAX / 32, AT = N > 4 ? 4 : 8;        // keys whose V is in flight
+  const int lane = threadIdx.x & 31;
+  const float s2 = p.scale_log2 * (p.ks ? __ldg(p.ks + p.ks_step * sg.h) : 1.0f);
+  int64_t q_at[CAREFUL];
+  int pos[CAREFUL];
+  uint32_t dead = 0;                                      // rows with a score of NaN or +inf: every output is NaN
+#pragma unroll
+  for (int x = 0; x < CAREFUL; x++) {
+    const int qr = sg.row0 + max(row[x], 0), tok = qr / p.group;
+    q_at[x] = (int64_t)(sg.start + tok) * p.q_tok + (int64_t)(sg.h * p.group + qr - tok * p.group) * p.q_head;
+    pos[x] = row[x] < 0 ? -1 : sg.first + tok;
+    m[x] = -INFINITY;
+    l[x] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) o[x][i] = 0.0f;
+  }
+#pragma unroll 1
+  for (int t = sg.t0; t < sg.t1; t++) {
+    if (deadline && lane == 0) *deadline = now_ns() + WAIT_NS;
+#pragma unroll 1
+    for (int j0 = 0; j0 < BN; j0 += 32) {
+      const int j = sg.tiles.at(t) * BN + j0 + lane;
+      bool see[CAREFUL], any = false;
+#pragma unroll
+      for (int x = 0; x < CAREFUL; x++) any |= see[x] = visible(p, j, pos[x]);
+      const int64_t off = any ? slot_offset(p, sg.r, j) : -1, e = off + (int64_t)sg.h * p.s_head;
+      const uint32_t there = __ballot_sync(~0u, off >= 0);
+      if (!there) continue;
+      float s[CAREFUL] = {};
+      if (off >= 0) {
+#pragma unroll 2
+        for (int d = 0; d < p.d; d += 16) {
+          float k[16];
+          load16<F16, KV>(p.k, e + d, k);
+#pragma unroll
+          for (int x = 0; x < CAREFUL; x++) {
+            float y[16];
+            load16<F16, F16 ? FP8B200_F16 : FP8B200_BF16>(p.q, q_at[x] + d, y);
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[x] = fmaf(y[i], k[i], s[x]);
+          }
+        }
+      }
+      float w[CAREFUL];
+      uint32_t sees[CAREFUL];
+#pragma unroll
+      for (int x = 0; x < CAREFUL; x++) {
+        see[x] = see[x] && off >= 0;
+        sees[x] = __ballot_sync(~0u, see[x]);
+        s[x] = see[x] ? s[x] * s2 : -INFINITY;
+        if (__any_sync(~0u, !(s[x] < INFINITY))) dead |= 1u << x;
+        float top = fmaxf(m[x], s[x]);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+        const float base = top == -INFINITY ? 0.0f : top, keep = exp2f(m[x] - base);
+        w[x] = see[x] ? exp2f(s[x] - base) : 0.0f;
+        m[x] = top;
+        float sum = w[x];
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        l[x] = l[x] * keep + sum;
+#pragma unroll
+        for (int i = 0; i < N; i++) o[x][i] *= keep;
+      }
+#pragma unroll 1
+      for (int k0 = 0; k0 < 32; k0 += AT) {
+        if (!((there >> k0) & ((1u << AT) - 1u))) continue;
+        float v[AT][N];
+#pragma unroll
+        for (int k = 0; k < AT; k++) {
+          const int64_t ek = __shfl_sync(~0u, e, k0 + k);
+#pragma unroll
+          for (int i = 0; i < N; i++) {
+            v[k][i] = 0.0f;
+            if (((there >> (k0 + k)) & 1u) && lane + 32 * i < p.d) v[k][i] = cache_value<F16, KV>(p.v, ek + lane + 32 * i);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < AT; k++)
+#pragma unroll
+          for (int x = 0; x < CAREFUL; x++) {
+            const float wk = __shfl_sync(~0u, w[x], k0 + k);
+            if ((sees[x] >> (k0 + k)) & 1u)               // a value that the row does not see is not touched
+#pragma unroll
+              for (int i = 0; i < N; i++) o[x][i] = fmaf(wk, v[k][i], o[x][i]);
+          }
+      }
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < CAREFUL; x++)
+    if ((dead >> x) & 1u) {
+      l[x] = u2f(0x7FC00000u);
+#pragma unroll
+      for (int i = 0; i < N; i++) o[x][i] = u2f(0x7FC00000u);
+    }
+}
+
+// The rows of a warp's lanes, `row` of the segment: `odd` for the rows to be
+// looked at, l their sum of weights. The rows' results lie in p.out (whole) or
+// in the segment's part of mr rows; other lanes' stores of them are ordered
+// before the call.
+template <bool F16, int KV, int DP, int BN>
+__device__ __noinline__ void odd_rows(const AttnParams &params, const SegmentRows<BN> &segment, int row, bool odd, float l, bool whole,
+                                      float *part, int mr, volatile uint64_t *deadline) {
+  const AttnParams p = params;                            // in registers
+  const SegmentRows<BN> sg = segment;
+  constexpr int N = DP / 32, AT = 8;
+  constexpr int ESZ = KV == FP8B200_E4M3 || KV == FP8B200_E5M2 ? 1 : 2;
+  const int lane = threadIdx.x & 31;
+  odd = odd && l == l;                                    // a NaN among the visible scores: so is every output, and stays it
+  const uint32_t rows = __ballot_sync(~0u, odd);
+  if (!rows) return;
+  const int tok = (sg.row0 + row) / p.group, pos = odd ? sg.first + tok : -1;
+  int last = pos;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) last = max(last, __shfl_xor_sync(~0u, last, d));
+  // a row whose weights are all 0 saw nothing, or scores of -inf alone: value by value
+  uint32_t redo = __ballot_sync(~0u, odd && l == 0.0f);
+  // bit q: in the row of lane q, a visible key holds NaN, +inf, -inf in this lane's dim i
+  uint32_t nan[N], up[N], down[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) nan[i] = up[i] = down[i] = 0u;
+  const int upr = p.d * ESZ / 16;                         // 16-byte units of a key's row
+  const int key_first = lane / upr, cu_first = lane % upr, key_step = 32 / upr, cu_step = 32 % upr;
+  bool done = false;
+#pragma unroll 1
+  for (int t = sg.t0; t < sg.t1 && !done; t++) {
+    if (deadline && lane == 0) *deadline = now_ns() + WAIT_NS;
+#pragma unroll 1
+    for (int j0 = 0; j0 < BN && !done; j0 += 32) {
+      const int j = sg.tiles.at(t) * BN + j0 + lane;
+      const int64_t off = j <= last ? slot_offset(p, sg.r, j) : -1, e = off + (int64_t)sg.h * p.s_head;
+      const uint32_t there = __ballot_sync(~0u, off >= 0);
+      if (!there) continue;
+      // units lane, lane + 32, ... of the 32 keys' rows
+      uint32_t found = 0;
+      int key = key_first, cu = cu_first;
+#pragma unroll 1
+      for (int k0 = 0; k0 < upr; k0 += AT) {
+        uint4 v[AT];
+        int keys[AT];
+#pragma unroll
+        for (int k = 0; k < AT; k++) {
+          keys[k] = key;
+          const int64_t ek = __shfl_sync(~0u, e, key & 31);
+          v[k] = make_uint4(0, 0, 0, 0);
+          if (k0 + k < upr && ((there >> (key & 31)) & 1u)) v[k] = __ldg(reinterpret_cast<const uint4 *>(p.v + ek * ESZ) + cu);
+          key += key_step;
+          cu += cu_step;
+          if (cu >= upr) cu -= upr, key++;
+        }
+#pragma unroll
+        for (int k = 0; k < AT; k++)
+          if (odd16<F16, KV>(v[k])) found |= 1u << (keys[k] & 31);
+      }
+      found = __reduce_or_sync(~0u, found);
+      for (; found; found &= found - 1) {
+        const int src = __ffs(found) - 1, jk = __shfl_sync(~0u, j, src);
+        const int64_t ek = __shfl_sync(~0u, e, src);
+        const uint32_t see = __ballot_sync(~0u, odd && visible(p, jk, pos));
+        if (!see) continue;
+        bool k_odd = false;                               // then the score may be -inf and the weight 0: value by value
+        float v[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+          v[i] = 0.0f;
+          if (lane + 32 * i < p.d) {
+            v[i] = cache_value<F16, KV>(p.v, ek + lane + 32 * i);
+            k_odd |= !(fabsf(cache_value<F16, KV>(p.k, ek + lane + 32 * i)) < INFINITY);
+          }
+        }
+        if (__any_sync(~0u, k_odd)) {
+          redo |= see;
+          continue;
+        }
+        bool all = true;                                  // NaN in every dim of every row: nothing changes that
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+          if (v[i] != v[i]) nan[i] |= see;
+          else if (v[i] == INFINITY) up[i] |= see;
+          else if (v[i] == -INFINITY) down[i] |= see;
+          all &= lane + 32 * i >= p.d || (nan[i] & rows) == rows;
+        }
+        done = __all_sync(~0u, all);
+        if (done) break;
+      }
+    }
+  }
+  const float vs = ESZ == 1 && p.vs ? __ldg(p.vs + p.vs_step * sg.h) : 1.0f;
+  auto out_at = [&](int row_s) {
+    const int qr = sg.row0 + row_s, t = qr / p.group;
+    return p.out + (int64_t)(sg.start + t) * p.o_tok + (int64_t)(sg.h * p.group + qr - t * p.group) * p.o_head;
+  };
+  // The row of lane src: its dims that are settled get their value; true if it has others that are not finite.
+  auto settled = [&](int src, int i) { return !((redo >> src) & 1u) && (((nan[i] | up[i] | down[i]) >> src) & 1u); };
+  auto value = [&](int src, int i) {
+    const bool n = (nan[i] >> src) & 1u, u = (up[i] >> src) & 1u, b = (down[i] >> src) & 1u;
+    return n || (u && b) ? u2f(0x7FC00000u) : u ? INFINITY : -INFINITY;
+  };
+  uint32_t again = 0;
+#pragma unroll 1
+  for (uint32_t rest = rows; rest; rest &= rest - 1) {
+    const int src = __ffs(rest) - 1, row_s = __shfl_sync(~0u, row, src);
+    const float l_s = __shfl_sync(~0u, l, src), inv = l_s == 0.0f ? 0.0f : vs / l_s;
+    uint16_t *os = out_at(row_s);
+    bool left = false;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int d = lane + 32 * i;
+      if (d >= p.d || fabsf(whole ? to_f32<F16>(os[d]) : part[row_s * DP + d]) < INFINITY) continue;
+      if (!settled(src, i)) left = true;
+      else if (whole) os[d] = (uint16_t)pack2<F16>(value(src, i) * inv, 0.0f);
+      else part[row_s * DP + d] = value(src, i);
+    }
+    if (__any_sync(~0u, left)) again |= 1u << src;
+  }
+#pragma unroll 1
+  while (again) {
+    int src[CAREFUL], row_s[CAREFUL];
+    float m[CAREFUL], ls[CAREFUL], o[CAREFUL][N];
+#pragma unroll
+    for (int x = 0; x < CAREFUL; x++) {
+      src[x] = __ffs(again) - 1;
+      row_s[x] = src[x] < 0 ? -1 : __shfl_sync(~0u, row, src[x]);
+      again &= again - 1;
+    }
+    careful_rows<F16, KV, DP, BN>(params, segment, row_s, deadline, m, ls, o);
+#pragma unroll
+    for (int x = 0; x < CAREFUL; x++) {
+      if (src[x] < 0) continue;
+      const float inv = ls[x] == 0.0f ? 0.0f : vs / ls[x];
+      uint16_t *os = out_at(row_s[x]);
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const int d = lane + 32 * i;
+        const float y = settled(src[x], i) ? value(src[x], i) : o[x][i];
+        if (!whole) part[row_s[x] * DP + d] = y;
+        else if (d < p.d) os[d] = (uint16_t)pack2<F16>(y * inv, 0.0f);
+      }
+      if (!whole && lane == 0) {
+        part[mr * DP + row_s[x]] = m[x];
+        part[mr * DP + mr + row_s[x]] = ls[x];
+      }
+    }
+  }
 }
 
 // Joins the parts of the segments that were cut: block c the one that began

@@ -69,9 +69,6 @@ constexpr int SEG_COST = 2;       // what a segment's start and end cost, in key
 constexpr int MAX_REQUESTS = 16384;  // their first rows pass through shared memory
 constexpr int SEGS = 4;           // segments in the ring
 constexpr int HIDE_RING = 8;     // tiles whose page masks are kept: more than the producers run ahead of the softmax
-// Long: a group that recomputes rows value by value (careful_row) over a long
-// segment keeps the other roles waiting for a second or more.
-constexpr unsigned long long WAIT_NS = 10000000000ull;
 
 __device__ uint32_t g_paged_status;  // 0, or the site of a wait that ran out
 
@@ -117,11 +114,6 @@ struct Tc {
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
 
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
@@ -139,15 +131,17 @@ __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Bounded: a wait that runs out records its site, tells the CTA's other roles
-// (s_failed) and holds its thread for 200 us so that copies and MMAs issued
+// Bounded: a wait runs out at the CTA's deadline (behind s_failed), which moves on
+// with every key tile of the first softmax group, and with every tile where odd_rows
+// keeps the other roles waiting (a wait with a clock of its own takes more code at
+// each of its places: 8 x 2048 324 us against 307). It then records its site, tells
+// the other roles (s_failed) and holds its thread for 200 us so that copies and MMAs issued
 // before it have landed when the CTA tears down.
 __device__ __forceinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile uint32_t *s_failed, uint32_t site) {
-  const uint64_t t0 = now_ns();
   for (uint32_t n = 1;; n++) {
     if (bar_test(bar, parity)) return true;
     if ((n & 31u) == 0) {
-      const bool late = now_ns() - t0 > WAIT_NS;
+      const bool late = now_ns() > *reinterpret_cast<volatile uint64_t *>(s_failed + 1);
       if (late || *s_failed) {
         if (late) {
           *s_failed = 1;
@@ -362,8 +356,9 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
   uint32_t *s_hide = reinterpret_cast<uint32_t *>(smem + C::OFF_HIDE);    // [HIDE_RING][4]
   const uint32_t bars = base_a + C::OFF_BARS;
   Segment *s_seg = reinterpret_cast<Segment *>(smem + C::OFF_SEGS);
-  uint32_t *s_misc = reinterpret_cast<uint32_t *>(smem + C::OFF_SEGS + SEGS * 48);  // tensor memory base, failed flag
+  uint32_t *s_misc = reinterpret_cast<uint32_t *>(smem + C::OFF_SEGS + SEGS * 48);  // tensor memory base, failed flag, deadline (64 bits)
   volatile uint32_t *s_failed = s_misc + 1;
+  volatile uint64_t *s_deadline = reinterpret_cast<volatile uint64_t *>(s_misc + 2);
   auto kv_full = [&](int s) { return bars + 8u * s; };
   auto kv_empty = [&](int s) { return bars + 8u * (C::SLOTS + s); };
   auto raw_full = [&](int s) { return bars + 8u * (2 * C::SLOTS + s); };
@@ -416,6 +411,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
     fence_async();  // Q and K arrive over it through TMA
   }
   if (tid < 2) s_found[tid][0] = -1;
+  if (tid == 0) *s_deadline = now_ns() + WAIT_NS;
   __syncthreads();
   const int places = p.requests == 0 ? 0 : place(p, min(max(__ldg(p.cu + p.requests), 0), p.tokens), p.requests);
   auto request_of = [&](int x) {
@@ -911,6 +907,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
         tst_wait();
         fence_before();
         bar_arrive(p_full + 8 * g);
+        if (tid == 0) *s_deadline = now_ns() + WAIT_NS;
         const float2 a2 = add2(acc[0], acc[1]);
         sum += a2.x + a2.y;
         tiles++;
@@ -992,29 +989,10 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
         part[QB * DP + brow] = mine_base;
         part[QB * DP + QB + brow] = sum;
       }
-      uint32_t redo = __ballot_sync(~0u, odd);             // see careful_row
-      while (redo) {
-        const int src = __ffs(redo) - 1;
-        redo &= redo - 1;
-        const int tok_s = __shfl_sync(~0u, tok, src), head_s = __shfl_sync(~0u, head, src), brow_s = __shfl_sync(~0u, brow, src);
-        float m, l, ov[DP / 32];
-        __syncwarp();
-        careful_row<F16, KV, DP, KT>(p, sg->r, sg->start + tok_s, head_s, first + tok_s, sg->tiles(), t_begin, t_end, m, l, ov);
-        const float li = l == 0.0f ? 0.0f : vs / l;
-        uint16_t *os = p.out + (int64_t)(sg->start + tok_s) * p.o_tok + (int64_t)head_s * p.o_head;
-#pragma unroll
-        for (int i = 0; i < DP / 32; i++) {
-          const int d = lane + 32 * i;
-          if (whole) {
-            if (d < p.d) os[d] = (uint16_t)pack2<F16>(ov[i] * li, 0.0f);
-          } else {
-            part[brow_s * DP + d] = ov[i];
-          }
-        }
-        if (!whole && lane == 0) {
-          part[QB * DP + brow_s] = m;
-          part[QB * DP + QB + brow_s] = l;
-        }
+      if (__any_sync(~0u, odd)) {
+        __syncwarp();                                      // the rows' stores, by other lanes too
+        const SegmentRows<KT> rows{sg->r, sg->start, first, h, sg->qt * QB, sg->tiles(), t_begin, t_end};
+        odd_rows<F16, KV, DP, KT>(p, rows, brow, odd, sum, whole, part, QB, s_deadline);
       }
       __syncwarp();
       if (lane == 0) bar_arrive(seg_empty + 8 * (segs % SEGS));
