@@ -201,10 +201,10 @@ __device__ __forceinline__ Share find_share(const AttnParams &p, long long *s_sc
 // bf16 rows of s_q to f16 with the largest value in [1, 2); `flip` changes the
 // signs (a negative scale: the maximum of the products is then that of the
 // scores). Rows are shared by the block's warps.
-template <bool TO_F16, int DP>
+template <bool TO_F16, int DP, int NW = 4>
 __device__ __forceinline__ void normalise_rows(uint8_t *s_q, int qrow, int rows, float *s_qscale, uint32_t flip) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int row = warp; row < rows; row += 4) {
+  for (int row = warp; row < rows; row += NW) {
     uint32_t *w = reinterpret_cast<uint32_t *>(s_q + row * qrow);
     if constexpr (TO_F16) {
       float a = 0.0f;
@@ -667,8 +667,8 @@ struct Cfg {
   static constexpr int CPR = ROWB / 16;                 // 16-byte units of it
   static constexpr int TILE = BN * ROWB;                // K or V
   // two blocks an SM (head size 256: one), the more bytes in flight the better
-  static constexpr int STAGES = FP8 ? (DP == 64 ? 8 : DP == 128 ? (RW == 4 ? 5 : 6) : 4)
-                                    : (DP == 64 ? 6 : DP == 128 ? (RW == 4 ? 2 : 3) : 2);
+  static constexpr int STAGES = FP8 ? (DP == 64 ? 8 : DP == 128 ? 5 : 4)
+                                    : (DP == 64 ? 6 : 2);
   static constexpr int MR = 16 * RW;                    // rows a block
   static constexpr int KW = NW / RW;                    // warps that share a tile's keys
   static constexpr int WN = BN / KW;                    // keys a warp
@@ -835,19 +835,7 @@ __global__ void __launch_bounds__(NW * 32, DP == 256 ? 1 : 2) paged_attention_ke
       cp_commit();
     }
     if constexpr (C::FP8 && !F16) {           // bf16 rows to f16, the largest value in [1, 2)
-      for (int row = warp; row < C::MR; row += NW) {
-        uint32_t *w = reinterpret_cast<uint32_t *>(s_q + row * C::QROW);
-        float a = 0.0f;
-        for (int i = lane; i < DP / 2; i += 32)
-          a = fmaxf(a, fmaxf(fabsf(u2f(w[i] << 16)), fabsf(u2f(w[i] & 0xFFFF0000u))));
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) a = fmaxf(a, __shfl_xor_sync(~0u, a, d));
-        uint32_t eb = f2u(a) >> 23;
-        eb = (eb == 255u || a == 0.0f) ? 127u : min(max(eb, 1u), 253u);
-        const float mul = u2f((254u - eb) << 23);
-        for (int i = lane; i < DP / 2; i += 32) w[i] = pack2<true>(u2f(w[i] << 16) * mul, u2f(w[i] & 0xFFFF0000u) * mul);
-        if (lane == 0) s_qscale[row] = u2f(eb << 23);
-      }
+      normalise_rows<true, DP, NW>(s_q, C::QROW, C::MR, s_qscale, 0u);
       __syncthreads();
     }
     const int wr = rw * 16;                   // this warp's first row in the tile

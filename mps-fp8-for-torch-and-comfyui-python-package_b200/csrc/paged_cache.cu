@@ -10,10 +10,7 @@
 //                       the cache
 //
 // No counterpart in the reference, which has no cache of any kind.
-#include "common.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include "paged_attention.cuh"
 
 #include <algorithm>
 #include <atomic>
@@ -364,21 +361,6 @@ auto rope_write(bool full) {
   return full ? rope_write_kernel<F16, CACHE, 4> : rope_write_kernel<F16, CACHE, 2>;
 }
 
-template <typename P>
-cudaError_t launch_pdl(void (*kernel)(P), int grid, int threads, int smem, cudaStream_t st, const P &p) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 }  // namespace
 }  // namespace paged
 }  // namespace fp8b200
@@ -417,7 +399,7 @@ int launch_slots(const char *what, const int32_t *cached_lens, const int32_t *ne
   SlotsParams p{cached_lens, new_lens, (int)requests, block_table, table_ld, (int)table_cols, free_pages, n_free,
                 free_head, (int)page_size, (int)tokens, cu_new, kv_lens, positions, slots, free_head_out, held, held_out};
   const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((tokens + SL_THREADS - 1) / SL_THREADS, current_sm_count()));
-  launch_pdl(slots_kernel<HELD>, grid, SL_THREADS, smem, (cudaStream_t)stream, p);
+  launch_dependent(slots_kernel<HELD>, dim3((unsigned)grid), SL_THREADS, smem, (cudaStream_t)stream, p);
   count_launch();
   return check_launch(what);
 }
@@ -496,7 +478,7 @@ extern "C" int fp8b200_rope_write_paged(const void *qkv, int dtype, int64_t toke
   if (cache_dtype == FP8B200_E4M3) kernel = f16 ? rope_write<true, FP8B200_E4M3>(full) : rope_write<false, FP8B200_E4M3>(full);
   else if (cache_dtype == FP8B200_E5M2) kernel = f16 ? rope_write<true, FP8B200_E5M2>(full) : rope_write<false, FP8B200_E5M2>(full);
   else kernel = f16 ? rope_write<true, FP8B200_F16>(full) : rope_write<false, FP8B200_BF16>(full);
-  launch_pdl(kernel, grid, RW_THREADS, 0, (cudaStream_t)stream, p);
+  launch_dependent(kernel, dim3((unsigned)grid), RW_THREADS, 0, (cudaStream_t)stream, p);
   count_launch();
   return check_launch("rope_write_paged");
 }
