@@ -14,13 +14,15 @@ Additions beyond the reference (used by the aten overrides in ops.py):
 `quantize_fp8`, `fp4_decode` (shape-preserving, any float dtype, f32
 scale), `scaled_mm` with torch._scaled_mm's full argument set,
 `fp4_scaled_mm` (packed FP4 operands multiplied on the tensor cores), and the
-paged key/value-cache operators of paged.py.
+paged key/value-cache operators of paged.py (`paged_status`: whether a wait of
+their kernels ever ran out).
 """
 from __future__ import annotations
 
 import torch
 
 from . import _lib as L
+from ._lib import paged_status  # noqa: F401
 from .paged import PagedKVCache, PagedStep, paged_attention, paged_slots, rope_write_paged  # noqa: F401
 
 _FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
