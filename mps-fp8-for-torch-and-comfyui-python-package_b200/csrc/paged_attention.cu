@@ -4,9 +4,9 @@
 //   o_i = sum_j softmax_j(scale * q_i . k_j) v_j   over the keys j <= p_i with
 //         p_i - j < window or j < sinks            (no window: all j <= p_i)
 //
-// Two kernels of blocks of four warps, for few query rows a request
-// (paged_few_kernel) and for more (paged_attention_kernel); chunks and prompts
-// go to paged_attention_tc.cu where it serves. The query heads that share a
+// Two kernels, for few query rows a request (paged_few_kernel, blocks of four
+// warps) and for more (paged_attention_kernel, four warps, eight at head sizes
+// above 128); chunks and prompts go to paged_attention_tc.cu where it serves. The query heads that share a
 // key/value head are rows of one tile: row token * group + g.
 //
 // Work: a segment is one row tile of one request under one key/value head;
@@ -240,7 +240,8 @@ __device__ __forceinline__ void normalise_rows(uint8_t *s_q, int qrow, int rows,
 // Measured, 64 decodes of up to 32768 cached tokens, 32 / 8 heads of 128, e4m3
 // (1.90 GB of cache, 290 us at the measured copy rate): 572 us with one block
 // barrier a tile and 16-row tiles, 470 us with a ring a warp, 424 us turned
-// around, 402 us (355 us in bursts of 50) with a line of work a head; before
+// around, 402 us with a line of work a head, 389 us (338 us in a graph) since the
+// segment's end no longer holds a row's recomputation; before
 // the kernels' shared-memory carve-out was fixed an SM could take one block of
 // three after a kernel without shared memory (672 us). 24 requests of 5 tokens,
 // 16 / 2 heads of 64, e5m2, up to 8000 cached: 35 us, of which about 16 are the
@@ -654,8 +655,8 @@ __global__ void __launch_bounds__(THREADS, (Few<F16, KV, DP, NG>::PER_SM)) paged
 // takes 16 rows; with fewer than 16 NW rows NW / RW warps share the tile's keys.
 // Head sizes up to 128: four warps, two blocks an SM. Above, where one block
 // fills the SM: eight warps, since four, one a scheduler, wait on each
-// instruction: 1073 rows of 8 heads over up to 2408 keys 182 -> 138 us in e4m3,
-// 111 us in bf16; 88 rows a request, 10 over 19531 keys in f16 183 -> 142 us. A
+// instruction: 1073 rows of 8 heads over up to 2408 keys 182 -> 138 us in e4m3
+// (127 now, 105 in bf16); 88 rows a request, 10 over 19531 keys in f16 183 -> 142 us. A
 // tile of 128 rows by 64 keys takes 5 to 6 us: 2 us of warp-level MMA, as much
 // of shared-memory reads (each warp reads all of K and V), little overlapped.
 template <bool F16, int KV, int DP, int RW, int NW>
@@ -1157,7 +1158,16 @@ int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 // Requests with more query rows than TC_OVER (tokens x group) go to the
 // tensor-memory kernel when the longest has more than TC_FROM and the head
-// size is at most 128.
+// size is at most 128. Both sides, in graphs, this file's kernel -> that one:
+//   96 rows, 24 requests x 24 tokens over 4000 keys, 32 / 8 heads of 128, bf16: 247 -> 115 us
+//   64 rows, 24 x 16: 141 -> 113 us; 1 x 16 over 2000: 25.9 -> 20.6 us
+//   36 rows, 24 x 9: 130 -> 110 us; 20 rows, 24 x 5 in e4m3: 94 -> 117 us
+//   96 rows, 24 x 12, 16 / 2 heads of 64: 53 -> 36 us; 1 x 12 over 30000: 33.5 -> 49.3 us
+//   48 rows, 24 x 6, 16 / 2 heads of 64: 39.2 -> 35.0 us; 1 x 6 over 2000: 18.0 -> 18.5 us
+// so 64 suits the small head sizes; at 128 the limit lies near 32.
+// Beside a chunk of 512 rows over 2000 keys, short requests there:
+//   32 rows, 16 x 8 over 4000, 32 / 8 heads of 128, bf16: 229 -> 113 us, e4m3 172 -> 129 us
+//   16 rows, 16 x 4: bf16 145 -> 112 us, e4m3 130 -> 129 us; 40 x 4 over 2000 in e4m3 143 -> 157 us
 static constexpr int64_t TC_FROM = 64, TC_OVER = 16;
 // Two parts a block (64 rows by two blocks an SM, 16 by four, ...: at most 128 rows an SM) and a descriptor.
 static int64_t paged_generic_workspace(int dp, int sms) { return (int64_t)sms * (2 * 128 * (int64_t)(dp + 2) * 4 + 4 * (int64_t)sizeof(fp8b200::paged::PartDesc)); }
@@ -1267,6 +1277,9 @@ extern "C" int fp8b200_paged_attention(const void *q, int dtype, int64_t q_strid
   if (int rc = launch_attributes((const void *)v.main, v.smem)) return rc;
   if (int rc = launch_attributes((const void *)v.merge, 0)) return rc;
   const int grid = current_sm_count() * v.per_sm;
+  // A line a head against one for all heads, in graphs: one decode of 30000 keys, 32 / 8 heads of 128, bf16 35 and 43 us, 64 of
+  // 4000 in e4m3 133 and 137 us; 32 heads of 128, one decode 87 and 91 us, 16 of 100 keys 26.8 and 25.1 us; 64 heads of 64, 64 of
+  // 4000 in e4m3 651 and 970 us, in bf16 1066 and 927 us. More heads than a quarter of the grid leave a line under four blocks.
   p.line_heads = v.few && n_kv_heads <= grid / 4 ? 1 : n_kv_heads;
   launch_dependent(v.main, dim3((unsigned)grid), v.threads, v.smem, (cudaStream_t)stream, p);
   p.blocks = grid;

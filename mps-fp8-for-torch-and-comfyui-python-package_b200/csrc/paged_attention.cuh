@@ -186,7 +186,7 @@ int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int s
 //      most the rows whose tiles hold the key and that do not see it.
 // 2048 rows of 32 / 8 heads of 128 over 16049 keys in bf16 (0.50 ms): 1.7 ms with
 // a NaN that all rows of one head see, 2.9 ms with one in each head; 78 ms with
-// one in the last key, which the last 256 rows of a head are recomputed for.
+// one in the last key, hidden from 252 rows of a head.
 constexpr int CAREFUL = 4;
 
 // An infinity or NaN among the 16 bytes of cached values.

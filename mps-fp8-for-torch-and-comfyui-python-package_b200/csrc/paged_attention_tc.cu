@@ -39,15 +39,18 @@
 // other's: 256 x 128 scores cost 2048 cycles of MMA at head size 128 and 2048
 // cycles of ex2 (16 a cycle), and take about 4100 (tensor pipe busy 49 % of the
 // time at 2048 rows over 14001 keys). Measured, 32 / 8 heads of 128: 2048 tokens
-// over 14001 cached in e4m3 512 us (985 TFLOP/s), prompts of 8 x 2048 in bf16
-// 351 us (783 TFLOP/s; short segments, so their starts and ends count), 1500
-// tokens with a window of 4096 and 4 sinks 142 us. SEG_COST of 2 gave 351 us on
-// the prompts, 3 gave 364. Tried and slower: two score buffers of 64 keys a row
-// tile (570 us against 540 then: N = 64 MMAs read A again for half the work),
-// two threads a row (the registers spill), part of the exponentials as a
-// polynomial on the multiply-add pipes (596 us against 540; issue slots are as
-// short as ex2), K and V through cp.async (a proxy fence waits for all of a
-// thread's copies) or four-row gathers.
+// over 14001 cached in e4m3 519 us (972 TFLOP/s), prompts of 8 x 2048 in bf16
+// 355 us (775 TFLOP/s; short segments, so their starts and ends count; 309 in a
+// graph), 1500 tokens with a window of 4096 and 4 sinks 144 us. SEG_COST of 2 gave
+// 351 us on the prompts, 3 gave 364. Slower when they were tried, on the kernel
+// whose MMAs still took 100 cycles to issue (540 us for the chunk then), and not
+// tried since: two score buffers of 64 keys a row tile (570 us), part of the
+// exponentials as a polynomial on the multiply-add pipes (596 us). Dropped for
+// good: two threads a row (the registers spill; the float8 forms here spill 272
+// to 296 bytes a thread themselves), K and V through cp.async (a proxy fence waits
+// for all of a thread's copies), four-row gathers. The time depends on the layout
+// of the code: variants of the page masks' few lines that do the same work took
+// 304 to 358 us on the prompts in a graph.
 //
 // No counterpart in the reference.
 #include "paged_attention.cuh"

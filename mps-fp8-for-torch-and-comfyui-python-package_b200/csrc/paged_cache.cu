@@ -5,7 +5,8 @@
 // tokens fill the pages its block-table row lists, in order.
 //
 //   slots_kernel        one step's page allotment and token placement from the
-//                       request lengths
+//                       request lengths, by itself or with the account that a
+//                       cache keeps of its pages (HELD)
 //   rope_write_kernel   rotary embedding of q and k, and k and v rounded into
 //                       the cache
 //

@@ -294,6 +294,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     max_new: the largest number of new tokens of one request, where the host
     knows it (it picks the kernels; a wrong value costs time, not results).
+    Without it, more than 64 rows (tokens x group) in all launch the kernels for
+    chunks too, with their workspace: give 1 for a step that only decodes.
     Scores, maxima, sums and outputs are float32, rounded once to q's type;
     see the kernels for the weights' type. A query that sees no key gives 0; a
     table entry outside the pool hides its keys; hidden keys' values, NaN
