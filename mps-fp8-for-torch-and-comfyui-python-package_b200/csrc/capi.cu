@@ -37,6 +37,7 @@ struct DevInfo {
 };
 DevInfo g_dev[kMaxDevices];
 thread_local int t_sms = 148;
+thread_local int t_current = -1;  // the device whose context this thread was seen to have current
 }  // namespace
 
 int check_device(int *device_out) {
@@ -58,6 +59,12 @@ int check_device(int *device_out) {
     return set_error(FP8B200_EDEVICE,
                      "device %d has compute capability %d.%d; this library is built for sm_100a (B200) only",
                      dev, d.major, d.minor);
+  if (t_current != dev) {
+    // a thread's first call may be one of the driver's (a tensor map), which does not bring the context up by itself
+    e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return set_error(FP8B200_EDEVICE, "device %d: %s", dev, cudaGetErrorString(e));
+    t_current = dev;
+  }
   t_sms = d.sms;
   if (device_out) *device_out = dev;
   return FP8B200_OK;
