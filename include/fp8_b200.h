@@ -366,6 +366,13 @@ int fp8b200_paged_attention(const void *q, int dtype, int64_t q_stride_token, in
 int fp8b200_paged_status(uint32_t *status_out, int reset);
 
 /*
+ * Test hook, for the calling host thread's later attention calls: no_tiles: in
+ * the tensor-memory kernel no tile of K and V arrives; wait_timeout_ns: how long
+ * after its last progress its waits run out (0: 10 s).
+ */
+int fp8b200_debug_paged(int no_tiles, unsigned long long wait_timeout_ns);
+
+/*
  * Device-side status of the scaled GEMM on the current device: 0 if no
  * bounded wait has timed out, else FP8B200_ETIMEOUT with *status_out holding
  * the site code of the last launch that timed out (that launch's output is

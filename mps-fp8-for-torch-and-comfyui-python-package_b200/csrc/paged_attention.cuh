@@ -45,6 +45,9 @@ struct AttnParams {
   float *part;
   PartDesc *desc;
   int blocks;                 // for the merge: how many descriptors there are
+  // the tensor-memory kernel: its waits run out that long after the last progress; test hook: no tile of K and V arrives
+  uint64_t wait_ns;
+  int no_tiles;
   int line_heads;             // key/value heads that a line of units holds: all, or one (a line a head)
 };
 
@@ -121,7 +124,6 @@ __device__ __forceinline__ int64_t slot_offset(const AttnParams &p, int r, int j
   return (int64_t)page * p.s_page + (int64_t)((uint32_t)j - col * (uint32_t)p.page) * p.s_slot;
 }
 
-constexpr uint64_t WAIT_NS = 10000000000ull;  // the tensor-memory kernel's waits run out that long after the last progress
 __device__ __forceinline__ uint64_t now_ns() {
   uint64_t t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -264,7 +266,7 @@ __device__ __noinline__ void careful_rows(const AttnParams &params, const Segmen
   }
 #pragma unroll 1
   for (int t = sg.t0; t < sg.t1; t++) {
-    if (deadline && lane == 0) *deadline = now_ns() + WAIT_NS;
+    if (deadline && lane == 0) *deadline = now_ns() + p.wait_ns;
 #pragma unroll 1
     for (int j0 = 0; j0 < BN; j0 += 32) {
       const int j = sg.tiles.at(t) * BN + j0 + lane;
@@ -374,7 +376,7 @@ __device__ __noinline__ void odd_rows(const AttnParams &params, const SegmentRow
   bool done = false;
 #pragma unroll 1
   for (int t = sg.t0; t < sg.t1 && !done; t++) {
-    if (deadline && lane == 0) *deadline = now_ns() + WAIT_NS;
+    if (deadline && lane == 0) *deadline = now_ns() + p.wait_ns;
 #pragma unroll 1
     for (int j0 = 0; j0 < BN && !done; j0 += 32) {
       const int j = sg.tiles.at(t) * BN + j0 + lane;

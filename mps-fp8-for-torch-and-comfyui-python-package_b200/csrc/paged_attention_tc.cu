@@ -414,7 +414,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
     fence_async();  // Q and K arrive over it through TMA
   }
   if (tid < 2) s_found[tid][0] = -1;
-  if (tid == 0) *s_deadline = now_ns() + WAIT_NS;
+  if (tid == 0) *s_deadline = now_ns() + p.wait_ns;
   __syncthreads();
   const int places = p.requests == 0 ? 0 : place(p, min(max(__ldg(p.cu + p.requests), 0), p.tokens), p.requests);
   auto request_of = [&](int x) {
@@ -622,7 +622,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
       // float8 tiles go to the raw ring, 16-bit ones straight to the operands' ring
       constexpr int RING = C::FP8 ? C::RAWS : C::SLOTS;
       uint32_t filled = 0, tiles = 0;
-      bool ok = true;
+      bool ok = !p.no_tiles;
       for (uint32_t segs = 0; ok; segs++) {
         const Segment *sg = seg_at(segs, 52);
         if (!__all_sync(~0u, sg != nullptr) || sg->r < 0) break;
@@ -910,7 +910,7 @@ __global__ void __launch_bounds__((Tc<F16, KV, DP>::THREADS), 1)
         tst_wait();
         fence_before();
         bar_arrive(p_full + 8 * g);
-        if (tid == 0) *s_deadline = now_ns() + WAIT_NS;
+        if (tid == 0) *s_deadline = now_ns() + p.wait_ns;
         const float2 a2 = add2(acc[0], acc[1]);
         sum += a2.x + a2.y;
         tiles++;
@@ -1042,6 +1042,10 @@ EncodeTiled encode_tiled() {
 
 }  // namespace
 
+constexpr uint64_t WAIT_NS = 10000000000ull;
+thread_local uint64_t g_wait_ns = WAIT_NS;
+thread_local int g_no_tiles = 0;
+
 // The attributes last as long as the process: set once a kernel and device.
 int launch_attributes(const void *kernel, int smem) {
   static std::mutex m;
@@ -1077,6 +1081,8 @@ int launch_tc(const AttnParams &params, bool f16, int cache_dtype, int dp, int s
   p.desc = (PartDesc *)workspace;
   p.part = (float *)(workspace + (int64_t)sms * sizeof(PartDesc));
   p.blocks = sms;
+  p.wait_ns = g_wait_ns;
+  p.no_tiles = g_no_tiles;
   const bool fp8 = cache_dtype == FP8B200_E4M3 || cache_dtype == FP8B200_E5M2;
   TcVariant v;
   if (cache_dtype == FP8B200_E4M3) v = f16 ? pick_tc<true, FP8B200_E4M3>(dp) : pick_tc<false, FP8B200_E4M3>(dp);
@@ -1136,4 +1142,11 @@ extern "C" int fp8b200_paged_status(uint32_t *status_out, int reset) {
   if (e != cudaSuccess) return set_error(FP8B200_ELAUNCH, "paged_status: %s", cudaGetErrorString(e));
   if (status_out) *status_out = s;
   return s ? set_error(FP8B200_ETIMEOUT, "paged_attention: a wait ran out (site %u)", s & 0x7FFFFFFFu) : FP8B200_OK;
+}
+
+extern "C" int fp8b200_debug_paged(int no_tiles, unsigned long long wait_timeout_ns) {
+  using namespace fp8b200::paged;
+  g_no_tiles = no_tiles ? 1 : 0;
+  g_wait_ns = wait_timeout_ns ? wait_timeout_ns : WAIT_NS;
+  return FP8B200_OK;
 }

@@ -72,6 +72,7 @@ def _declare(L):
         "fp8b200_paged_status": [ctypes.POINTER(ctypes.c_uint32), i32],
         "fp8b200_gemm_status": [ctypes.POINTER(ctypes.c_uint32), i32],
         "fp8b200_debug_gemm": [i32, ctypes.c_ulonglong],
+        "fp8b200_debug_paged": [i32, ctypes.c_ulonglong],
         "fp8b200_gemm_set_path": [i32],
     }
     for name, args in sigs.items():
